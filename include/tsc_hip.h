@@ -392,6 +392,46 @@ int tsc_rowdot_many(int n_terms, const float *const *a, const int64_t *a_stride,
 int tsc_project_features(const float *x, int64_t M, int d_in, const float *b_dec, const float *Pt,
                          const float *bias, int F, int apply_relu, float *out, tsc_stream_t stream);
 
+/*
+ * ---- the head of the language model: layer norm and the unembedding's cross entropy ----
+ *
+ * Element types of these entry points (elem / param_elem): what the pointers behind `void *` hold.
+ */
+#define TSC_ELEM_F32 0
+#define TSC_ELEM_BF16 1
+#define TSC_ELEM_F16 2
+
+/* Rows in device memory: row r starts `(r / inner) * outer_stride + (r % inner) * inner_stride` elements behind data, and
+ * its elements are neighbours.  A dense [M, D] matrix: inner = 1, both strides D; x[:, :-1] of a dense [B, T, D] tensor:
+ * inner = T - 1, strides T * D and D; an expanded row: strides 0.  inner >= 1; data aligned to its element. */
+typedef struct tsc_rows {
+    const void *data;
+    int64_t inner, outer_stride, inner_stride;
+} tsc_rows_t;
+
+/*
+ * Layer norm of `rows` rows of `width` elements:
+ *   mean = sum(x) / width,  scale = sqrt(sum((x - mean)^2) / width + eps),  y = (x - mean) / scale * weight + bias.
+ * y [rows, width] dense, in x's type; mean and scale [rows] fp32 (scale is what TransformerLens hooks as `hook_scale`:
+ * the divisor).  weight, bias [width] in param_elem or NULL (1 and 0: a model whose layer norms are folded, the
+ * LayerNormPre of the model behind load_model_and_encoders.py:21).  Statistics are fp32 for every type; y is rounded once.
+ */
+int tsc_layer_norm(int elem, const tsc_rows_t *x, int64_t rows, int width, const void *weight, const void *bias,
+                   int param_elem, float eps, void *y, float *mean, float *scale, tsc_stream_t stream);
+
+/*
+ * Its backward pass from the kept mean and scale [rows] fp32:
+ *   dn = dy * weight,  xh = (x - mean) / scale,  dx = (dn - sum(dn) / width - xh * sum(dn * xh) / width) / scale,
+ *   dweight = sum over rows of dy * xh,  dbias = sum over rows of dy.
+ * dx [rows, width] dense in x's type (dy has that type too); dweight, dbias [width] in param_elem, each or both NULL = not
+ * wanted.  workspace: tsc_layer_norm_workspace_bytes(rows, width) bytes, needed only with dweight or dbias; its contents
+ * need not survive the call.  Sums are fp32 in a fixed order: the same call gives the same bits.
+ */
+size_t tsc_layer_norm_workspace_bytes(int64_t rows, int width);
+int tsc_layer_norm_backward(int elem, const tsc_rows_t *dy, const tsc_rows_t *x, const float *mean, const float *scale,
+                            int64_t rows, int width, const void *weight, int param_elem, void *dx, void *dweight,
+                            void *dbias, void *workspace, size_t workspace_bytes, tsc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

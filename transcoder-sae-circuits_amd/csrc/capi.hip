@@ -568,4 +568,56 @@ int tsc_project_features(const float *x, int64_t M, int d_in, const float *b_dec
     return tsc_launch_project(x, M, d_in, b_dec, Pt, bias, F, apply_relu, out, (hipStream_t)stream);
 }
 
+// ---- the language model's head -----------------------------------------------------------------------------
+static int elem_size(int elem) { return elem == TSC_ELEM_F32 ? 4 : elem == TSC_ELEM_BF16 || elem == TSC_ELEM_F16 ? 2 : 0; }
+
+static int check_rows(const tsc_rows_t *r, int elem, int64_t rows, const char *name) {
+    if (!r) return tsc_fail(TSC_ERR_ARG, "null %s", name);
+    if (rows > 0 && !r->data) return tsc_fail(TSC_ERR_ARG, "null %s pointer", name);
+    if (r->inner < 1 || r->inner_stride < 0 || r->outer_stride < 0)
+        return tsc_fail(TSC_ERR_ARG, "%s: inner %lld, strides %lld and %lld", name, (long long)r->inner,
+                        (long long)r->outer_stride, (long long)r->inner_stride);
+    if ((uintptr_t)r->data % elem_size(elem)) return tsc_fail(TSC_ERR_ARG, "%s is not aligned to its elements", name);
+    return TSC_OK;
+}
+
+static int check_norm(int elem, int param_elem, int64_t rows, int width) {
+    if (!elem_size(elem)) return tsc_fail(TSC_ERR_ARG, "unknown element type %d", elem);
+    if (!elem_size(param_elem)) return tsc_fail(TSC_ERR_ARG, "unknown parameter element type %d", param_elem);
+    if (rows < 0 || width < 1) return tsc_fail(TSC_ERR_ARG, "layer norm of %lld rows of %d elements", (long long)rows, width);
+    if (width > (1 << 24)) return tsc_fail(TSC_ERR_UNSUPPORTED, "layer norm rows of %d elements (at most 2^24)", width);
+    return TSC_OK;
+}
+
+int tsc_layer_norm(int elem, const tsc_rows_t *x, int64_t rows, int width, const void *weight, const void *bias,
+                   int param_elem, float eps, void *y, float *mean, float *scale, tsc_stream_t stream) {
+    int rc = check_norm(elem, param_elem, rows, width);
+    if (!rc) rc = check_rows(x, elem, rows, "x");
+    if (rc) return rc;
+    if (!(eps >= 0.f)) return tsc_fail(TSC_ERR_ARG, "eps must not be negative");
+    if (rows == 0) return TSC_OK;
+    if (!y || !mean || !scale) return tsc_fail(TSC_ERR_ARG, "null output pointer");
+    return tsc_launch_layer_norm(elem, *x, rows, width, weight, bias, param_elem, eps, y, mean, scale, (hipStream_t)stream);
+}
+
+size_t tsc_layer_norm_workspace_bytes(int64_t rows, int width) {
+    return rows < 1 || width < 1 ? 0 : 2 * sizeof(float) * tsc_layer_norm_parts(rows) * (size_t)width;
+}
+
+int tsc_layer_norm_backward(int elem, const tsc_rows_t *dy, const tsc_rows_t *x, const float *mean, const float *scale,
+                            int64_t rows, int width, const void *weight, int param_elem, void *dx, void *dweight,
+                            void *dbias, void *workspace, size_t workspace_bytes, tsc_stream_t stream) {
+    int rc = check_norm(elem, param_elem, rows, width);
+    if (!rc) rc = check_rows(x, elem, rows, "x");
+    if (!rc) rc = check_rows(dy, elem, rows, "dy");
+    if (rc) return rc;
+    if (rows > 0 && (!mean || !scale || !dx)) return tsc_fail(TSC_ERR_ARG, "null statistics or dx pointer");
+    if (rows > 0 && (dweight || dbias) &&
+        (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < tsc_layer_norm_workspace_bytes(rows, width)))
+        return tsc_fail(TSC_ERR_ARG, "layer norm backward needs a workspace of %zu bytes (got %zu)",
+                        tsc_layer_norm_workspace_bytes(rows, width), workspace ? workspace_bytes : (size_t)0);
+    return tsc_launch_layer_norm_backward(elem, *dy, *x, mean, scale, rows, width, weight, param_elem, dx, dweight, dbias,
+                                          (float *)workspace, (hipStream_t)stream);
+}
+
 }  // extern "C"

@@ -145,3 +145,12 @@ int tsc_launch_rowdot_many(int n, const float *const *a, const long long *sa, co
                            long long R, int d, hipStream_t stream);
 int tsc_launch_project(const float *x, long long M, int d_in, const float *b_dec, const float *Pt,
                        const float *bias, int F, int relu, float *out, hipStream_t stream);
+
+// layer_norm.hip
+typedef tsc_rows_t TscRows;
+size_t tsc_layer_norm_parts(long long rows);  // rows of the backward pass' workspace, for each of dweight and dbias
+int tsc_launch_layer_norm(int elem, const TscRows &x, long long rows, int D, const void *w, const void *b, int param_elem,
+                          float eps, void *y, float *mean, float *scale, hipStream_t stream);
+int tsc_launch_layer_norm_backward(int elem, const TscRows &dy, const TscRows &x, const float *mean, const float *scale,
+                                   long long rows, int D, const void *w, int param_elem, void *dx, void *dw, void *db,
+                                   float *workspace, hipStream_t stream);

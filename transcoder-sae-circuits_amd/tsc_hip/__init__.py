@@ -73,6 +73,12 @@ _SIGNATURES = {
                                    _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_void_p]),
     "tsc_project_features": (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p,
                                         _c.c_int, _c.c_int, _c.c_void_p, _c.c_void_p]),
+    "tsc_layer_norm": (_c.c_int, [_c.c_int, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_float,
+                                  _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p]),
+    "tsc_layer_norm_workspace_bytes": (_c.c_size_t, [_c.c_int64, _c.c_int]),
+    "tsc_layer_norm_backward": (_c.c_int, [_c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int,
+                                           _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
+                                           _c.c_size_t, _c.c_void_p]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
@@ -84,6 +90,10 @@ class TscError(RuntimeError):
 class _TopkStateStruct(ctypes.Structure):
     _fields_ = [("vals", _c.c_void_p), ("idx", _c.c_void_p), ("d_sae", _c.c_int32), ("k", _c.c_int32),
                 ("n_slots", _c.c_int32), ("flags", _c.c_int32), ("floor", _c.c_void_p)]
+
+
+class _RowsStruct(ctypes.Structure):
+    _fields_ = [("data", _c.c_void_p), ("inner", _c.c_int64), ("outer_stride", _c.c_int64), ("inner_stride", _c.c_int64)]
 
 
 def library_path() -> str:
@@ -862,3 +872,115 @@ def _project_rows(x2: torch.Tensor, Pt: torch.Tensor, bias: torch.Tensor, b_dec:
                                               _stream()))
             parts.append(out)
     return parts[0] if len(parts) == 1 else torch.cat(parts, dim=1)
+
+
+# ---------------------------------------------------------------------------- the language model's head
+_ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # include/tsc_hip.h: TSC_ELEM_F32, TSC_ELEM_BF16, TSC_ELEM_F16
+
+
+def _elem(t: torch.Tensor, name: str) -> int:
+    if not t.is_cuda:
+        raise TscError(f"{name} must live on the GPU (got {t.device}); the HIP path has no CPU fallback")
+    if t.dtype not in _ELEM:
+        raise TscError(f"{name} must be float32, bfloat16 or float16 (got {t.dtype})")
+    return _ELEM[t.dtype]
+
+
+def _rows(t: torch.Tensor, name: str) -> _RowsStruct:
+    """``tsc_rows_t`` of a ``[..., D]`` tensor: its last axis is dense, the leading ones step with at most two strides
+    (``x[:, :-1]`` of a dense ``[B, T, D]``, a slice of one position, an expanded gradient)."""
+    if t.dim() < 1:
+        raise TscError(f"{name} must have a last axis")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise TscError(f"{name}: the elements of a row must be contiguous (stride {t.stride(-1)})")
+    levels = []  # (size, stride), outermost first
+    for n, st in zip(t.shape[:-1], t.stride()[:-1]):
+        if n == 1:
+            continue
+        if levels and levels[-1][1] == n * st:
+            levels[-1] = (levels[-1][0] * n, st)
+        else:
+            levels.append((n, st))
+    if t.numel() == 0 or not levels:
+        levels = [(1, 0)]
+    if len(levels) > 2:
+        raise TscError(f"{name}: rows with strides {t.stride()[:-1]} over {tuple(t.shape[:-1])} need more than two strides; "
+                       "make it contiguous")
+    if len(levels) == 1:
+        return _RowsStruct(t.data_ptr(), 1, levels[0][1], levels[0][1])
+    return _RowsStruct(t.data_ptr(), levels[1][0], levels[0][1], levels[1][1])
+
+
+def _same_device(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise TscError(f"{name} lives on {t.device}, the other operands on {device}")
+
+
+def _norm_param(p: Optional[torch.Tensor], x: torch.Tensor, name: str) -> None:
+    if p is None:
+        return
+    _elem(p, name)
+    if p.dtype not in (x.dtype, torch.float32):
+        raise TscError(f"{name} must be float32 or {x.dtype} like the rows (got {p.dtype})")
+    if tuple(p.shape) != (x.shape[-1],) or not p.is_contiguous():
+        raise TscError(f"{name} must be a contiguous [{x.shape[-1]}] tensor (got {tuple(p.shape)})")
+
+
+def _norm_params(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]) -> int:
+    _norm_param(weight, x, "weight")
+    _norm_param(bias, x, "bias")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TscError(f"weight and bias must have one type (got {weight.dtype} and {bias.dtype})")
+    p = weight if weight is not None else bias
+    return _ELEM[p.dtype if p is not None else x.dtype]
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return t.data_ptr() if t is not None else None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``tsc_layer_norm`` over the last axis of ``x`` (float32, bfloat16 or float16; leading axes with at most two strides):
+    ``(y, mean, scale)``, ``y`` dense in x's type, ``mean`` and ``scale = sqrt(var + eps)`` float32 of shape
+    ``x.shape[:-1]``.  ``weight`` / ``bias``: ``[D]`` in x's type or float32, or None (a folded layer norm)."""
+    elem, rows = _elem(x, "x"), _rows(x, "x")
+    if x.shape[-1] < 1:
+        raise TscError("layer norm of rows without elements")
+    pe = _norm_params(x, weight, bias)
+    _same_device(x.device, weight=weight, bias=bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    scale = torch.empty_like(mean)
+    with torch.cuda.device(x.device):
+        _check(lib().tsc_layer_norm(elem, ctypes.byref(rows), mean.numel(), x.shape[-1], _ptr(weight), _ptr(bias), pe, float(eps),
+                                    y.data_ptr(), mean.data_ptr(), scale.data_ptr(), _stream()))
+    return y, mean, scale
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, scale: torch.Tensor,
+                        weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None):
+    """``tsc_layer_norm_backward``: ``(dx, dweight, dbias)`` from the ``mean`` and ``scale`` that :func:`layer_norm` returned.
+    ``dweight`` (``dbias``) is None where ``weight`` (``bias``) is; else it has that parameter's type.  The same call gives
+    the same bits."""
+    elem, xr, dr = _elem(x, "x"), _rows(x, "x"), _rows(dy, "dy")
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise TscError(f"dy must be {x.dtype} {tuple(x.shape)} like x (got {dy.dtype} {tuple(dy.shape)})")
+    if x.shape[-1] < 1:
+        raise TscError("layer norm of rows without elements")
+    pe = _norm_params(x, weight, bias)
+    for name, t in (("mean", mean), ("scale", scale)):
+        if _dev(t, torch.float32, name).shape != x.shape[:-1]:
+            raise TscError(f"{name} must be {tuple(x.shape[:-1])} (got {tuple(t.shape)})")
+    _same_device(x.device, dy=dy, mean=mean, scale=scale, weight=weight, bias=bias)
+    n, d = mean.numel(), x.shape[-1]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = torch.empty_like(weight) if weight is not None else None
+    db = torch.empty_like(bias) if bias is not None else None
+    nws = lib().tsc_layer_norm_workspace_bytes(n, d) if dw is not None or db is not None else 0
+    ws = torch.empty(nws // 4, dtype=torch.float32, device=x.device) if nws else None
+    with torch.cuda.device(x.device):
+        _check(lib().tsc_layer_norm_backward(elem, ctypes.byref(dr), ctypes.byref(xr), mean.data_ptr(), scale.data_ptr(), n, d,
+                                             _ptr(weight), pe, dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), nws, _stream()))
+    return dx, dw, db
