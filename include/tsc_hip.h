@@ -432,6 +432,52 @@ int tsc_layer_norm_backward(int elem, const tsc_rows_t *dy, const tsc_rows_t *x,
                             int64_t rows, int width, const void *weight, int param_elem, void *dx, void *dweight,
                             void *dbias, void *workspace, size_t workspace_bytes, tsc_stream_t stream);
 
+/*
+ * The unembedding W_U [d_model, d_vocab] (+ b_U) of one model on one GPU, for the cross entropy of rows behind it.
+ * W element (d, v) lies d * stride_d + v * stride_v elements behind W; one of the strides is 1 (an embedding that is also
+ * the unembedding is passed as its transpose: stride_d 1, stride_v d_model), the other one at least as long as the axis it
+ * steps over.  bias [d_vocab] in bias_elem or NULL; an entry below -1e38 takes that token out
+ * (probability 0; a row for which none is left has the loss NaN).  Both are borrowed.
+ * The handle owns what the matrix pipe reads: W in both orders, padded, in 16 bits -- for TSC_ELEM_F32 as two fp16 planes
+ * that hold 22 bits of every weight down to 2^-27 of the largest and a fixed 2^-49 of it below -- 2 x 77 MB (fp32: 2 x 154)
+ * at 768 x 50257.  After an in-place change of W or bias call tsc_unembed_refresh, in order with the calls that use the
+ * handle.  d_model <= 32768, d_vocab <= 2^20.  One handle may be used from several streams.
+ */
+typedef struct tsc_unembed tsc_unembed_t;
+int tsc_unembed_create(tsc_unembed_t **out, int d_model, int d_vocab, int elem, const void *W, int64_t stride_d,
+                       int64_t stride_v, const void *bias, int bias_elem, tsc_stream_t stream);
+int tsc_unembed_refresh(tsc_unembed_t *head, tsc_stream_t stream);
+int tsc_unembed_destroy(tsc_unembed_t *head);
+
+/*
+ * Cross entropy of `rows` rows x [rows, d_model] (the handle's type) against their targets:
+ *   l = x W + b,  lse[m] = log sum_v exp l[m][v],  loss[m] = lse[m] - l[m][targets[m]],
+ * loss and lse [rows] fp32 for every type (products exact, sums fp32); the [rows, d_vocab] logits are never stored.
+ * targets [rows] int64: ignore_index = no loss (0, whatever the row holds); any other value outside 0 .. d_vocab - 1 gives
+ * NaN.  workspace: tsc_unembed_workspace_bytes(head, rows, 0, 0, 0) bytes, 256-byte aligned; rows < 2^24.
+ * Next-token loss of the model behind load_model_and_encoders.py:21, by which spliced-in dictionaries are judged.
+ */
+size_t tsc_unembed_workspace_bytes(const tsc_unembed_t *head, int64_t rows, int backward, int want_x, int want_bias);
+int tsc_unembed_loss(const tsc_unembed_t *head, const tsc_rows_t *x, int64_t rows, const int64_t *targets,
+                     int64_t ignore_index, float *loss, float *lse, void *workspace, size_t workspace_bytes,
+                     tsc_stream_t stream);
+
+/*
+ * Its gradient from the kept lse and dloss [rows] fp32 (the gradient of every row's loss):
+ *   G[m][v] = dloss[m] (exp(l[m][v] - lse[m]) - [v = targets[m]]),  dx = G W^T,  dW = x^T G,  dbias = sum over rows of G.
+ * dx [rows, d_model] dense; dW dense in W's order ([d_model, d_vocab] where stride_v is 1, else [d_vocab, d_model]); dbias
+ * [d_vocab] in bias_elem; each may be NULL = not wanted.  Ignored rows have a zero dx and add nothing, whatever they hold; a
+ * target outside the vocabulary makes its row's dx and all of dW NaN.  G is made in pieces of the vocabulary (1 GiB of
+ * workspace) and rounded to 16 bits as the operand of the two products (fp32: two planes, 22 bits down to 2^-27 of the
+ * largest and a fixed 2^-49 of it below; fp16: 11 bits down to 2^-27, a fixed 2^-38 below; the largest: of |dloss|, for fp32
+ * of |dloss| times the row's largest |x|).  dbias sums unrounded values.
+ * Sums are fp32 in a fixed order: the same call gives the same bits.
+ * workspace: tsc_unembed_workspace_bytes(head, rows, 1, dx != NULL, dbias != NULL) bytes, 256-byte aligned.
+ */
+int tsc_unembed_loss_backward(const tsc_unembed_t *head, const float *dloss, const tsc_rows_t *x, int64_t rows,
+                              const int64_t *targets, int64_t ignore_index, const float *lse, void *dx, void *dW,
+                              void *dbias, void *workspace, size_t workspace_bytes, tsc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -620,4 +620,69 @@ int tsc_layer_norm_backward(int elem, const tsc_rows_t *dy, const tsc_rows_t *x,
                                           (float *)workspace, (hipStream_t)stream);
 }
 
+int tsc_unembed_create(tsc_unembed_t **out, int d_model, int d_vocab, int elem, const void *W, int64_t stride_d,
+                       int64_t stride_v, const void *bias, int bias_elem, tsc_stream_t stream) {
+    if (!out) return tsc_fail(TSC_ERR_ARG, "null output handle");
+    *out = nullptr;
+    if (!elem_size(elem) || !elem_size(bias_elem)) return tsc_fail(TSC_ERR_ARG, "unknown element type (%d, bias %d)", elem, bias_elem);
+    if (d_model < 1 || d_vocab < 1) return tsc_fail(TSC_ERR_ARG, "an unembedding of %d x %d", d_model, d_vocab);
+    if (d_model > 32768 || d_vocab > (1 << 20))
+        return tsc_fail(TSC_ERR_UNSUPPORTED, "an unembedding of %d x %d (at most 32768 x 2^20)", d_model, d_vocab);
+    if (!W) return tsc_fail(TSC_ERR_ARG, "W is required");
+    if (!(stride_v == 1 && stride_d >= d_vocab) && !(stride_d == 1 && stride_v >= d_model))
+        return tsc_fail(TSC_ERR_ARG, "strides %lld and %lld: one of them must be 1 and the other one span its axis",
+                        (long long)stride_d, (long long)stride_v);
+    if ((uintptr_t)W % elem_size(elem) || (uintptr_t)bias % elem_size(bias_elem))
+        return tsc_fail(TSC_ERR_ARG, "W and bias must be aligned to their elements");
+    return tsc_unembed_create_(out, d_model, d_vocab, elem, W, stride_d, stride_v, bias, bias_elem, (hipStream_t)stream);
+}
+
+int tsc_unembed_refresh(tsc_unembed_t *h, tsc_stream_t stream) {
+    if (!h) return tsc_fail(TSC_ERR_ARG, "null unembedding handle");
+    return tsc_unembed_refresh_(h, (hipStream_t)stream);
+}
+
+int tsc_unembed_destroy(tsc_unembed_t *h) { return tsc_unembed_destroy_(h); }
+
+size_t tsc_unembed_workspace_bytes(const tsc_unembed_t *h, int64_t rows, int backward, int want_x, int want_bias) {
+    return !h || rows < 1 || rows >= (1 << 24) ? 0 : tsc_unembed_workspace_(h, rows, backward, want_x, want_bias);
+}
+
+static int check_unembed(const tsc_unembed_t *h, const tsc_rows_t *x, int64_t rows, const int64_t *targets, const float *lse,
+                         const void *workspace, size_t workspace_bytes, size_t need) {
+    if (!h) return tsc_fail(TSC_ERR_ARG, "null unembedding handle");
+    if (rows < 0) return tsc_fail(TSC_ERR_ARG, "negative row count %lld", (long long)rows);
+    if (rows >= (1 << 24)) return tsc_fail(TSC_ERR_UNSUPPORTED, "%lld rows in one call (fewer than 2^24)", (long long)rows);
+    int elem, d, v;
+    tsc_unembed_shape_(h, &elem, &d, &v);
+    int rc = check_rows(x, elem, rows, "x");
+    if (rc || rows == 0) return rc;
+    if (!targets || !lse) return tsc_fail(TSC_ERR_ARG, "null targets or lse pointer");
+    if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need)
+        return tsc_fail(TSC_ERR_ARG, "a 256-byte aligned workspace of %zu bytes is needed (got %zu)", need,
+                        workspace ? workspace_bytes : (size_t)0);
+    return TSC_OK;
+}
+
+int tsc_unembed_loss(const tsc_unembed_t *h, const tsc_rows_t *x, int64_t rows, const int64_t *targets, int64_t ignore_index,
+                     float *loss, float *lse, void *workspace, size_t workspace_bytes, tsc_stream_t stream) {
+    int rc = check_unembed(h, x, rows, targets, lse, workspace, workspace_bytes, tsc_unembed_workspace_bytes(h, rows, 0, 0, 0));
+    if (rc || rows == 0) return rc;
+    if (!loss) return tsc_fail(TSC_ERR_ARG, "null loss pointer");
+    return tsc_launch_unembed_loss(h, *x, (int)rows, (const long long *)targets, ignore_index, loss, lse, (char *)workspace,
+                                   (hipStream_t)stream);
+}
+
+int tsc_unembed_loss_backward(const tsc_unembed_t *h, const float *dloss, const tsc_rows_t *x, int64_t rows,
+                              const int64_t *targets, int64_t ignore_index, const float *lse, void *dx, void *dW, void *dbias,
+                              void *workspace, size_t workspace_bytes, tsc_stream_t stream) {
+    int rc = check_unembed(h, x, rows, targets, lse, workspace, workspace_bytes,
+                           tsc_unembed_workspace_bytes(h, rows, 1, dx != nullptr, dbias != nullptr));
+    if (rc) return rc;
+    if (rows > 0 && !dloss) return tsc_fail(TSC_ERR_ARG, "null dloss pointer");
+    if (!dx && !dW && !dbias) return TSC_OK;
+    return tsc_launch_unembed_backward(h, dloss, *x, (int)rows, (const long long *)targets, ignore_index, lse, dx, dW, dbias,
+                                       (char *)workspace, (hipStream_t)stream);
+}
+
 }  // extern "C"

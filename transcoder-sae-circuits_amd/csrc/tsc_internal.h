@@ -154,3 +154,15 @@ int tsc_launch_layer_norm(int elem, const TscRows &x, long long rows, int D, con
 int tsc_launch_layer_norm_backward(int elem, const TscRows &dy, const TscRows &x, const float *mean, const float *scale,
                                    long long rows, int D, const void *w, int param_elem, void *dx, void *dw, void *db,
                                    float *workspace, hipStream_t stream);
+
+// unembed.hip
+int tsc_unembed_create_(tsc_unembed **out, int D, int V, int elem, const void *W, long long sd, long long sv, const void *bias,
+                        int bias_elem, hipStream_t stream);
+int tsc_unembed_refresh_(tsc_unembed *h, hipStream_t stream);
+int tsc_unembed_destroy_(tsc_unembed *h);
+void tsc_unembed_shape_(const tsc_unembed *h, int *elem, int *D, int *V);
+size_t tsc_unembed_workspace_(const tsc_unembed *h, long long M, int backward, int want_x, int want_bias);
+int tsc_launch_unembed_loss(const tsc_unembed *h, const TscRows &x, int M, const long long *targets, long long ignore, float *loss,
+                            float *lse, char *workspace, hipStream_t stream);
+int tsc_launch_unembed_backward(const tsc_unembed *h, const float *dloss, const TscRows &x, int M, const long long *targets,
+                                long long ignore, const float *lse, void *dx, void *dW, void *db, char *workspace, hipStream_t stream);

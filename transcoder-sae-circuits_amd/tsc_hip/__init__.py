@@ -79,6 +79,16 @@ _SIGNATURES = {
     "tsc_layer_norm_backward": (_c.c_int, [_c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int,
                                            _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
                                            _c.c_size_t, _c.c_void_p]),
+    "tsc_unembed_create": (_c.c_int, [_c.POINTER(_c.c_void_p), _c.c_int, _c.c_int, _c.c_int, _c.c_void_p, _c.c_int64,
+                                      _c.c_int64, _c.c_void_p, _c.c_int, _c.c_void_p]),
+    "tsc_unembed_refresh": (_c.c_int, [_c.c_void_p, _c.c_void_p]),
+    "tsc_unembed_destroy": (_c.c_int, [_c.c_void_p]),
+    "tsc_unembed_workspace_bytes": (_c.c_size_t, [_c.c_void_p, _c.c_int64, _c.c_int, _c.c_int, _c.c_int]),
+    "tsc_unembed_loss": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p,
+                                    _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "tsc_unembed_loss_backward": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64,
+                                             _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_size_t,
+                                             _c.c_void_p]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
@@ -984,3 +994,116 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, s
         _check(lib().tsc_layer_norm_backward(elem, ctypes.byref(dr), ctypes.byref(xr), mean.data_ptr(), scale.data_ptr(), n, d,
                                              _ptr(weight), pe, dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), nws, _stream()))
     return dx, dw, db
+
+
+class UnembedHead:
+    """The unembedding ``W_U [d_model, d_vocab]`` and ``b_U [d_vocab]`` of one model, for the cross entropy behind it without
+    the ``[rows, d_vocab]`` logits (``tsc_unembed_create``).  ``W_U``: float32, bfloat16 or float16, dense along one of its
+    axes (an embedding that is also the unembedding is passed as ``W_E.t()``); ``b_U``: that type or float32, or None.
+
+    Borrows both tensors and owns 16-bit copies of ``W_U`` in both orders, laid out at construction and again by
+    :meth:`refresh`.  :meth:`loss` and :meth:`loss_backward` do that by themselves when torch's version counters say that a
+    tensor was changed in place (inference tensors have none: call :meth:`refresh`)."""
+
+    def __init__(self, W_U: torch.Tensor, b_U: Optional[torch.Tensor] = None):
+        self._handle = ctypes.c_void_p()
+        elem = _elem(W_U, "W_U")
+        if W_U.dim() != 2 or W_U.numel() == 0:
+            raise TscError(f"W_U must be [d_model, d_vocab] (got {tuple(W_U.shape)})")
+        self.d_model, self.d_vocab = W_U.shape
+        sd, sv = W_U.stride()
+        if self.d_vocab == 1:
+            sd, sv = (1, max(sv, self.d_model)) if sd == 1 else (sd, 1)
+        elif self.d_model == 1:
+            sd, sv = (max(sd, self.d_vocab), 1) if sv == 1 else (1, sv)
+        if not (sv == 1 and sd >= self.d_vocab) and not (sd == 1 and sv >= self.d_model):
+            raise TscError(f"W_U must be dense along one of its axes (strides {W_U.stride()})")
+        if b_U is not None:
+            _elem(b_U, "b_U")
+            if tuple(b_U.shape) != (self.d_vocab,) or not b_U.is_contiguous() or b_U.dtype not in (W_U.dtype, torch.float32):
+                raise TscError(f"b_U must be a contiguous [{self.d_vocab}] tensor of {W_U.dtype} or float32")
+            _same_device(W_U.device, b_U=b_U)
+        self._by_d = sv == 1
+        self._keep = [W_U] if b_U is None else [W_U, b_U]
+        self.W_U, self.b_U, self.device, self.dtype = W_U, b_U, W_U.device, W_U.dtype
+        with torch.cuda.device(self.device):
+            _check(lib().tsc_unembed_create(ctypes.byref(self._handle), self.d_model, self.d_vocab, elem, W_U.data_ptr(), sd, sv,
+                                            _ptr(b_U), _ELEM[b_U.dtype] if b_U is not None else elem, _stream()))
+        self._versions = self._param_versions()
+
+    def _param_versions(self):
+        return tuple(0 if t.is_inference() else t._version for t in self._keep)
+
+    def refresh(self) -> None:
+        """Lay the weights out again (``tsc_unembed_refresh``)."""
+        with torch.cuda.device(self.device):
+            _check(lib().tsc_unembed_refresh(self._handle, _stream()))
+        self._versions = self._param_versions()
+
+    def refresh_if_modified(self) -> None:
+        if self._param_versions() != self._versions:
+            self.refresh()
+
+    def close(self) -> None:
+        if self._handle:
+            lib().tsc_unembed_destroy(self._handle)
+            self._handle = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _operands(self, x: torch.Tensor, targets: torch.Tensor):
+        _elem(x, "x")
+        if not self._handle:
+            raise TscError("this UnembedHead is closed")
+        if x.dtype != self.dtype or x.dim() < 1 or x.shape[-1] != self.d_model:
+            raise TscError(f"x must be {self.dtype} [..., {self.d_model}] (got {x.dtype} {tuple(x.shape)})")
+        if _dev(targets, torch.int64, "targets").shape != x.shape[:-1]:
+            raise TscError(f"targets must be {tuple(x.shape[:-1])} (got {tuple(targets.shape)})")
+        _same_device(self.device, x=x, targets=targets)
+        return _rows(x, "x"), targets.numel()
+
+    def _workspace(self, *shape):
+        n = lib().tsc_unembed_workspace_bytes(self._handle, *shape)
+        return torch.empty(n, dtype=torch.uint8, device=self.device), n
+
+    def loss(self, x: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``tsc_unembed_loss``: ``(loss, lse)``, float32 of shape ``x.shape[:-1]``: every row's cross entropy (0 where the
+        target is ``ignore_index``, NaN where it is outside the vocabulary otherwise) and the logarithm of its sum of
+        exponentials, which :meth:`loss_backward` takes."""
+        rows, m = self._operands(x, targets)
+        self.refresh_if_modified()
+        loss = torch.empty(targets.shape, dtype=torch.float32, device=self.device)
+        lse = torch.empty_like(loss)
+        with torch.cuda.device(self.device):
+            ws, n = self._workspace(m, 0, 0, 0)
+            _check(lib().tsc_unembed_loss(self._handle, ctypes.byref(rows), m, targets.data_ptr(), int(ignore_index),
+                                          loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), n, _stream()))
+        return loss, lse
+
+    def loss_backward(self, dloss: torch.Tensor, x: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
+                      ignore_index: int = -100, want_x: bool = True, want_weight: bool = True, want_bias: bool = True):
+        """``tsc_unembed_loss_backward``: ``(dx, dW, db)`` for the gradient ``dloss`` (float32, ``x.shape[:-1]``) of the rows'
+        losses, None where not wanted (``db`` also without ``b_U``).  ``dx`` and ``dW`` have x's type, ``dW`` the shape and
+        the order of ``W_U``, ``db`` the type of ``b_U``."""
+        rows, m = self._operands(x, targets)
+        for name, t in (("dloss", dloss), ("lse", lse)):
+            if _dev(t, torch.float32, name).shape != targets.shape:
+                raise TscError(f"{name} must be {tuple(targets.shape)} (got {tuple(t.shape)})")
+            _same_device(self.device, **{name: t})
+        self.refresh_if_modified()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=self.device) if want_x else None
+        dW = None
+        if want_weight:
+            dW = torch.empty((self.d_model, self.d_vocab) if self._by_d else (self.d_vocab, self.d_model), dtype=x.dtype,
+                             device=self.device)
+        db = torch.empty_like(self.b_U) if want_bias and self.b_U is not None else None
+        with torch.cuda.device(self.device):
+            ws, n = self._workspace(m, 1, int(dx is not None), int(db is not None))
+            _check(lib().tsc_unembed_loss_backward(self._handle, dloss.data_ptr(), ctypes.byref(rows), m, targets.data_ptr(),
+                                                   int(ignore_index), lse.data_ptr(), _ptr(dx), _ptr(dW), _ptr(db), ws.data_ptr(),
+                                                   n, _stream()))
+        return dx, dW if dW is None or self._by_d else dW.t(), db
