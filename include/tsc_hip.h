@@ -454,10 +454,11 @@ int tsc_unembed_destroy(tsc_unembed_t *head);
  *   l = x W + b,  lse[m] = log sum_v exp l[m][v],  loss[m] = lse[m] - l[m][targets[m]],
  * loss and lse [rows] fp32 for every type (products exact, sums fp32); the [rows, d_vocab] logits are never stored.
  * targets [rows] int64: ignore_index = no loss (0, whatever the row holds); any other value outside 0 .. d_vocab - 1 gives
- * NaN.  workspace: tsc_unembed_workspace_bytes(head, rows, 0, 0, 0) bytes, 256-byte aligned; rows < 2^24.
+ * NaN.  workspace: tsc_unembed_workspace_bytes(head, rows, 0, 0, 0, 0) bytes, 256-byte aligned; rows < 2^24.
  * Next-token loss of the model behind load_model_and_encoders.py:21, by which spliced-in dictionaries are judged.
  */
-size_t tsc_unembed_workspace_bytes(const tsc_unembed_t *head, int64_t rows, int backward, int want_x, int want_bias);
+size_t tsc_unembed_workspace_bytes(const tsc_unembed_t *head, int64_t rows, int backward, int want_x, int want_w,
+                                   int want_bias);
 int tsc_unembed_loss(const tsc_unembed_t *head, const tsc_rows_t *x, int64_t rows, const int64_t *targets,
                      int64_t ignore_index, float *loss, float *lse, void *workspace, size_t workspace_bytes,
                      tsc_stream_t stream);
@@ -467,12 +468,12 @@ int tsc_unembed_loss(const tsc_unembed_t *head, const tsc_rows_t *x, int64_t row
  *   G[m][v] = dloss[m] (exp(l[m][v] - lse[m]) - [v = targets[m]]),  dx = G W^T,  dW = x^T G,  dbias = sum over rows of G.
  * dx [rows, d_model] dense; dW dense in W's order ([d_model, d_vocab] where stride_v is 1, else [d_vocab, d_model]); dbias
  * [d_vocab] in bias_elem; each may be NULL = not wanted.  Ignored rows have a zero dx and add nothing, whatever they hold; a
- * target outside the vocabulary makes its row's dx and all of dW NaN.  G is made in pieces of the vocabulary (1 GiB of
+ * target outside the vocabulary makes its row's dx and all of dW NaN.  G is made in pieces of the vocabulary (1.5 GiB of
  * workspace) and rounded to 16 bits as the operand of the two products (fp32: two planes, 22 bits down to 2^-27 of the
  * largest and a fixed 2^-49 of it below; fp16: 11 bits down to 2^-27, a fixed 2^-38 below; the largest: of |dloss|, for fp32
  * of |dloss| times the row's largest |x|).  dbias sums unrounded values.
  * Sums are fp32 in a fixed order: the same call gives the same bits.
- * workspace: tsc_unembed_workspace_bytes(head, rows, 1, dx != NULL, dbias != NULL) bytes, 256-byte aligned.
+ * workspace: tsc_unembed_workspace_bytes(head, rows, 1, dx != NULL, dW != NULL, dbias != NULL) bytes, 256-byte aligned.
  */
 int tsc_unembed_loss_backward(const tsc_unembed_t *head, const float *dloss, const tsc_rows_t *x, int64_t rows,
                               const int64_t *targets, int64_t ignore_index, const float *lse, void *dx, void *dW,

@@ -392,7 +392,7 @@ def test_refusals_on_device():
             bad()
     lib = tsc_hip.lib()
     R = tsc_hip._RowsStruct(x.data_ptr(), 1, 16, 16)
-    n = lib.tsc_unembed_workspace_bytes(head._handle, 8, 0, 0, 0)
+    n = lib.tsc_unembed_workspace_bytes(head._handle, 8, 0, 0, 0, 0)
     ws = torch.empty(n, dtype=torch.uint8, device=DEV)
     loss = torch.empty(8, device=DEV)
     call = lambda rows=8, w=ws.data_ptr(), size=n: lib.tsc_unembed_loss(  # noqa: E731
@@ -420,7 +420,7 @@ def test_c_entry_points_refuse_bad_arguments():
     assert make_(d=40000, sd=1 << 40) == -3 and make_(v=(1 << 20) + 1, sd=1 << 40) == -3
     assert lib.tsc_unembed_create(None, 8, 9, 0, 4096, 9, 1, None, 0, None) == -1
     assert lib.tsc_unembed_refresh(None, None) == -1 and lib.tsc_unembed_destroy(None) == 0
-    assert lib.tsc_unembed_workspace_bytes(None, 4, 0, 0, 0) == 0
+    assert lib.tsc_unembed_workspace_bytes(None, 4, 0, 0, 0, 0) == 0
     assert lib.tsc_unembed_loss(None, None, 4, None, 0, None, None, None, 0, None) == -1
     assert lib.tsc_unembed_loss_backward(None, None, None, 4, None, 0, None, None, None, None, None, 0, None) == -1
 

@@ -644,8 +644,9 @@ int tsc_unembed_refresh(tsc_unembed_t *h, tsc_stream_t stream) {
 
 int tsc_unembed_destroy(tsc_unembed_t *h) { return tsc_unembed_destroy_(h); }
 
-size_t tsc_unembed_workspace_bytes(const tsc_unembed_t *h, int64_t rows, int backward, int want_x, int want_bias) {
-    return !h || rows < 1 || rows >= (1 << 24) ? 0 : tsc_unembed_workspace_(h, rows, backward, want_x, want_bias);
+size_t tsc_unembed_workspace_bytes(const tsc_unembed_t *h, int64_t rows, int backward, int want_x, int want_w,
+                                   int want_bias) {
+    return !h || rows < 1 || rows >= (1 << 24) ? 0 : tsc_unembed_workspace_(h, rows, backward, want_x, want_w, want_bias);
 }
 
 static int check_unembed(const tsc_unembed_t *h, const tsc_rows_t *x, int64_t rows, const int64_t *targets, const float *lse,
@@ -666,7 +667,7 @@ static int check_unembed(const tsc_unembed_t *h, const tsc_rows_t *x, int64_t ro
 
 int tsc_unembed_loss(const tsc_unembed_t *h, const tsc_rows_t *x, int64_t rows, const int64_t *targets, int64_t ignore_index,
                      float *loss, float *lse, void *workspace, size_t workspace_bytes, tsc_stream_t stream) {
-    int rc = check_unembed(h, x, rows, targets, lse, workspace, workspace_bytes, tsc_unembed_workspace_bytes(h, rows, 0, 0, 0));
+    int rc = check_unembed(h, x, rows, targets, lse, workspace, workspace_bytes, tsc_unembed_workspace_bytes(h, rows, 0, 0, 0, 0));
     if (rc || rows == 0) return rc;
     if (!loss) return tsc_fail(TSC_ERR_ARG, "null loss pointer");
     return tsc_launch_unembed_loss(h, *x, (int)rows, (const long long *)targets, ignore_index, loss, lse, (char *)workspace,
@@ -677,7 +678,7 @@ int tsc_unembed_loss_backward(const tsc_unembed_t *h, const float *dloss, const 
                               const int64_t *targets, int64_t ignore_index, const float *lse, void *dx, void *dW, void *dbias,
                               void *workspace, size_t workspace_bytes, tsc_stream_t stream) {
     int rc = check_unembed(h, x, rows, targets, lse, workspace, workspace_bytes,
-                           tsc_unembed_workspace_bytes(h, rows, 1, dx != nullptr, dbias != nullptr));
+                           tsc_unembed_workspace_bytes(h, rows, 1, dx != nullptr, dW != nullptr, dbias != nullptr));
     if (rc) return rc;
     if (rows > 0 && !dloss) return tsc_fail(TSC_ERR_ARG, "null dloss pointer");
     if (!dx && !dW && !dbias) return TSC_OK;

@@ -161,7 +161,7 @@ int tsc_unembed_create_(tsc_unembed **out, int D, int V, int elem, const void *W
 int tsc_unembed_refresh_(tsc_unembed *h, hipStream_t stream);
 int tsc_unembed_destroy_(tsc_unembed *h);
 void tsc_unembed_shape_(const tsc_unembed *h, int *elem, int *D, int *V);
-size_t tsc_unembed_workspace_(const tsc_unembed *h, long long M, int backward, int want_x, int want_bias);
+size_t tsc_unembed_workspace_(const tsc_unembed *h, long long M, int backward, int want_x, int want_w, int want_bias);
 int tsc_launch_unembed_loss(const tsc_unembed *h, const TscRows &x, int M, const long long *targets, long long ignore, float *loss,
                             float *lse, char *workspace, hipStream_t stream);
 int tsc_launch_unembed_backward(const tsc_unembed *h, const float *dloss, const TscRows &x, int M, const long long *targets,

@@ -180,154 +180,235 @@ __device__ __forceinline__ float2 merge(float2 a, float2 b) {
 }
 
 struct LogitArgs {
-    Operand W, x;       // i = v, j = m
-    int nk, passes, ti, tj, v0;  // v0: first entry of the piece (tiles are counted from it)
+    Operand W, x;
+    int nk, passes;
+    int nm, ns, nv, v0;  // blocks of rows, streams of a block, tiles of the vocabulary (counted from entry v0)
     int M, V;
-    const float *bias;   // -inf behind V
-    const float *wscale, *xscale;  // null: 1
+    const float *bias;                  // -inf behind V
+    const float *wscale, *xscale;       // null: 1
     const long long *targets;
     long long ignore;
     // forward
-    float2 *part;        // [ti][M]: maximum, sum of exp2((l - maximum) log2 e)
+    float2 *part;        // [ns][M]: reference, sum of 2^(l log2 e - reference)
     float *hit;          // [M]
     // backward
     const float *lse, *rowf;
     short *G;            // [Mp][ldg], second plane at gplane
     long long ldg, gplane;
-    int Mp, f16, planes;
-    float *dbias;        // [tj][ldg] or null
-    const float *g;      // d(loss) of the rows
+    int Mp;
+    float *dbias;        // [parts of the rows][ldg] or null
 };
 
-template <class C, bool F16, bool GRAD> __global__ __launch_bounds__(C::NT) void logits_kernel(const LogitArgs a) {
+// Forward, i = v, j = m: a lane holds 16 WI logits of one row for each of its WJ columns.  The workgroup walks every ns-th
+// tile of the vocabulary for one block of rows.  The first tile's maximum becomes the row's reference; from then on a tile
+// costs an fma, an exponential and an add an element: sums of 2^(l - reference) are exact enough whatever the later maxima
+// are, as long as nothing overflows (the tile is then repeated with its own maximum) -- what underflows is below 2^-126 of a
+// term that is already in the sum.
+template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, 2) void loss_logits_kernel(const LogitArgs a) {
     typedef Gemm<C, false, F16> G;
     __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
-    int bi, bj;
-    tile_of(blockIdx.x, a.ti, a.tj, bi, bj);
-    const int i0 = a.v0 + bi * C::BI, j0 = bj * C::BJ;
-    f32x16 acc[C::WI][C::WJ];
-    G::run(a.W, a.x, i0, j0, 0, a.nk, a.passes, lds, acc);
+    int bj, st;
+    tile_of(blockIdx.x, a.nm, a.ns, bj, st);
+    const int j0 = bj * C::BJ;
     const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wi = wave / C::VJ, wi0 = i0 + wi * (C::WI * 32), wj0 = j0 + (wave % C::VJ) * (C::WJ * 32);
-    const float ws = a.wscale ? a.wscale[0] : 1.f;
-    float sc[C::WJ];
-    long long tg[C::WJ];
+    const int wi = wave / C::VJ, wj0 = j0 + (wave % C::VJ) * (C::WJ * 32);
+    float sc[C::WJ], ref[C::WJ], sum[C::WJ];
+    int tg[C::WJ];
 #pragma unroll
     for (int q = 0; q < C::WJ; ++q) {
         const int m = wj0 + q * 32 + li, mc = m < a.M ? m : a.M - 1;
-        sc[q] = a.xscale ? a.xscale[mc] * ws : 1.f;
-        tg[q] = m < a.M ? a.targets[mc] : -1;
+        sc[q] = SPLIT ? a.xscale[mc] * a.wscale[0] : 1.f;
+        const long long t = a.targets[mc];
+        tg[q] = m < a.M && t >= 0 && t < a.V ? (int)t : -1;
+        ref[q] = -__builtin_inff();
+        sum[q] = 0.f;
     }
-    // logits in place of the products
+    auto tile = [&](int t) { return TileAt{(st + t * a.ns) * C::BI, j0}; };
+    auto first = [&](int t) { return (st + t * a.ns) * C::BI + wi * (C::WI * 32); };
+    auto begin = [&](int t, f32x16 (&acc)[C::WI][C::WJ]) {
+        const float *b0 = a.bias + first(t) + 4 * lh;
 #pragma unroll
-    for (int p = 0; p < C::WI; ++p)
+        for (int p = 0; p < C::WI; ++p)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const f32x4 b = *(const f32x4 *)(a.bias + wi0 + p * 32 + 8 * s + 4 * lh);
+            for (int s = 0; s < 4; ++s) {
+                const f32x4 b = SPLIT ? (f32x4){0.f, 0.f, 0.f, 0.f} : *(const f32x4 *)(b0 + p * 32 + 8 * s);
 #pragma unroll
-            for (int q = 0; q < C::WJ; ++q)
+                for (int q = 0; q < C::WJ; ++q)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[p][q][s * 4 + e] = fmaf(acc[p][q][s * 4 + e], sc[q], b[e]);
+                    for (int e = 0; e < 4; ++e) acc[p][q][s * 4 + e] = b[e];  // products start from the bias
+            }
+    };
+    auto done = [&](int t, f32x16 (&acc)[C::WI][C::WJ]) {
+        const int wi0 = first(t);
+        if (SPLIT) {
+#pragma unroll
+            for (int p = 0; p < C::WI; ++p) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const f32x4 b = *(const f32x4 *)(a.bias + wi0 + 4 * lh + p * 32 + 8 * s);
+#pragma unroll
+                    for (int q = 0; q < C::WJ; ++q)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[p][q][s * 4 + e] = fmaf(acc[p][q][s * 4 + e], sc[q], b[e]);
+                }
+                __builtin_amdgcn_sched_barrier(0);  // (block by block: together the temporaries spill)
+            }
         }
-    if constexpr (!GRAD) {
-        __syncthreads();  // the operand tiles are no longer read: their place takes the waves' parts
-        float2 *sm = (float2 *)lds;
 #pragma unroll
         for (int q = 0; q < C::WJ; ++q) {
-            float top = acc[0][q][0];
+            float part[4];
+            auto add = [&](float r) {
+                part[0] = part[1] = part[2] = part[3] = 0.f;
 #pragma unroll
-            for (int p = 0; p < C::WI; ++p)
+                for (int p = 0; p < C::WI; ++p) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[p][q][r]);
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float ref = top > -__builtin_inff() ? top * LOG2E : 0.f;  // nothing but -inf: the sum is 0
-            float sum = 0.f;
+                    for (int e = 0; e < 16; ++e) part[e & 3] += exp2_(fmaf(acc[p][q][e], LOG2E, -r));
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                return (part[0] + part[1]) + (part[2] + part[3]);
+            };
+            float s = add(ref[q] > -__builtin_inff() ? ref[q] : 0.f);
+            const bool ok = ref[q] > -__builtin_inff() && s < 0x1p100f;
+            if (__builtin_amdgcn_ballot_w64(!ok)) {
+                float top = acc[0][q][0];
 #pragma unroll
-            for (int p = 0; p < C::WI; ++p)
+                for (int p = 0; p < C::WI; ++p)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sum += exp2_(fmaf(acc[p][q][r], LOG2E, -ref));
-            sum += __shfl_xor(sum, 32);
-            const int jl = wj0 - j0 + q * 32 + li;
-            if (lh == 0) sm[wi * C::BJ + jl] = make_float2(top > -__builtin_inff() ? ref : -__builtin_inff(), sum);
+                    for (int e = 0; e < 16; ++e) top = fmaxf(top, acc[p][q][e]);
+                const float r = ok ? ref[q] : top > -__builtin_inff() ? fmaxf(ref[q], top * LOG2E) : ref[q];
+                s = add(r > -__builtin_inff() ? r : 0.f);  // (nothing but -inf so far: the sum is 0)
+                if (ref[q] > -__builtin_inff()) sum[q] *= exp2_(ref[q] - r);
+                ref[q] = r;
+            }
+            sum[q] += s;
             // the target's logit, where it is one of this wave's
-            const long long at = tg[q] - wi0;
-            const bool mine = at >= 0 && at < C::WI * 32 && tg[q] < a.V && ((at >> 2) & 1) == lh;
+            const int at = tg[q] - wi0 - 4 * lh;  // a lane's entries: block_row(r, 0) of each block
+            const bool mine = tg[q] >= 0 && at >= 0 && at < C::WI * 32 && (at & 4) == 0;
             if (__builtin_amdgcn_ballot_w64(mine)) {
 #pragma unroll
                 for (int p = 0; p < C::WI; ++p)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (mine && at == p * 32 + block_row(r, lh)) a.hit[wj0 + q * 32 + li] = acc[p][q][r];
+                        if (mine && at == p * 32 + block_row(r, 0)) a.hit[wj0 + q * 32 + li] = acc[p][q][r];
             }
         }
-        __syncthreads();
-        for (int jl = threadIdx.x; jl < C::BJ; jl += C::NT) {
-            if (j0 + jl >= a.M) continue;
-            float2 v = sm[jl];
+    };
+    G::run(a.W, a.x, (a.nv - st + a.ns - 1) / a.ns, tile, 0, a.nk, a.passes, lds, begin, done);
+    __syncthreads();  // the operand tiles are no longer read: their place takes the waves' parts
+    float2 *sm = (float2 *)lds;
 #pragma unroll
-            for (int w = 1; w < C::VI; ++w) {
-                const float2 u = sm[w * C::BJ + jl];
-                v = merge(v, u);
-            }
-            a.part[(long long)bi * a.M + j0 + jl] = v;
-        }
-    } else {
-        float db[C::WI][16];
-        if (a.dbias)
+    for (int q = 0; q < C::WJ; ++q) {
+        const float2 v = merge(make_float2(ref[q], sum[q]), make_float2(__shfl_xor(ref[q], 32), __shfl_xor(sum[q], 32)));
+        if (lh == 0) sm[wi * C::BJ + wj0 - j0 + q * 32 + li] = v;
+    }
+    __syncthreads();
+    for (int jl = threadIdx.x; jl < C::BJ; jl += C::NT) {
+        if (j0 + jl >= a.M) continue;
+        float2 v = sm[jl];
 #pragma unroll
-            for (int p = 0; p < C::WI; ++p)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) db[p][r] = 0.f;
-#pragma unroll
-        for (int q = 0; q < C::WJ; ++q) {
-            const int m = wj0 + q * 32 + li, mc = m < a.M ? m : a.M - 1;
-            const bool live = m < a.M && tg[q] != a.ignore;
-            const float lse2 = a.lse[mc] * LOG2E, f = a.rowf[mc], g = a.dbias ? a.g[mc] : 0.f;
-            const long long at = tg[q] - wi0;
-            short *row = a.G + (long long)m * a.ldg + (wi0 - a.v0) + 4 * lh;
-#pragma unroll
-            for (int p = 0; p < C::WI; ++p)
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    short h1[4], h2[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = s * 4 + e, v = p * 32 + block_row(r, lh);
-                        float d = exp2_(fmaf(acc[p][q][r], LOG2E, -lse2));
-                        d -= at == v ? 1.f : 0.f;
-                        const float w = live ? d * f : 0.f;
-                        if (a.dbias) db[p][r] += live ? d * g : 0.f;
-                        if (!F16) h1[e] = bits((__bf16)w);
-                        else if (a.planes == 2) split(w, h1[e], h2[e]);
-                        else h1[e] = bits((_Float16)w);
-                    }
-                    if (m < a.Mp) {
-                        *(s16x4 *)(row + p * 32 + 8 * s) = (s16x4){h1[0], h1[1], h1[2], h1[3]};
-                        if (a.planes == 2) *(s16x4 *)(row + a.gplane + p * 32 + 8 * s) = (s16x4){h2[0], h2[1], h2[2], h2[3]};
-                    }
-                }
-        }
-        if (a.dbias) {  // over the wave's rows (lanes), then over the waves beside it
-            __syncthreads();
-            float *sm = (float *)lds;
-#pragma unroll
-            for (int p = 0; p < C::WI; ++p)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float v = db[p][r];
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor(v, o);
-                    if (li == 0) sm[(wave % C::VJ) * C::BI + wi * (C::WI * 32) + p * 32 + block_row(r, lh)] = v;
-                }
-            __syncthreads();
-            for (int il = threadIdx.x; il < C::BI; il += C::NT) {
-                float v = 0.f;
-#pragma unroll
-                for (int w = 0; w < C::VJ; ++w) v += sm[w * C::BI + il];
-                a.dbias[(long long)bj * a.ldg + bi * C::BI + il] = v;
-            }
+        for (int w = 1; w < C::VI; ++w) v = merge(v, sm[w * C::BJ + jl]);
+        a.part[(long long)st * a.M + j0 + jl] = v;
+    }
+}
+
+// Backward, i = m, j = v: a lane holds one entry of the vocabulary and 16 WI rows of it, so db is a sum over its registers,
+// and two neighbouring lanes exchange halves to store two entries of a row each.  The rows' constants lie in LDS.
+template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, 2) void grad_logits_kernel(const LogitArgs a) {
+    typedef Gemm<C, false, F16> G;
+    __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
+    __shared__ __attribute__((aligned(16))) float r_lse[C::BI], r_f[C::BI], r_sc[SPLIT ? C::BI : 4], r_inv[SPLIT ? C::BI : 4];
+    __shared__ __attribute__((aligned(16))) int r_t[C::BI];
+    int bi, st;
+    tile_of(blockIdx.x, a.nm, a.ns, bi, st);
+    const int i0 = bi * C::BI;
+    const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wi = wave / C::VJ, wr = wi * (C::WI * 32), wj = (wave % C::VJ) * (C::WJ * 32);
+    for (int i = threadIdx.x; i < C::BI; i += C::NT) {
+        const int m = i0 + i, mc = m < a.M ? m : a.M - 1;
+        const long long t = a.targets[mc];
+        const bool live = m < a.M && t != a.ignore;
+        // rows without a loss: every exponential is 2^-inf = 0
+        r_lse[i] = live ? a.lse[mc] * LOG2E : __builtin_inff();
+        r_f[i] = live ? a.rowf[mc] : 0.f;
+        r_t[i] = live && t >= 0 && t < a.V ? (int)t - a.v0 : -1;
+        if (SPLIT) {
+            r_sc[i] = a.xscale[mc] * a.wscale[0] * LOG2E;
+            r_inv[i] = 1.f / a.xscale[mc];
         }
     }
+    __syncthreads();
+    const unsigned sel = lane & 1 ? 0x03020706u : 0x05040100u;  // of (neighbour's pair : own pair)
+    auto tile = [&](int t) { return TileAt{i0, a.v0 + (st + t * a.ns) * C::BJ}; };
+    auto first = [&](int t) { return (st + t * a.ns) * C::BJ + wj; };  // in the piece
+    auto begin = [&](int t, f32x16 (&acc)[C::WI][C::WJ]) {
+#pragma unroll
+        for (int q = 0; q < C::WJ; ++q) {
+            const float b = SPLIT ? 0.f : a.bias[a.v0 + first(t) + q * 32 + li];
+#pragma unroll
+            for (int p = 0; p < C::WI; ++p)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[p][q][r] = b;
+        }
+    };
+    auto done = [&](int t, f32x16 (&acc)[C::WI][C::WJ]) {
+        const int v = first(t);
+        bool any = false;  // is one of the wave's targets in its columns?
+#pragma unroll
+        for (int i = 0; i < C::WI * 32; i += 64) {
+            const int at = r_t[wr + (i + lane < C::WI * 32 ? i + lane : 0)] - v;
+            any = any || (at >= 0 && at < C::WJ * 32);
+        }
+        const bool hot = __builtin_amdgcn_ballot_w64(any) != 0;
+#pragma unroll
+        for (int q = 0; q < C::WJ; ++q) {
+            const int col = v + q * 32 + li;
+            const float b2 = SPLIT ? a.bias[a.v0 + col] * LOG2E : 0.f;
+            float db = 0.f;
+            short *out = a.G + (long long)(i0 + wr + 4 * lh + (lane & 1)) * a.ldg + (col & ~1);
+#pragma unroll
+            for (int p = 0; p < C::WI; ++p) {
+                if (i0 + wr + p * 32 >= a.Mp) break;  // (Mp is a multiple of 64)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const int at = wr + p * 32 + 8 * s + 4 * lh;
+                    const f32x4 l = *(const f32x4 *)&r_lse[at], f = *(const f32x4 *)&r_f[at];
+                    f32x4 sc, inv;
+                    if (SPLIT) sc = *(const f32x4 *)&r_sc[at], inv = *(const f32x4 *)&r_inv[at];
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = acc[p][q][s * 4 + e];
+                        const float pr = exp2_(SPLIT ? fmaf(x, sc[e], b2) - l[e] : fmaf(x, LOG2E, -l[e]));
+                        w[e] = hot ? (pr - (r_t[at + e] == col ? 1.f : 0.f)) * f[e] : pr * f[e];
+                        db = SPLIT ? fmaf(w[e], inv[e], db) : db + w[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        auto store = [&](unsigned own, short *to) {
+                            const unsigned other = __builtin_amdgcn_update_dpp(0, own, 0xB1, 0xF, 0xF, true);  // lane ^ 1
+                            *(unsigned *)(to + (long long)(p * 32 + 8 * s + e) * a.ldg) = __builtin_amdgcn_perm(other, own, sel);
+                        };
+                        if constexpr (SPLIT) {
+                            short h1[2], h2[2];
+                            split(w[e], h1[0], h2[0]);
+                            split(w[e + 1], h1[1], h2[1]);
+                            store((unsigned short)h1[0] | (unsigned)(unsigned short)h1[1] << 16, out);
+                            store((unsigned short)h2[0] | (unsigned)(unsigned short)h2[1] << 16, out + a.gplane);
+                        } else if constexpr (F16) {
+                            store((unsigned short)bits((_Float16)w[e]) | (unsigned)(unsigned short)bits((_Float16)w[e + 1]) << 16, out);
+                        } else {
+                            store((unsigned short)bits((__bf16)w[e]) | (unsigned)(unsigned short)bits((__bf16)w[e + 1]) << 16, out);
+                        }
+                    }
+                }
+            }
+            if (a.dbias) {
+                db += __shfl_xor(db, 32);
+                if (lh == 0) a.dbias[(long long)(bi * C::VI + wi) * a.ldg + col] = db;
+            }
+        }
+    };
+    G::run(a.x, a.W, (a.nv - st + a.ns - 1) / a.ns, tile, 0, a.nk, a.passes, lds, begin, done);
 }
 
 // lse and loss of the rows from the tiles' parts: one wave a row
@@ -345,32 +426,86 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2 *part, int n, in
     loss[m] = t == ignore ? 0.f : t < 0 || t >= V ? __builtin_nanf("") : l - hit[m];
 }
 
-struct SumArgs {  // dx: C[z][i][j] = (or +=) the z-th part of the k-steps
+struct SumArgs {  // C[z][i][j] = (or +=) the z-th part of the k-steps
     Operand A, B;
     int nk, per, passes, ti, tj, I, J, add;
     float *out;
 };
-template <class C, bool F16> __global__ __launch_bounds__(C::NT) void sum_kernel(const SumArgs a) {
-    typedef Gemm<C, false, F16> G;
+struct OutArgs {  // C[i][j] * post, in the elements' type
+    Operand A, B;
+    int nk, passes, ti, tj, I, J;
+    const float *post;
+    void *out;
+    long long ld;
+    int elem;
+};
+__device__ __forceinline__ void clear(f32x16 &v) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) v[r] = 0.f;
+}
+template <class C, bool KMAJOR, bool F16> __global__ __launch_bounds__(C::NT, 2) void sum_kernel(const SumArgs a) {
+    typedef Gemm<C, KMAJOR, F16> G;
     __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
     int bi, bj;
     tile_of(blockIdx.x, a.ti, a.tj, bi, bj);
     const int k0 = blockIdx.y * a.per, k1 = k0 + a.per < a.nk ? k0 + a.per : a.nk;
-    f32x16 acc[C::WI][C::WJ];
-    G::run(a.A, a.B, bi * C::BI, bj * C::BJ, k0, k1, a.passes, lds, acc);
     const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5, wave = threadIdx.x >> 6;
     const int wi0 = bi * C::BI + (wave / C::VJ) * (C::WI * 32), wj0 = bj * C::BJ + (wave % C::VJ) * (C::WJ * 32);
+    auto begin = [&](int, f32x16 (&acc)[C::WI][C::WJ]) {
 #pragma unroll
-    for (int p = 0; p < C::WI; ++p)
+        for (int p = 0; p < C::WI; ++p)
 #pragma unroll
-        for (int q = 0; q < C::WJ; ++q)
+            for (int q = 0; q < C::WJ; ++q) clear(acc[p][q]);
+    };
+    auto done = [&](int, f32x16 (&acc)[C::WI][C::WJ]) {
+        float *o = a.out + ((long long)blockIdx.y * a.I + wi0 + 4 * lh) * a.J + wj0 + li;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = wi0 + p * 32 + block_row(r, lh), j = wj0 + q * 32 + li;
-                if (i >= a.I || j >= a.J) continue;
-                float *o = a.out + ((long long)blockIdx.y * a.I + i) * a.J + j;
-                *o = a.add ? *o + acc[p][q][r] : acc[p][q][r];
-            }
+        for (int p = 0; p < C::WI; ++p)
+#pragma unroll
+            for (int q = 0; q < C::WJ; ++q)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    if (wi0 + p * 32 + block_row(r, lh) >= a.I || wj0 + q * 32 + li >= a.J) continue;
+                    float *to = o + (long long)(p * 32 + block_row(r, 0)) * a.J + q * 32;
+                    *to = a.add ? *to + acc[p][q][r] : acc[p][q][r];
+                }
+    };
+    G::run(a.A, a.B, 1, [&](int) { return TileAt{bi * C::BI, bj * C::BJ}; }, k0, k1, a.passes, lds, begin, done);
+}
+template <class C, bool F16> __global__ __launch_bounds__(C::NT, 2) void out_kernel(const OutArgs a) {
+    typedef Gemm<C, true, F16> G;
+    __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
+    int bi, bj;
+    tile_of(blockIdx.x, a.ti, a.tj, bi, bj);
+    const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5, wave = threadIdx.x >> 6;
+    const int wi0 = bi * C::BI + (wave / C::VJ) * (C::WI * 32), wj0 = bj * C::BJ + (wave % C::VJ) * (C::WJ * 32);
+    const float post = a.post[0];
+    auto begin = [&](int, f32x16 (&acc)[C::WI][C::WJ]) {
+#pragma unroll
+        for (int p = 0; p < C::WI; ++p)
+#pragma unroll
+            for (int q = 0; q < C::WJ; ++q) clear(acc[p][q]);
+    };
+    auto done = [&](int, f32x16 (&acc)[C::WI][C::WJ]) {
+        const long long at = (long long)(wi0 + 4 * lh) * a.ld + wj0 + li;
+#pragma unroll
+        for (int p = 0; p < C::WI; ++p)
+#pragma unroll
+            for (int q = 0; q < C::WJ; ++q)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (wi0 + p * 32 + block_row(r, lh) < a.I && wj0 + q * 32 + li < a.J)
+                        write_elem(a.out, a.elem, at + (long long)(p * 32 + block_row(r, 0)) * a.ld + q * 32, acc[p][q][r] * post);
+    };
+    G::run(a.A, a.B, 1, [&](int) { return TileAt{bi * C::BI, bj * C::BJ}; }, 0, a.nk, a.passes, lds, begin, done);
+}
+// C = sum over z of the parts, for a dW whose k-steps were split
+__global__ __launch_bounds__(256) void join_kernel(const float *part, int n, int I, int J, const float *post, void *out, long long ld, int elem) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (long long)I * J) return;
+    float v = 0.f;
+    for (int z = 0; z < n; ++z) v += part[(long long)z * I * J + i];
+    write_elem(out, elem, i / J * ld + i % J, v * post[0]);
 }
 // dx[m][d] = sum over z, with the scales undone
 __global__ __launch_bounds__(256) void dx_kernel(const float *part, int n, int M, int D, const float *wscale, const float *xscale,
@@ -385,40 +520,13 @@ __global__ __launch_bounds__(256) void dx_kernel(const float *part, int n, int M
     write_elem(dx, elem, i, targets[m] == ignore ? 0.f : v);
 }
 
-struct OutArgs {  // dW: both operands k-major
-    Operand A, B;
-    int nk, passes, ti, tj, I, J;
-    const float *post;
-    void *out;
-    long long ld;
-    int elem;
-};
-template <class C, bool F16> __global__ __launch_bounds__(C::NT) void out_kernel(const OutArgs a) {
-    typedef Gemm<C, true, F16> G;
-    __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
-    int bi, bj;
-    tile_of(blockIdx.x, a.ti, a.tj, bi, bj);
-    f32x16 acc[C::WI][C::WJ];
-    G::run(a.A, a.B, bi * C::BI, bj * C::BJ, 0, a.nk, a.passes, lds, acc);
-    const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5, wave = threadIdx.x >> 6;
-    const int wi0 = bi * C::BI + (wave / C::VJ) * (C::WI * 32), wj0 = bj * C::BJ + (wave % C::VJ) * (C::WJ * 32);
-    const float post = a.post[0];
-#pragma unroll
-    for (int p = 0; p < C::WI; ++p)
-#pragma unroll
-        for (int q = 0; q < C::WJ; ++q)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = wi0 + p * 32 + block_row(r, lh), j = wj0 + q * 32 + li;
-                if (i < a.I && j < a.J) write_elem(a.out, a.elem, i * a.ld + j, acc[p][q][r] * post);
-            }
-}
-__global__ __launch_bounds__(256) void dbias_kernel(const float *part, int n, long long ld, int J, int elem, void *out, long long at) {
+__global__ __launch_bounds__(256) void dbias_kernel(const float *part, int n, long long ld, int J, const float *post, int elem, void *out,
+                                                    long long at) {
     const int j = blockIdx.x * 256 + threadIdx.x;
     if (j >= J) return;
     float v = 0.f;
     for (int i = 0; i < n; ++i) v += part[i * ld + j];
-    write_elem(out, elem, at + j, v);
+    write_elem(out, elem, at + j, v * post[0]);
 }
 __global__ void zero_elem_kernel(void *p, int elem, long long n) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -428,7 +536,7 @@ __global__ void zero_elem_kernel(void *p, int elem, long long n) {
 inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 inline long long up(long long a, long long b) { return (a + b - 1) / b * b; }
 
-constexpr long long PIECE_BYTES = 1ll << 30;  // G of one piece of the vocabulary
+constexpr long long PIECE_BYTES = 3ll << 29;  // G of one piece of the vocabulary
 
 }  // namespace
 
@@ -489,101 +597,201 @@ int tsc_unembed_create_(tsc_unembed **out, int D, int V, int elem, const void *W
 // ------------------------------------------------------------------------------------------------ launches
 namespace {
 
-// What a call keeps in its workspace, in this order (each part starts at a multiple of 256 bytes)
-struct Plan {
-    int Mp, tile, bi, bj, ti, tj;      // logits: i = v (of a piece), j = m
-    int Vc, pieces;                    // backward: entries of a piece
-    int z, per;                        // dx: parts of a piece's k-steps, k-steps of a part
-    long long xp, xscale, part, hit, rowf, post, g, db, dx, bytes;
+// Tiles of a launch.  LARGE: one workgroup a CU; MEDIUM: two; FEW (64 rows of x at most): three.
+enum { LARGE, MEDIUM, FEW };
+constexpr int CUS = 256;
+struct Shape {
+    int kind, bi, bj, slots;
 };
-int tile_for(long long I, long long J) {
-    if (J <= 64) return 2;
-    return (long long)cdiv(I, 256) * cdiv(J, 256) >= 256 ? 0 : 1;  // the large tile once it fills the chip
+Shape shape_of(int kind) {  // bi: rows of x (products of logits), or of the result
+    return kind == LARGE ? Shape{LARGE, 256, 256, CUS} : kind == MEDIUM ? Shape{MEDIUM, 128, 128, 2 * CUS} : Shape{FEW, 64, 128, 3 * CUS};
 }
-void tile_size(int t, int &bi, int &bj) {
-    bi = t == 0 ? 256 : 128;
-    bj = t == 0 ? 256 : t == 1 ? 128 : 64;
+
+// Logits: blocks of rows x streams of vocabulary tiles.  A stream's length times the rounds of workgroups is what a CU does;
+// at least four streams a block where there are many blocks, so that the tiles resident on an XCD share its L2.
+struct Streams {
+    Shape s;
+    int nm, nv, ns;
+};
+Streams streams(long long M, long long V) {
+    Streams r{};
+    r.s = shape_of(M <= 64 ? FEW : cdiv(M, 256) * (long long)cdiv(V, 256) >= CUS ? LARGE : MEDIUM);
+    r.nm = cdiv(M, r.s.bi);
+    r.nv = cdiv(V, r.s.bj);
+    long long best = -1;
+    for (int ns = r.nv < 4 ? r.nv : 4; ns <= r.nv; ++ns) {
+        const long long cost = (long long)cdiv((long long)r.nm * ns, r.s.slots) * cdiv(r.nv, ns);
+        if (best < 0 || cost < best) best = cost, r.ns = ns;
+        if ((long long)r.nm * ns >= 4ll * r.s.slots) break;
+    }
+    return r;
 }
-Plan plan(const tsc_unembed *h, long long M, bool backward, bool want_x, bool want_b) {
+
+// A product of I x J with nk k-steps: tiles and the parts that its k-steps are split into, by the time of the slowest CU
+// (k-steps of a LARGE tile cost 4 units, of a MEDIUM one, two of which share a CU, 2.5) plus the traffic of the fp32 parts.
+struct Split {
+    Shape s;
+    int ti, tj, z, per;
+};
+Split split_of(long long I, long long J, int nk, int passes, bool always_parts) {
+    Split best{};
+    double least = 0;
+    for (int kind : {LARGE, MEDIUM}) {
+        Split r{};
+        r.s = shape_of(kind);
+        r.ti = cdiv(I, r.s.bi);
+        r.tj = cdiv(J, r.s.bj);
+        const double step = kind == LARGE ? 1.6e-6 : 1.0e-6, part = (double)I * J * 8 / 4e12;
+        for (int z = 1; z <= 64 && z <= nk; ++z) {
+            r.per = cdiv(nk, z);
+            r.z = cdiv(nk, r.per);
+            const double cost = (double)cdiv((long long)r.ti * r.tj * r.z, r.s.slots) * (r.per * passes + 3) * step +
+                                (r.z > 1 || always_parts ? r.z * part : 0);
+            if (least == 0 || cost < least) least = cost, best = r;
+        }
+    }
+    return best;
+}
+
+// What a call keeps in its workspace (each part starts at a multiple of 256 bytes)
+struct Plan {
+    int Mp;
+    Streams st;
+    int Vc, pieces;  // backward: entries of a piece
+    Split dx;        // of a whole piece
+    long long xp, xscale, part, hit, rowf, post, g, db, dxp, dwp, bytes;
+};
+Split dw_split(const tsc_unembed *h, long long Mp, int nv) {
+    return h->sv == 1 ? split_of(h->D, nv, (int)(Mp / BK), h->planes == 2 ? 3 : 1, false)
+                      : split_of(nv, h->D, (int)(Mp / BK), h->planes == 2 ? 3 : 1, false);
+}
+Plan plan(const tsc_unembed *h, long long M, bool backward, bool want_x, bool want_w, bool want_b) {
     Plan p{};
     p.Mp = (int)up(M, BK);
-    p.Vc = h->Vp;
+    int nv = h->V;
     if (backward) {
-        const long long fit = PIECE_BYTES / (2ll * h->planes * p.Mp) / 256 * 256;
-        p.Vc = (int)(fit < 256 ? 256 : fit < h->Vp ? fit : h->Vp);
+        // tiles of a piece: what fits PIECE_BYTES, and of that the number whose dW fills whole rounds of the chip best
+        const int all = cdiv(h->V, 256), dt = cdiv(h->D, 256);
+        long long fit = PIECE_BYTES / (2ll * h->planes * p.Mp * 256);
+        int vt = (int)(fit < 1 ? 1 : fit < all ? fit : all);
+        if (vt < all) {
+            double best = 0;
+            int pick = vt;
+            for (int t = vt; t > vt / 2; --t) {
+                const double full = (double)t * dt / (CUS * cdiv((long long)t * dt, CUS));
+                if (full > best + 0.01) best = full, pick = t;
+            }
+            vt = pick;
+        }
+        p.Vc = vt * 256;
+        p.pieces = cdiv(h->V, p.Vc);
+        if (p.Vc < nv) nv = p.Vc;
     }
-    p.pieces = cdiv(h->V, p.Vc);
-    p.tile = tile_for(p.Vc < h->V ? p.Vc : h->V, M);
-    tile_size(p.tile, p.bi, p.bj);
-    p.ti = cdiv(p.Vc < h->V ? p.Vc : h->V, p.bi);
-    p.tj = cdiv(M, p.bj);
+    p.st = streams(M, nv);
     long long at = 0;
     auto take = [&](long long n) { const long long q = at; at = up(at + n, 256); return q; };
     p.xp = take(2ll * h->planes * p.Mp * h->Dp);
     p.xscale = take(4 * M);
     if (!backward) {
-        p.part = take(8ll * p.ti * M);
+        p.part = take(8ll * p.st.ns * M);
         p.hit = take(4 * M);
     } else {
         p.rowf = take(4 * M);
         p.post = take(4);
         p.g = take(2ll * h->planes * p.Mp * p.Vc);
-        if (want_b) p.db = take(4ll * p.tj * p.Vc);
+        if (want_b) p.db = take(4ll * 2 * p.st.nm * p.Vc);
         if (want_x) {
-            const int nk = p.Vc / BK, t = tile_for(M, h->D) == 0 ? 0 : 1;
-            int bi, bj;
-            tile_size(t, bi, bj);
-            const long long tiles = (long long)cdiv(M, bi) * cdiv(h->D, bj);
-            long long z = cdiv(t == 0 ? 256 : 512, tiles);
-            if (z > nk / 8) z = nk / 8;
-            if (z < 1) z = 1;
-            p.per = cdiv(nk, z);
-            p.z = cdiv(nk, p.per);
-            p.dx = take(4ll * p.z * M * h->D);
+            p.dx = split_of(M, h->D, cdiv(nv, BK), h->planes == 2 ? 3 : 1, true);
+            p.dxp = take(4ll * p.dx.z * M * h->D);
+        }
+        if (want_w) {  // a piece's dW and the last, shorter one's may be split differently
+            long long most = 0;
+            for (int n : {nv, h->V - (p.pieces - 1) * p.Vc}) {
+                const Split w = dw_split(h, p.Mp, n);
+                if (w.z > 1 && (long long)w.z * n > most) most = (long long)w.z * n;
+            }
+            p.dwp = take(4ll * most * h->D);
         }
     }
     p.bytes = at;
     return p;
 }
 
-template <bool F16, bool GRAD> int launch_logits(int tile, const LogitArgs &a, hipStream_t s) {
-    const dim3 grid(a.ti * a.tj);
-    if (tile == 0) hipLaunchKernelGGL((logits_kernel<TileLarge, F16, GRAD>), grid, dim3(TileLarge::NT), 0, s, a);
-    else if (tile == 1) hipLaunchKernelGGL((logits_kernel<TileMedium, F16, GRAD>), grid, dim3(TileMedium::NT), 0, s, a);
-    else hipLaunchKernelGGL((logits_kernel<TileSkinny, F16, GRAD>), grid, dim3(TileSkinny::NT), 0, s, a);
+template <bool F16, bool SPLIT, bool GRAD> int launch_logits(const Streams &st, const LogitArgs &a, hipStream_t s) {
+    const dim3 grid(a.nm * a.ns);
+#define TSC_LOGITS(T1, T2)                                                                                                     \
+    {                                                                                                                          \
+        if (GRAD) hipLaunchKernelGGL((grad_logits_kernel<T1, F16, SPLIT>), grid, dim3(T1::NT), 0, s, a);                      \
+        else hipLaunchKernelGGL((loss_logits_kernel<T2, F16, SPLIT>), grid, dim3(T2::NT), 0, s, a);                           \
+    }
+    if (st.s.kind == LARGE) TSC_LOGITS(TileLarge, TileLarge)
+    else if (st.s.kind == MEDIUM) TSC_LOGITS(TileMedium, TileMedium)
+    else TSC_LOGITS(TileWide, TileTall)
+#undef TSC_LOGITS
     TSC_HIP_CHECK(hipGetLastError());
     return TSC_OK;
+}
+template <bool GRAD> int logits(const tsc_unembed *h, const Streams &st, const LogitArgs &a, hipStream_t s) {
+    return h->elem == TSC_ELEM_F32    ? launch_logits<true, true, GRAD>(st, a, s)
+           : h->elem == TSC_ELEM_BF16 ? launch_logits<false, false, GRAD>(st, a, s)
+                                      : launch_logits<true, false, GRAD>(st, a, s);
 }
 LogitArgs logit_args(const tsc_unembed *h, const Plan &p, char *ws, int M, const long long *targets, long long ignore) {
     LogitArgs a{};
     a.W = {h->Wt, (long long)h->planes * h->Dp, h->Dp, h->V};
     a.x = {(const short *)(ws + p.xp), (long long)h->planes * h->Dp, h->Dp, M};
     a.nk = h->Dp / BK; a.passes = h->planes == 2 ? 3 : 1;
-    a.ti = p.ti; a.tj = p.tj; a.M = M; a.V = h->V;
+    a.nm = p.st.nm; a.ns = p.st.ns; a.nv = p.st.nv; a.M = M; a.V = h->V;
     a.bias = h->bias32;
     a.wscale = h->planes == 2 ? h->wscale : nullptr;
     a.xscale = h->planes == 2 ? (const float *)(ws + p.xscale) : nullptr;
-    a.targets = targets; a.ignore = ignore; a.planes = h->planes;
+    a.targets = targets; a.ignore = ignore;
     return a;
+}
+template <bool KMAJOR> int launch_sum(const Split &w, bool f16, SumArgs &q, hipStream_t s) {
+    q.per = w.per; q.ti = w.ti; q.tj = w.tj;
+    const dim3 grid(w.ti * w.tj, w.z);
+    if (w.s.kind == LARGE) {
+        if (f16) hipLaunchKernelGGL((sum_kernel<TileLarge, KMAJOR, true>), grid, dim3(TileLarge::NT), 0, s, q);
+        else hipLaunchKernelGGL((sum_kernel<TileLarge, KMAJOR, false>), grid, dim3(TileLarge::NT), 0, s, q);
+    } else {
+        if (f16) hipLaunchKernelGGL((sum_kernel<TileMedium, KMAJOR, true>), grid, dim3(TileMedium::NT), 0, s, q);
+        else hipLaunchKernelGGL((sum_kernel<TileMedium, KMAJOR, false>), grid, dim3(TileMedium::NT), 0, s, q);
+    }
+    TSC_HIP_CHECK(hipGetLastError());
+    return TSC_OK;
+}
+int launch_out(const Split &w, bool f16, OutArgs &q, hipStream_t s) {
+    q.ti = w.ti; q.tj = w.tj;
+    const dim3 grid(w.ti * w.tj);
+    if (w.s.kind == LARGE) {
+        if (f16) hipLaunchKernelGGL((out_kernel<TileLarge, true>), grid, dim3(TileLarge::NT), 0, s, q);
+        else hipLaunchKernelGGL((out_kernel<TileLarge, false>), grid, dim3(TileLarge::NT), 0, s, q);
+    } else {
+        if (f16) hipLaunchKernelGGL((out_kernel<TileMedium, true>), grid, dim3(TileMedium::NT), 0, s, q);
+        else hipLaunchKernelGGL((out_kernel<TileMedium, false>), grid, dim3(TileMedium::NT), 0, s, q);
+    }
+    TSC_HIP_CHECK(hipGetLastError());
+    return TSC_OK;
 }
 
 }  // namespace
 
-size_t tsc_unembed_workspace_(const tsc_unembed *h, long long M, int backward, int want_x, int want_b) {
-    return M < 1 ? 0 : (size_t)plan(h, M, backward, want_x, want_b).bytes;
+size_t tsc_unembed_workspace_(const tsc_unembed *h, long long M, int backward, int want_x, int want_w, int want_b) {
+    return M < 1 ? 0 : (size_t)plan(h, M, backward, want_x, want_w, want_b).bytes;
 }
 
 int tsc_launch_unembed_loss(const tsc_unembed *h, const TscRows &x, int M, const long long *targets, long long ignore, float *loss,
                             float *lse, char *ws, hipStream_t s) {
-    const Plan p = plan(h, M, false, false, false);
+    const Plan p = plan(h, M, false, false, false, false);
     hipLaunchKernelGGL(pack_x_kernel, dim3(cdiv(p.Mp, 4)), dim3(256), 0, s, x, h->elem, M, p.Mp, h->D, h->Dp, (const long long *)nullptr, ignore,
                        (short *)(ws + p.xp), (float *)(ws + p.xscale));
     LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
     a.part = (float2 *)(ws + p.part);
     a.hit = (float *)(ws + p.hit);
-    const int rc = h->elem == TSC_ELEM_BF16 ? launch_logits<false, false>(p.tile, a, s) : launch_logits<true, false>(p.tile, a, s);
+    const int rc = logits<false>(h, p.st, a, s);
     if (rc) return rc;
-    hipLaunchKernelGGL(loss_kernel, dim3(cdiv(M, 4)), dim3(256), 0, s, a.part, p.ti, M, h->V, a.hit, targets, ignore, loss, lse);
+    hipLaunchKernelGGL(loss_kernel, dim3(cdiv(M, 4)), dim3(256), 0, s, a.part, p.st.ns, M, h->V, a.hit, targets, ignore, loss, lse);
     TSC_HIP_CHECK(hipGetLastError());
     return TSC_OK;
 }
@@ -591,73 +799,67 @@ int tsc_launch_unembed_loss(const tsc_unembed *h, const TscRows &x, int M, const
 int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscRows &x, int M, const long long *targets, long long ignore,
                                 const float *lse, void *dx, void *dW, void *db, char *ws, hipStream_t s) {
     const bool f16 = h->elem != TSC_ELEM_BF16;
+    const int passes = h->planes == 2 ? 3 : 1;
     if (M == 0) {
         if (dW) hipLaunchKernelGGL(zero_elem_kernel, dim3(cdiv((long long)h->D * h->V, 256)), dim3(256), 0, s, dW, h->elem, (long long)h->D * h->V);
         if (db) hipLaunchKernelGGL(zero_elem_kernel, dim3(cdiv(h->V, 256)), dim3(256), 0, s, db, h->belem, (long long)h->V);
         TSC_HIP_CHECK(hipGetLastError());
         return TSC_OK;
     }
-    const Plan p = plan(h, M, true, dx != nullptr, db != nullptr);
+    const Plan p = plan(h, M, true, dx != nullptr, dW != nullptr, db != nullptr);
     short *xp = (short *)(ws + p.xp), *G = (short *)(ws + p.g);
-    float *xscale = (float *)(ws + p.xscale), *rowf = (float *)(ws + p.rowf), *post = (float *)(ws + p.post), *dxp = (float *)(ws + p.dx);
+    float *xscale = (float *)(ws + p.xscale), *rowf = (float *)(ws + p.rowf), *post = (float *)(ws + p.post), *dxp = (float *)(ws + p.dxp);
     hipLaunchKernelGGL(pack_x_kernel, dim3(cdiv(p.Mp, 4)), dim3(256), 0, s, x, h->elem, M, p.Mp, h->D, h->Dp, targets, ignore, xp, xscale);
     hipLaunchKernelGGL(row_factor_kernel, dim3(1), dim3(1024), 0, s, g, xscale, targets, ignore, h->V, M, f16, rowf, post);
     LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
-    a.lse = lse; a.rowf = rowf; a.G = G; a.ldg = p.Vc; a.gplane = (long long)p.Mp * p.Vc; a.Mp = p.Mp; a.f16 = f16;
+    a.lse = lse; a.rowf = rowf; a.G = G; a.ldg = p.Vc; a.gplane = (long long)p.Mp * p.Vc; a.Mp = p.Mp;
     a.dbias = db ? (float *)(ws + p.db) : nullptr;
-    a.g = g;
     const long long xld = (long long)h->planes * h->Dp;
+    const int db_parts = p.st.nm * (p.st.s.kind == FEW ? 1 : 2);  // waves of a tile's rows
     for (int c = 0; c < p.pieces; ++c) {
-        const int v0 = c * p.Vc, nv = h->V - v0 < p.Vc ? h->V - v0 : p.Vc, nvp = (int)up(nv, p.bi);
+        const int v0 = c * p.Vc, nv = h->V - v0 < p.Vc ? h->V - v0 : p.Vc;
         a.v0 = v0;
-        a.ti = nvp / p.bi;
-        int rc = f16 ? launch_logits<true, true>(p.tile, a, s) : launch_logits<false, true>(p.tile, a, s);
+        a.nv = cdiv(nv, p.st.s.bj);
+        a.ns = p.st.ns < a.nv ? p.st.ns : a.nv;
+        int rc = logits<true>(h, p.st, a, s);
         if (rc) return rc;
-        if (db) hipLaunchKernelGGL(dbias_kernel, dim3(cdiv(nv, 256)), dim3(256), 0, s, a.dbias, p.tj, a.ldg, nv, h->belem, db, (long long)v0);
+        if (db) hipLaunchKernelGGL(dbias_kernel, dim3(cdiv(nv, 256)), dim3(256), 0, s, a.dbias, db_parts, a.ldg, nv, post, h->belem, db, (long long)v0);
         if (dx) {
             SumArgs q{};
             q.A = {G, p.Vc, a.gplane, M};
             q.B = {h->Wd + v0, (long long)h->planes * h->Vp, h->Vp, h->D};
-            q.nk = nvp / BK; q.per = p.per; q.passes = a.passes; q.I = M; q.J = h->D; q.add = c > 0; q.out = dxp;
-            const int t = tile_for(M, h->D) == 0 ? 0 : 1;
-            int bi, bj;
-            tile_size(t, bi, bj);
-            q.ti = cdiv(M, bi); q.tj = cdiv(h->D, bj);
-            const dim3 grid(q.ti * q.tj, c == 0 ? p.z : cdiv(q.nk, p.per));
-            if (t == 0) {
-                if (f16) hipLaunchKernelGGL((sum_kernel<TileLarge, true>), grid, dim3(TileLarge::NT), 0, s, q);
-                else hipLaunchKernelGGL((sum_kernel<TileLarge, false>), grid, dim3(TileLarge::NT), 0, s, q);
-            } else {
-                if (f16) hipLaunchKernelGGL((sum_kernel<TileMedium, true>), grid, dim3(TileMedium::NT), 0, s, q);
-                else hipLaunchKernelGGL((sum_kernel<TileMedium, false>), grid, dim3(TileMedium::NT), 0, s, q);
-            }
+            q.nk = cdiv(nv, BK); q.passes = passes; q.I = M; q.J = h->D; q.add = c > 0; q.out = dxp;
+            Split w = p.dx;
+            if (c > 0) w.per = cdiv(q.nk, w.z);  // the same parts, shorter
+            rc = launch_sum<false>(w, f16, q, s);
+            if (rc) return rc;
         }
         if (dW) {
-            OutArgs q{};
             const Operand X = {xp, xld, h->Dp, h->D}, Gk = {G, p.Vc, a.gplane, nv};
             const bool by_d = h->sv == 1;  // dW is dense in W's order: [D][V] or [V][D]
-            q.A = by_d ? X : Gk;
-            q.B = by_d ? Gk : X;
-            q.nk = p.Mp / BK; q.passes = a.passes; q.I = by_d ? h->D : nv; q.J = by_d ? nv : h->D;
-            q.post = post; q.elem = h->elem; q.ld = by_d ? h->V : h->D;
-            const long long first = by_d ? v0 : (long long)v0 * h->D;
-            q.out = (char *)dW + first * (h->elem == TSC_ELEM_F32 ? 4 : 2);
-            const int t = tile_for(q.I, q.J) == 0 ? 0 : 1;
-            int bi, bj;
-            tile_size(t, bi, bj);
-            q.ti = cdiv(q.I, bi); q.tj = cdiv(q.J, bj);
-            const dim3 grid(q.ti * q.tj);
-            if (t == 0) {
-                if (f16) hipLaunchKernelGGL((out_kernel<TileLarge, true>), grid, dim3(TileLarge::NT), 0, s, q);
-                else hipLaunchKernelGGL((out_kernel<TileLarge, false>), grid, dim3(TileLarge::NT), 0, s, q);
+            const Split w = dw_split(h, p.Mp, nv);
+            const int I = by_d ? h->D : nv, J = by_d ? nv : h->D;
+            const long long first = by_d ? v0 : (long long)v0 * h->D, ld = by_d ? h->V : h->D;
+            void *out = (char *)dW + first * (h->elem == TSC_ELEM_F32 ? 4 : 2);
+            if (w.z == 1) {
+                OutArgs q{};
+                q.A = by_d ? X : Gk;
+                q.B = by_d ? Gk : X;
+                q.nk = p.Mp / BK; q.passes = passes; q.I = I; q.J = J; q.post = post; q.elem = h->elem; q.ld = ld; q.out = out;
+                rc = launch_out(w, f16, q, s);
             } else {
-                if (f16) hipLaunchKernelGGL((out_kernel<TileMedium, true>), grid, dim3(TileMedium::NT), 0, s, q);
-                else hipLaunchKernelGGL((out_kernel<TileMedium, false>), grid, dim3(TileMedium::NT), 0, s, q);
+                SumArgs q{};
+                q.A = by_d ? X : Gk;
+                q.B = by_d ? Gk : X;
+                q.nk = p.Mp / BK; q.passes = passes; q.I = I; q.J = J; q.out = (float *)(ws + p.dwp);
+                rc = launch_sum<true>(w, f16, q, s);
+                if (!rc) hipLaunchKernelGGL(join_kernel, dim3(cdiv((long long)I * J, 256)), dim3(256), 0, s, q.out, w.z, I, J, post, out, ld, h->elem);
             }
+            if (rc) return rc;
         }
         TSC_HIP_CHECK(hipGetLastError());
     }
-    if (dx) hipLaunchKernelGGL(dx_kernel, dim3(cdiv((long long)M * h->D, 256)), dim3(256), 0, s, dxp, p.z, M, h->D,
+    if (dx) hipLaunchKernelGGL(dx_kernel, dim3(cdiv((long long)M * h->D, 256)), dim3(256), 0, s, dxp, p.dx.z, M, h->D,
                                a.wscale, a.xscale, post, targets, ignore, h->elem, dx);
     TSC_HIP_CHECK(hipGetLastError());
     return TSC_OK;

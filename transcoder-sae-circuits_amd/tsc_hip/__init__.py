@@ -83,7 +83,7 @@ _SIGNATURES = {
                                       _c.c_int64, _c.c_void_p, _c.c_int, _c.c_void_p]),
     "tsc_unembed_refresh": (_c.c_int, [_c.c_void_p, _c.c_void_p]),
     "tsc_unembed_destroy": (_c.c_int, [_c.c_void_p]),
-    "tsc_unembed_workspace_bytes": (_c.c_size_t, [_c.c_void_p, _c.c_int64, _c.c_int, _c.c_int, _c.c_int]),
+    "tsc_unembed_workspace_bytes": (_c.c_size_t, [_c.c_void_p, _c.c_int64, _c.c_int, _c.c_int, _c.c_int, _c.c_int]),
     "tsc_unembed_loss": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p,
                                     _c.c_void_p, _c.c_size_t, _c.c_void_p]),
     "tsc_unembed_loss_backward": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64,
@@ -1079,7 +1079,7 @@ class UnembedHead:
         loss = torch.empty(targets.shape, dtype=torch.float32, device=self.device)
         lse = torch.empty_like(loss)
         with torch.cuda.device(self.device):
-            ws, n = self._workspace(m, 0, 0, 0)
+            ws, n = self._workspace(m, 0, 0, 0, 0)
             _check(lib().tsc_unembed_loss(self._handle, ctypes.byref(rows), m, targets.data_ptr(), int(ignore_index),
                                           loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), n, _stream()))
         return loss, lse
@@ -1102,7 +1102,7 @@ class UnembedHead:
                              device=self.device)
         db = torch.empty_like(self.b_U) if want_bias and self.b_U is not None else None
         with torch.cuda.device(self.device):
-            ws, n = self._workspace(m, 1, int(dx is not None), int(db is not None))
+            ws, n = self._workspace(m, 1, int(dx is not None), int(dW is not None), int(db is not None))
             _check(lib().tsc_unembed_loss_backward(self._handle, dloss.data_ptr(), ctypes.byref(rows), m, targets.data_ptr(),
                                                    int(ignore_index), lse.data_ptr(), _ptr(dx), _ptr(dW), _ptr(db), ws.data_ptr(),
                                                    n, _stream()))
