@@ -438,8 +438,8 @@ int tsc_layer_norm_backward(int elem, const tsc_rows_t *dy, const tsc_rows_t *x,
  * the unembedding is passed as its transpose: stride_d 1, stride_v d_model), the other one at least as long as the axis it
  * steps over.  bias [d_vocab] in bias_elem or NULL; an entry below -1e38 takes that token out
  * (probability 0; a row for which none is left has the loss NaN).  Both are borrowed.
- * The handle owns what the matrix pipe reads: W in both orders, padded, in 16 bits -- for TSC_ELEM_F32 as two fp16 planes
- * that hold 22 bits of every weight down to 2^-27 of the largest and a fixed 2^-49 of it below -- 2 x 77 MB (fp32: 2 x 154)
+ * The handle owns what the matrix pipe reads: W in both orders, padded, in 16 bits -- for TSC_ELEM_F32 as fp16 planes
+ * that hold 22 bits of every weight down to 2^-17 of the largest and a fixed 2^-39 of it below -- 2 x 77 MB (fp32: 154 + 232)
  * at 768 x 50257.  After an in-place change of W or bias call tsc_unembed_refresh, in order with the calls that use the
  * handle.  d_model <= 32768, d_vocab <= 2^20.  One handle may be used from several streams.
  */
@@ -452,7 +452,8 @@ int tsc_unembed_destroy(tsc_unembed_t *head);
 /*
  * Cross entropy of `rows` rows x [rows, d_model] (the handle's type) against their targets:
  *   l = x W + b,  lse[m] = log sum_v exp l[m][v],  loss[m] = lse[m] - l[m][targets[m]],
- * loss and lse [rows] fp32 for every type (products exact, sums fp32); the [rows, d_vocab] logits are never stored.
+ * loss and lse [rows] fp32 for every type (products of 16-bit operands are exact, sums are fp32;
+ * a row of fp32 x is held like the weights, against its own largest element); the [rows, d_vocab] logits are never stored.
  * targets [rows] int64: ignore_index = no loss (0, whatever the row holds); any other value outside 0 .. d_vocab - 1 gives
  * NaN.  workspace: tsc_unembed_workspace_bytes(head, rows, 0, 0, 0, 0) bytes, 256-byte aligned; rows < 2^24.
  * Next-token loss of the model behind load_model_and_encoders.py:21, by which spliced-in dictionaries are judged.
@@ -469,8 +470,8 @@ int tsc_unembed_loss(const tsc_unembed_t *head, const tsc_rows_t *x, int64_t row
  * dx [rows, d_model] dense; dW dense in W's order ([d_model, d_vocab] where stride_v is 1, else [d_vocab, d_model]); dbias
  * [d_vocab] in bias_elem; each may be NULL = not wanted.  Ignored rows have a zero dx and add nothing, whatever they hold; a
  * target outside the vocabulary makes its row's dx and all of dW NaN.  G is made in pieces of the vocabulary (1.5 GiB of
- * workspace) and rounded to 16 bits as the operand of the two products (fp32: two planes, 22 bits down to 2^-27 of the
- * largest and a fixed 2^-49 of it below; fp16: 11 bits down to 2^-27, a fixed 2^-38 below; the largest: of |dloss|, for fp32
+ * workspace) and rounded to 16 bits as the operand of the two products (fp32: two planes, 22 bits down to 2^-28 of the
+ * largest and a fixed 2^-50 of it below; fp16: 11 bits down to 2^-28, a fixed 2^-39 below; the largest: of |dloss|, for fp32
  * of |dloss| times the row's largest |x|).  dbias sums unrounded values.
  * Sums are fp32 in a fixed order: the same call gives the same bits.
  * workspace: tsc_unembed_workspace_bytes(head, rows, 1, dx != NULL, dW != NULL, dbias != NULL) bytes, 256-byte aligned.

@@ -1,7 +1,7 @@
 """Cross entropy behind the unembedding (``tsc_unembed_*``, ``tsc_hip.UnembedHead``) against its definition in float64.
 
 Tolerances.  u = 2^-24.  A product of split fp32 operands is off by at most 3 * 2^-22 of its size (two residuals, the dropped
-product of the second planes), plus 2^-49 of the operands' largest; 16-bit operands multiply exactly.  Sums: Higham and Mary's
+product of the second planes), plus 2^-39 of either operand's largest times the other operand; 16-bit operands multiply exactly.  Sums: Higham and Mary's
 probabilistic bound 4 sqrt(n) u of the sum of the absolute terms for n additions (a fixed order, so a run repeats itself).
 An error e of a logit is a relative error e of its exponential; G is rounded to 16 bits as an operand (bf16 2^-8, fp16 2^-11,
 fp32 2^-22 and the floors that the header names); results are rounded once to their type."""
@@ -49,7 +49,8 @@ def reference(x, W, b, t, dloss, ignore=-100):
     passes = 3 if dt == torch.float32 else 1
     e_l = 4 * math.sqrt(passes * D) * U * mag
     if dt == torch.float32:
-        e_l += 3 * 2.0 ** -22 * mag + 2 * 2.0 ** -49 * D * xd.abs().amax(-1, keepdim=True) * wd.abs().max()
+        e_l += 3 * 2.0 ** -22 * mag + 2.0 ** -39 * (xd.abs().amax(-1, keepdim=True) * wd.abs().sum(0)
+                                                    + xd.abs().sum(-1, keepdim=True) * wd.abs().max())
     if b is not None:
         bd = b.double()
         bd = torch.where(bd < -1e38, -math.inf, bd)
@@ -72,10 +73,10 @@ def reference(x, W, b, t, dloss, ignore=-100):
     out_G, e_raw = G * g, e_G * g.abs()
     if dt == torch.float32:
         top = (xd.abs().amax(-1, keepdim=True) * g.abs()).max()
-        floor = 2.0 ** -49 * 2 * top / xd.abs().amax(-1, keepdim=True).clamp_min(1e-30)  # 2: the row's scale is a power of two
+        floor = 2.0 ** -50 * 2 * top / xd.abs().amax(-1, keepdim=True).clamp_min(1e-30)  # 2: the row's scale is a power of two
         rnd = 2.0 ** -22 * out_G.abs() + torch.where(g == 0, 0.0, floor)
     elif dt == torch.float16:
-        rnd = 2.0 ** -11 * out_G.abs() + 2.0 ** -38 * g.abs().max()
+        rnd = 2.0 ** -11 * out_G.abs() + 2.0 ** -39 * g.abs().max()
     else:
         rnd = 2.0 ** -8 * out_G.abs()
     e_op = e_raw + rnd
@@ -83,9 +84,11 @@ def reference(x, W, b, t, dloss, ignore=-100):
     aG, aw = out_G.abs(), wd.abs()
     wt = wd.t().contiguous()
     out["dx"] = (out_G @ wt, e_op @ aw.t().contiguous() + (4 * math.sqrt(passes * V) * U + passes_rel) * (aG @ aw.t().contiguous())
-                 + (2.0 ** -49 * 2 * wd.abs().max() * aG.sum(-1, keepdim=True) if dt == torch.float32 else 0.0))
+                 + (2 * 2.0 ** -39 * wd.abs().max() * aG.sum(-1, keepdim=True) if dt == torch.float32 else 0.0))
     xt = xd.t().contiguous()
-    out["dW"] = (xt @ out_G, xt.abs() @ e_op + (4 * math.sqrt(passes * M) * U + passes_rel) * (xt.abs() @ aG))
+    # (an element of x is held against its row's largest: 2^-39 of that, twice for its h1 / 2048)
+    e_x_ = 2 * 2.0 ** -39 * (xd.abs().amax(-1) @ aG) if dt == torch.float32 else 0.0
+    out["dW"] = (xt @ out_G, xt.abs() @ e_op + (4 * math.sqrt(passes * M) * U + passes_rel) * (xt.abs() @ aG) + e_x_)
     out["db"] = (out_G.sum(0), e_raw.sum(0) + 4 * math.sqrt(M) * U * aG.sum(0))
     return out
 

@@ -9,6 +9,7 @@
 // the workgroup.  Backward, in pieces of the vocabulary: G of a piece goes to the workspace in 16 bits (fp32: two fp16
 // planes), and the two products read it from there.
 #include <new>
+#include <type_traits>
 
 #include "unembed_gemm.h"
 
@@ -32,18 +33,29 @@ __device__ __forceinline__ void write_elem(void *p, int elem, long long i, float
 __device__ __forceinline__ short bits(_Float16 v) { return __builtin_bit_cast(short, v); }
 __device__ __forceinline__ short bits(__bf16 v) { return __builtin_bit_cast(short, v); }
 
-// power of two s that brings a magnitude into [2^13, 2^14) when divided by s (1 for 0, infinities and NaN)
+// power of two s that brings a magnitude into [2^14, 2^15) when divided by s (1 for 0, infinities and NaN)
 __device__ __forceinline__ float pow2_scale(float top) {
     if (!(top > 0.f) || !(top < __builtin_inff())) return 1.f;
-    const int e = (int)(__float_as_uint(top) >> 23) - 13;  // biased exponent of s; 1: the smallest normal
+    const int e = (int)(__float_as_uint(top) >> 23) - 14;  // biased exponent of s; 1: the smallest normal
     return __uint_as_float((unsigned)(e < 1 ? 1 : e) << 23);
 }
-// h1 + h2 / 2048 = v to 22 bits.  A value that fp16 does not hold (it is not finite, or NaN) goes to h1 alone.
+// h1 + h2 = v (unembed_gemm.h).  A value that fp16 does not hold (it is not finite, or NaN) goes to h1 alone.
 __device__ __forceinline__ void split(float v, short &h1, short &h2) {
     const _Float16 a = (_Float16)v;
-    const float r = (v - (float)a) * 2048.f;
     h1 = bits(a);
-    h2 = fabsf((float)a) < __builtin_inff() ? bits((_Float16)r) : (short)0;
+    h2 = fabsf((float)a) < __builtin_inff() ? bits((_Float16)(v - (float)a)) : (short)0;
+}
+// the planes of a value: one in 16 bits, or h1, h2 and (three planes) h1 / 2048, Cp elements apart
+__device__ __forceinline__ void store_planes(short *o, int Cp, float v, int elem, int planes) {
+    if (elem == TSC_ELEM_F32) {
+        short h1, h2;
+        split(v, h1, h2);
+        o[0] = h1;
+        o[Cp] = h2;
+        if (planes == 3) o[2 * Cp] = bits((_Float16)((float)__builtin_bit_cast(_Float16, h1) * (1.f / 2048.f)));
+    } else {
+        o[0] = elem == TSC_ELEM_BF16 ? bits((__bf16)v) : bits((_Float16)v);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ operands
@@ -80,7 +92,7 @@ __global__ void bias_kernel(const void *b, int elem, int V, int n, float *out) {
 
 // out[r][c] = in[r * sr + c * sc], c < C, zero up to the pitch (of a plane); one of sr, sc is 1
 __global__ __launch_bounds__(256) void pack_w_kernel(const void *in, int elem, long long sr, long long sc, int R, int C, int Cp,
-                                                     const float *wscale, short *out) {
+                                                     int planes, const float *wscale, short *out) {
     __shared__ float t[64][65];
     const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, a = threadIdx.x & 63, b = threadIdx.x >> 6;
     for (int i = b; i < 64; i += 4) {
@@ -89,15 +101,10 @@ __global__ __launch_bounds__(256) void pack_w_kernel(const void *in, int elem, l
         t[sc == 1 ? i : a][sc == 1 ? a : i] = v;
     }
     __syncthreads();
-    const int planes = elem == TSC_ELEM_F32 ? 2 : 1;
     const float inv = elem == TSC_ELEM_F32 ? 1.f / wscale[0] : 1.f;
     for (int i = b; i < 64; i += 4) {
         const int r = r0 + i, c = c0 + a;
-        if (r >= R || c >= Cp) continue;
-        const float v = t[i][a];
-        short *o = out + (long long)r * planes * Cp + c;
-        if (elem == TSC_ELEM_F32) split(v * inv, o[0], o[Cp]);
-        else o[0] = elem == TSC_ELEM_BF16 ? bits((__bf16)v) : bits((_Float16)v);
+        if (r < R && c < Cp) store_planes(out + (long long)r * planes * Cp + c, Cp, t[i][a] * inv, elem, planes);
     }
 }
 
@@ -106,11 +113,10 @@ __device__ __forceinline__ long long row_at(const TscRows &r, long long row) {
 }
 
 // One wave a row: x[m] / s_m in planes of Dp elements, rows behind M (up to Mp) and rows without a loss zero; s_m to xscale.
-__global__ __launch_bounds__(256) void pack_x_kernel(const TscRows x, int elem, int M, int Mp, int D, int Dp, const long long *targets,
-                                                     long long ignore, short *out, float *xscale) {
+__global__ __launch_bounds__(256) void pack_x_kernel(const TscRows x, int elem, int M, int Mp, int D, int Dp, int planes,
+                                                     const long long *targets, long long ignore, short *out, float *xscale) {
     const int m = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (m >= Mp) return;
-    const int planes = elem == TSC_ELEM_F32 ? 2 : 1;
     short *o = out + (long long)m * planes * Dp;
     const bool live = m < M && (!targets || targets[m] != ignore);
     const long long at = live ? row_at(x, m) : 0;
@@ -129,13 +135,13 @@ __global__ __launch_bounds__(256) void pack_x_kernel(const TscRows x, int elem, 
     const float inv = 1.f / s;
     for (int d = lane; d < Dp; d += 64) {
         const bool in = live && d < D;
-        if (elem == TSC_ELEM_F32) split(in ? ((const float *)x.data)[at + d] * inv : 0.f, o[d], o[Dp + d]);
+        if (elem == TSC_ELEM_F32) store_planes(o + d, Dp, in ? ((const float *)x.data)[at + d] * inv : 0.f, elem, planes);
         else o[d] = in ? ((const short *)x.data)[at + d] : (short)0;
     }
 }
 
 // rowf[m] = g_m s_m S (0 without a loss, NaN with a target outside the vocabulary), post[0] = 1 / S.  S = 1 for bf16, whose
-// range is fp32's; for the fp16 planes the power of two that keeps |G'| = |rowf (p - [v = t])| within 2^14.
+// range is fp32's; for the fp16 planes the power of two that keeps |G'| = |rowf (p - [v = t])| below 2^15.
 __global__ __launch_bounds__(1024) void row_factor_kernel(const float *g, const float *xscale, const long long *targets, long long ignore,
                                                           int V, int M, int f16, float *rowf, float *post) {
     __shared__ float s[17];
@@ -173,6 +179,10 @@ __device__ __forceinline__ void tile_of(int b, int ti, int tj, int &i, int &j) {
     j = r / gi;
 }
 
+__device__ __forceinline__ void clear(f32x16 &v) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) v[r] = 0.f;
+}
 // (reference, sum of 2^(l - reference)) of two sets of logits; a set of nothing but -inf is (-inf, 0)
 __device__ __forceinline__ float2 merge(float2 a, float2 b) {
     const float t = fmaxf(a.x, b.x);
@@ -204,7 +214,7 @@ struct LogitArgs {
 // costs an fma, an exponential and an add an element: sums of 2^(l - reference) are exact enough whatever the later maxima
 // are, as long as nothing overflows (the tile is then repeated with its own maximum) -- what underflows is below 2^-126 of a
 // term that is already in the sum.
-template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, 2) void loss_logits_kernel(const LogitArgs a) {
+template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::OCC) void loss_logits_kernel(const LogitArgs a) {
     typedef Gemm<C, false, F16> G;
     __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
     int bj, st;
@@ -225,7 +235,7 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, 2) 
     }
     auto tile = [&](int t) { return TileAt{(st + t * a.ns) * C::BI, j0}; };
     auto first = [&](int t) { return (st + t * a.ns) * C::BI + wi * (C::WI * 32); };
-    auto begin = [&](int t, f32x16 (&acc)[C::WI][C::WJ]) {
+    auto begin = [&](int t, f32x16 (&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
         const float *b0 = a.bias + first(t) + 4 * lh;
 #pragma unroll
         for (int p = 0; p < C::WI; ++p)
@@ -238,7 +248,7 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, 2) 
                     for (int e = 0; e < 4; ++e) acc[p][q][s * 4 + e] = b[e];  // products start from the bias
             }
     };
-    auto done = [&](int t, f32x16 (&acc)[C::WI][C::WJ]) {
+    auto done = [&](int t, f32x16 (&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
         const int wi0 = first(t);
         if (SPLIT) {
 #pragma unroll
@@ -313,7 +323,7 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, 2) 
 
 // Backward, i = m, j = v: a lane holds one entry of the vocabulary and 16 WI rows of it, so db is a sum over its registers,
 // and two neighbouring lanes exchange halves to store two entries of a row each.  The rows' constants lie in LDS.
-template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, 2) void grad_logits_kernel(const LogitArgs a) {
+template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::OCC) void grad_logits_kernel(const LogitArgs a) {
     typedef Gemm<C, false, F16> G;
     __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
     __shared__ __attribute__((aligned(16))) float r_lse[C::BI], r_f[C::BI], r_sc[SPLIT ? C::BI : 4], r_inv[SPLIT ? C::BI : 4];
@@ -340,73 +350,104 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, 2) 
     const unsigned sel = lane & 1 ? 0x03020706u : 0x05040100u;  // of (neighbour's pair : own pair)
     auto tile = [&](int t) { return TileAt{i0, a.v0 + (st + t * a.ns) * C::BJ}; };
     auto first = [&](int t) { return (st + t * a.ns) * C::BJ + wj; };  // in the piece
-    auto begin = [&](int t, f32x16 (&acc)[C::WI][C::WJ]) {
+    // (products that start from the bias would save an add an element, but make the compiler spill the sums)
+    auto begin = [&](int, f32x16 (&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int q = 0; q < C::WJ; ++q) {
-            const float b = SPLIT ? 0.f : a.bias[a.v0 + first(t) + q * 32 + li];
+        for (int p = 0; p < C::WI; ++p)
 #pragma unroll
-            for (int p = 0; p < C::WI; ++p)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[p][q][r] = b;
-        }
+            for (int q = 0; q < C::WJ; ++q) clear(acc[p][q]);
     };
-    auto done = [&](int t, f32x16 (&acc)[C::WI][C::WJ]) {
+    auto done = [&](int t, f32x16 (&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
         const int v = first(t);
-        bool any = false;  // is one of the wave's targets in its columns?
+        // blocks that hold a target: bit q * WI + p
+        unsigned hot = 0;
 #pragma unroll
         for (int i = 0; i < C::WI * 32; i += 64) {
-            const int at = r_t[wr + (i + lane < C::WI * 32 ? i + lane : 0)] - v;
-            any = any || (at >= 0 && at < C::WJ * 32);
+            const int at = r_t[wr + i + (i + lane < C::WI * 32 ? lane : 0)] - v;
+#pragma unroll
+            for (int q = 0; q < C::WJ; ++q) {
+                const unsigned long long m = __builtin_amdgcn_ballot_w64(at >= q * 32 && at < q * 32 + 32);
+                hot |= ((unsigned)m ? 1u << (q * C::WI + i / 32) : 0u) | (i + 32 < C::WI * 32 && (m >> 32) ? 2u << (q * C::WI + i / 32) : 0u);
+            }
         }
-        const bool hot = __builtin_amdgcn_ballot_w64(any) != 0;
+        long long ld2 = a.ldg * 2;
+        asm volatile("" : "+s"(ld2));  // (else the distances of all rows are computed once and spilled)
+        // a lane stores row (lane & 1) of a pair of rows, columns col & ~1 and the next
+        char *base = (char *)(a.G + (long long)(i0 + wr) * a.ldg + v);
+        const unsigned lane_at = (unsigned)((4 * lh + (lane & 1)) * (int)a.ldg + (li & ~1)) * 2u;
+        float db[C::WJ], b2[C::WJ];
 #pragma unroll
         for (int q = 0; q < C::WJ; ++q) {
-            const int col = v + q * 32 + li;
-            const float b2 = SPLIT ? a.bias[a.v0 + col] * LOG2E : 0.f;
-            float db = 0.f;
-            short *out = a.G + (long long)(i0 + wr + 4 * lh + (lane & 1)) * a.ldg + (col & ~1);
+            b2[q] = a.bias[a.v0 + v + q * 32 + li] * LOG2E;
+            db[q] = 0.f;
+        }
+        // four rows (8 s .. of block p) by the wave's columns from block q0 on; again: once more, with the targets taken off
+        auto quad = [&](auto again_, int p, int s, int q0, int q1) __attribute__((always_inline)) {
+            constexpr bool AGAIN = decltype(again_)::value;
+            int at = wr + p * 32 + 8 * s + 4 * lh;
+            if (AGAIN) asm volatile("" : "+v"(at));  // (else everything of the first time is kept for the second, and spilled)
+            const f32x4 l = *(const f32x4 *)&r_lse[at], f = *(const f32x4 *)&r_f[at];
+            f32x4 sc, inv;
+            if (SPLIT) sc = *(const f32x4 *)&r_sc[at], inv = *(const f32x4 *)&r_inv[at];
+            char *row = base + (p * 32 + 8 * s) * ld2;
 #pragma unroll
-            for (int p = 0; p < C::WI; ++p) {
-                if (i0 + wr + p * 32 >= a.Mp) break;  // (Mp is a multiple of 64)
+            for (int q = q0; q < q1; ++q) {
+                float w[4];
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const int at = wr + p * 32 + 8 * s + 4 * lh;
-                    const f32x4 l = *(const f32x4 *)&r_lse[at], f = *(const f32x4 *)&r_f[at];
-                    f32x4 sc, inv;
-                    if (SPLIT) sc = *(const f32x4 *)&r_sc[at], inv = *(const f32x4 *)&r_inv[at];
-                    float w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = acc[p][q][s * 4 + e];
-                        const float pr = exp2_(SPLIT ? fmaf(x, sc[e], b2) - l[e] : fmaf(x, LOG2E, -l[e]));
-                        w[e] = hot ? (pr - (r_t[at + e] == col ? 1.f : 0.f)) * f[e] : pr * f[e];
-                        db = SPLIT ? fmaf(w[e], inv[e], db) : db + w[e];
+                for (int e = 0; e < 4; ++e) {
+                    const float x = acc[p][q][s * 4 + e];
+                    w[e] = exp2_(fmaf(x, SPLIT ? sc[e] : LOG2E, b2[q]) - l[e]);
+                    if (AGAIN) {
+                        const float hit = r_t[at + e] == v + q * 32 + li ? 1.f : 0.f;
+                        w[e] -= hit;
+                        db[q] -= SPLIT ? hit * f[e] * inv[e] : hit * f[e];
                     }
+                    w[e] *= f[e];
+                    if (!AGAIN) db[q] = SPLIT ? fmaf(w[e], inv[e], db[q]) : db[q] + w[e];
+                }
 #pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        auto store = [&](unsigned own, short *to) {
-                            const unsigned other = __builtin_amdgcn_update_dpp(0, own, 0xB1, 0xF, 0xF, true);  // lane ^ 1
-                            *(unsigned *)(to + (long long)(p * 32 + 8 * s + e) * a.ldg) = __builtin_amdgcn_perm(other, own, sel);
-                        };
-                        if constexpr (SPLIT) {
-                            short h1[2], h2[2];
-                            split(w[e], h1[0], h2[0]);
-                            split(w[e + 1], h1[1], h2[1]);
-                            store((unsigned short)h1[0] | (unsigned)(unsigned short)h1[1] << 16, out);
-                            store((unsigned short)h2[0] | (unsigned)(unsigned short)h2[1] << 16, out + a.gplane);
-                        } else if constexpr (F16) {
-                            store((unsigned short)bits((_Float16)w[e]) | (unsigned)(unsigned short)bits((_Float16)w[e + 1]) << 16, out);
-                        } else {
-                            store((unsigned short)bits((__bf16)w[e]) | (unsigned)(unsigned short)bits((__bf16)w[e + 1]) << 16, out);
+                for (int e = 0; e < 4; e += 2) {
+                    auto put = [&](unsigned own, char *to) __attribute__((always_inline)) {
+                        const unsigned other = __builtin_amdgcn_update_dpp(0, own, 0xB1, 0xF, 0xF, true);  // lane ^ 1
+                        *(unsigned *)(to + e * ld2 + q * 64 + lane_at) = __builtin_amdgcn_perm(other, own, sel);
+                    };
+                    const f32x2 pair = {w[e], w[e + 1]};
+                    if constexpr (F16) {
+                        const f16x2 h = __builtin_convertvector(pair, f16x2);
+                        put(__builtin_bit_cast(unsigned, h), row);
+                        if constexpr (SPLIT) {  // h2 is held times 2048
+                            const f32x2 r = {fmaf((float)h[0], -2048.f, pair[0] * 2048.f), fmaf((float)h[1], -2048.f, pair[1] * 2048.f)};
+                            put(__builtin_bit_cast(unsigned, __builtin_convertvector(r, f16x2)), row + a.gplane * 2);
                         }
+                    } else {
+                        put(__builtin_bit_cast(unsigned, __builtin_convertvector(pair, bf16x2)), row);
                     }
                 }
             }
-            if (a.dbias) {
-                db += __shfl_xor(db, 32);
-                if (lh == 0) a.dbias[(long long)(bi * C::VI + wi) * a.ldg + col] = db;
-            }
+            __builtin_amdgcn_sched_barrier(0);  // (quad by quad: together the temporaries spill)
+        };
+#pragma unroll
+        for (int p = 0; p < C::WI; ++p) {
+            if (i0 + wr + p * 32 >= a.Mp) break;  // (Mp is a multiple of 64)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) quad(std::false_type(), p, s, 0, C::WJ);
         }
+        // The few blocks with a target are stored twice, by the same lanes: a test in the loop above would cost every block more
+        if (hot) {
+#pragma unroll
+            for (int p = 0; p < C::WI; ++p)
+#pragma unroll
+                for (int q = 0; q < C::WJ; ++q)
+                    if (hot >> (q * C::WI + p) & 1)
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) quad(std::true_type(), p, s, q, q + 1);
+        }
+        if (a.dbias)
+#pragma unroll
+            for (int q = 0; q < C::WJ; ++q) {
+                db[q] += __shfl_xor(db[q], 32);
+                if (lh == 0) a.dbias[(long long)(bi * C::VI + wi) * a.ldg + v + q * 32 + li] = db[q];
+            }
     };
     G::run(a.x, a.W, (a.nv - st + a.ns - 1) / a.ns, tile, 0, a.nk, a.passes, lds, begin, done);
 }
@@ -439,11 +480,7 @@ struct OutArgs {  // C[i][j] * post, in the elements' type
     long long ld;
     int elem;
 };
-__device__ __forceinline__ void clear(f32x16 &v) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) v[r] = 0.f;
-}
-template <class C, bool KMAJOR, bool F16> __global__ __launch_bounds__(C::NT, 2) void sum_kernel(const SumArgs a) {
+template <class C, bool KMAJOR, bool F16> __global__ __launch_bounds__(C::NT, C::OCC) void sum_kernel(const SumArgs a) {
     typedef Gemm<C, KMAJOR, F16> G;
     __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
     int bi, bj;
@@ -451,13 +488,13 @@ template <class C, bool KMAJOR, bool F16> __global__ __launch_bounds__(C::NT, 2)
     const int k0 = blockIdx.y * a.per, k1 = k0 + a.per < a.nk ? k0 + a.per : a.nk;
     const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5, wave = threadIdx.x >> 6;
     const int wi0 = bi * C::BI + (wave / C::VJ) * (C::WI * 32), wj0 = bj * C::BJ + (wave % C::VJ) * (C::WJ * 32);
-    auto begin = [&](int, f32x16 (&acc)[C::WI][C::WJ]) {
+    auto begin = [&](int, f32x16 (&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
 #pragma unroll
         for (int p = 0; p < C::WI; ++p)
 #pragma unroll
             for (int q = 0; q < C::WJ; ++q) clear(acc[p][q]);
     };
-    auto done = [&](int, f32x16 (&acc)[C::WI][C::WJ]) {
+    auto done = [&](int, f32x16 (&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
         float *o = a.out + ((long long)blockIdx.y * a.I + wi0 + 4 * lh) * a.J + wj0 + li;
 #pragma unroll
         for (int p = 0; p < C::WI; ++p)
@@ -472,7 +509,7 @@ template <class C, bool KMAJOR, bool F16> __global__ __launch_bounds__(C::NT, 2)
     };
     G::run(a.A, a.B, 1, [&](int) { return TileAt{bi * C::BI, bj * C::BJ}; }, k0, k1, a.passes, lds, begin, done);
 }
-template <class C, bool F16> __global__ __launch_bounds__(C::NT, 2) void out_kernel(const OutArgs a) {
+template <class C, bool F16> __global__ __launch_bounds__(C::NT, C::OCC) void out_kernel(const OutArgs a) {
     typedef Gemm<C, true, F16> G;
     __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
     int bi, bj;
@@ -480,13 +517,13 @@ template <class C, bool F16> __global__ __launch_bounds__(C::NT, 2) void out_ker
     const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5, wave = threadIdx.x >> 6;
     const int wi0 = bi * C::BI + (wave / C::VJ) * (C::WI * 32), wj0 = bj * C::BJ + (wave % C::VJ) * (C::WJ * 32);
     const float post = a.post[0];
-    auto begin = [&](int, f32x16 (&acc)[C::WI][C::WJ]) {
+    auto begin = [&](int, f32x16 (&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
 #pragma unroll
         for (int p = 0; p < C::WI; ++p)
 #pragma unroll
             for (int q = 0; q < C::WJ; ++q) clear(acc[p][q]);
     };
-    auto done = [&](int, f32x16 (&acc)[C::WI][C::WJ]) {
+    auto done = [&](int, f32x16 (&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
         const long long at = (long long)(wi0 + 4 * lh) * a.ld + wj0 + li;
 #pragma unroll
         for (int p = 0; p < C::WI; ++p)
@@ -541,10 +578,10 @@ constexpr long long PIECE_BYTES = 3ll << 29;  // G of one piece of the vocabular
 }  // namespace
 
 struct tsc_unembed {
-    int D, V, elem, belem, planes, Dp, Vp, Vb;  // paddings: 64 for a product's k, 256 for the bias a tile reads
+    int D, V, elem, belem, planes, wplanes, Dp, Vp, Vb;  // paddings: 64 for a product's k, 256 for the bias a tile reads
     long long sd, sv;                    // strides of W (elements): one of them is 1
     const void *W, *bias;                // borrowed
-    short *Wt, *Wd;                      // [V][planes * Dp] and [D][planes * Vp]
+    short *Wt, *Wd;                      // [V][planes of Dp] and [D][wplanes of Vp]
     float *bias32, *wscale;
 };
 
@@ -569,8 +606,8 @@ int tsc_unembed_refresh_(tsc_unembed *h, hipStream_t s) {
         hipLaunchKernelGGL(absmax_kernel, dim3((int)(rows < 1024 ? rows : 1024)), dim3(1024), 0, s, (const float *)h->W, rows, cols, ld, (unsigned *)h->wscale);
         hipLaunchKernelGGL(wscale_kernel, dim3(1), dim3(1), 0, s, h->wscale);
     }
-    hipLaunchKernelGGL(pack_w_kernel, dim3(h->Dp / 64, cdiv(h->V, 64)), dim3(256), 0, s, h->W, h->elem, h->sv, h->sd, h->V, h->D, h->Dp, h->wscale, h->Wt);
-    hipLaunchKernelGGL(pack_w_kernel, dim3(h->Vp / 64, cdiv(h->D, 64)), dim3(256), 0, s, h->W, h->elem, h->sd, h->sv, h->D, h->V, h->Vp, h->wscale, h->Wd);
+    hipLaunchKernelGGL(pack_w_kernel, dim3(h->Dp / 64, cdiv(h->V, 64)), dim3(256), 0, s, h->W, h->elem, h->sv, h->sd, h->V, h->D, h->Dp, h->planes, h->wscale, h->Wt);
+    hipLaunchKernelGGL(pack_w_kernel, dim3(h->Vp / 64, cdiv(h->D, 64)), dim3(256), 0, s, h->W, h->elem, h->sd, h->sv, h->D, h->V, h->Vp, h->wplanes, h->wscale, h->Wd);
     TSC_HIP_CHECK(hipGetLastError());
     return TSC_OK;
 }
@@ -578,11 +615,11 @@ int tsc_unembed_refresh_(tsc_unembed *h, hipStream_t s) {
 int tsc_unembed_create_(tsc_unembed **out, int D, int V, int elem, const void *W, long long sd, long long sv, const void *bias, int belem, hipStream_t s) {
     tsc_unembed *h = new (std::nothrow) tsc_unembed();
     if (!h) return tsc_fail(TSC_ERR_HIP, "out of host memory");
-    h->D = D; h->V = V; h->elem = elem; h->belem = belem; h->planes = elem == TSC_ELEM_F32 ? 2 : 1;
+    h->D = D; h->V = V; h->elem = elem; h->belem = belem; h->planes = elem == TSC_ELEM_F32 ? 2 : 1; h->wplanes = elem == TSC_ELEM_F32 ? 3 : 1;
     h->Dp = (int)up(D, BK); h->Vp = (int)up(V, 256); h->Vb = h->Vp + 256;
     h->sd = sd; h->sv = sv; h->W = W; h->bias = bias;
     hipError_t e = hipMalloc((void **)&h->Wt, (size_t)V * h->planes * h->Dp * 2);
-    if (e == hipSuccess) e = hipMalloc((void **)&h->Wd, (size_t)D * h->planes * h->Vp * 2);
+    if (e == hipSuccess) e = hipMalloc((void **)&h->Wd, (size_t)D * h->wplanes * h->Vp * 2);
     if (e == hipSuccess) e = hipMalloc((void **)&h->bias32, (size_t)h->Vb * 4);
     if (e == hipSuccess) e = hipMalloc((void **)&h->wscale, 256);
     int rc = e == hipSuccess ? tsc_unembed_refresh_(h, s) : tsc_fail(TSC_ERR_HIP, "hipMalloc of the unembedding's operands failed: %s", hipGetErrorString(e));
@@ -690,7 +727,7 @@ Plan plan(const tsc_unembed *h, long long M, bool backward, bool want_x, bool wa
     p.st = streams(M, nv);
     long long at = 0;
     auto take = [&](long long n) { const long long q = at; at = up(at + n, 256); return q; };
-    p.xp = take(2ll * h->planes * p.Mp * h->Dp);
+    p.xp = take(2ll * (backward ? h->wplanes : h->planes) * p.Mp * h->Dp);
     p.xscale = take(4 * M);
     if (!backward) {
         p.part = take(8ll * p.st.ns * M);
@@ -736,10 +773,11 @@ template <bool GRAD> int logits(const tsc_unembed *h, const Streams &st, const L
            : h->elem == TSC_ELEM_BF16 ? launch_logits<false, false, GRAD>(st, a, s)
                                       : launch_logits<true, false, GRAD>(st, a, s);
 }
-LogitArgs logit_args(const tsc_unembed *h, const Plan &p, char *ws, int M, const long long *targets, long long ignore) {
+LogitArgs logit_args(const tsc_unembed *h, const Plan &p, char *ws, int xplanes, int M, const long long *targets, long long ignore) {
     LogitArgs a{};
-    a.W = {h->Wt, (long long)h->planes * h->Dp, h->Dp, h->V};
-    a.x = {(const short *)(ws + p.xp), (long long)h->planes * h->Dp, h->Dp, M};
+    // x W: h2 h1', h1 h2', h1 h1'
+    a.W = {h->Wt, (long long)h->planes * h->Dp, 0, h->Dp, h->V};
+    a.x = {(const short *)(ws + p.xp), (long long)xplanes * h->Dp, h->Dp, 0, M};
     a.nk = h->Dp / BK; a.passes = h->planes == 2 ? 3 : 1;
     a.nm = p.st.nm; a.ns = p.st.ns; a.nv = p.st.nv; a.M = M; a.V = h->V;
     a.bias = h->bias32;
@@ -784,9 +822,9 @@ size_t tsc_unembed_workspace_(const tsc_unembed *h, long long M, int backward, i
 int tsc_launch_unembed_loss(const tsc_unembed *h, const TscRows &x, int M, const long long *targets, long long ignore, float *loss,
                             float *lse, char *ws, hipStream_t s) {
     const Plan p = plan(h, M, false, false, false, false);
-    hipLaunchKernelGGL(pack_x_kernel, dim3(cdiv(p.Mp, 4)), dim3(256), 0, s, x, h->elem, M, p.Mp, h->D, h->Dp, (const long long *)nullptr, ignore,
+    hipLaunchKernelGGL(pack_x_kernel, dim3(cdiv(p.Mp, 4)), dim3(256), 0, s, x, h->elem, M, p.Mp, h->D, h->Dp, h->planes, (const long long *)nullptr, ignore,
                        (short *)(ws + p.xp), (float *)(ws + p.xscale));
-    LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
+    LogitArgs a = logit_args(h, p, ws, h->planes, M, targets, ignore);
     a.part = (float2 *)(ws + p.part);
     a.hit = (float *)(ws + p.hit);
     const int rc = logits<false>(h, p.st, a, s);
@@ -809,12 +847,12 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
     const Plan p = plan(h, M, true, dx != nullptr, dW != nullptr, db != nullptr);
     short *xp = (short *)(ws + p.xp), *G = (short *)(ws + p.g);
     float *xscale = (float *)(ws + p.xscale), *rowf = (float *)(ws + p.rowf), *post = (float *)(ws + p.post), *dxp = (float *)(ws + p.dxp);
-    hipLaunchKernelGGL(pack_x_kernel, dim3(cdiv(p.Mp, 4)), dim3(256), 0, s, x, h->elem, M, p.Mp, h->D, h->Dp, targets, ignore, xp, xscale);
+    hipLaunchKernelGGL(pack_x_kernel, dim3(cdiv(p.Mp, 4)), dim3(256), 0, s, x, h->elem, M, p.Mp, h->D, h->Dp, h->wplanes, targets, ignore, xp, xscale);
     hipLaunchKernelGGL(row_factor_kernel, dim3(1), dim3(1024), 0, s, g, xscale, targets, ignore, h->V, M, f16, rowf, post);
-    LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
+    LogitArgs a = logit_args(h, p, ws, h->wplanes, M, targets, ignore);
     a.lse = lse; a.rowf = rowf; a.G = G; a.ldg = p.Vc; a.gplane = (long long)p.Mp * p.Vc; a.Mp = p.Mp;
     a.dbias = db ? (float *)(ws + p.db) : nullptr;
-    const long long xld = (long long)h->planes * h->Dp;
+    const long long xld = (long long)h->wplanes * h->Dp;
     const int db_parts = p.st.nm * (p.st.s.kind == FEW ? 1 : 2);  // waves of a tile's rows
     for (int c = 0; c < p.pieces; ++c) {
         const int v0 = c * p.Vc, nv = h->V - v0 < p.Vc ? h->V - v0 : p.Vc;
@@ -826,8 +864,9 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
         if (db) hipLaunchKernelGGL(dbias_kernel, dim3(cdiv(nv, 256)), dim3(256), 0, s, a.dbias, db_parts, a.ldg, nv, post, h->belem, db, (long long)v0);
         if (dx) {
             SumArgs q{};
-            q.A = {G, p.Vc, a.gplane, M};
-            q.B = {h->Wd + v0, (long long)h->planes * h->Vp, h->Vp, h->D};
+            // G W^T: h2 (2048 of it) by h1' / 2048, h1 by h2', h1 by h1'
+            q.A = {G, p.Vc, a.gplane, 0, M};
+            q.B = {h->Wd + v0, (long long)h->wplanes * h->Vp, 2ll * h->Vp, h->Vp, h->D};
             q.nk = cdiv(nv, BK); q.passes = passes; q.I = M; q.J = h->D; q.add = c > 0; q.out = dxp;
             Split w = p.dx;
             if (c > 0) w.per = cdiv(q.nk, w.z);  // the same parts, shorter
@@ -835,7 +874,7 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
             if (rc) return rc;
         }
         if (dW) {
-            const Operand X = {xp, xld, h->Dp, h->D}, Gk = {G, p.Vc, a.gplane, nv};
+            const Operand X = {xp, xld, 2 * h->Dp, h->Dp, h->D}, Gk = {G, p.Vc, a.gplane, 0, nv};
             const bool by_d = h->sv == 1;  // dW is dense in W's order: [D][V] or [V][D]
             const Split w = dw_split(h, p.Mp, nv);
             const int I = by_d ? h->D : nv, J = by_d ? nv : h->D;

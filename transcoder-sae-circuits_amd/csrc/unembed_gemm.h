@@ -2,21 +2,30 @@
 //
 //   C[i][j] = sum_k A(i, k) * B(j, k)
 //
-// One workgroup computes a BI x BJ tile in k-steps of 64.  Both operand tiles of a k-step go global -> LDS by
-// global_load_lds_dwordx4 (1 KiB a wave and instruction, no registers) into one of two buffers while the other one is
-// multiplied; one barrier a k-step.  Operands come in two layouts:
-//   row-major  A(i, k) = A[i * ld + k]: LDS rows of 128 bytes (64 k), a fragment is one ds_read_b128
-//   k-major    A(i, k) = A[k * ld + i]: LDS rows of BI elements, a fragment is two transposing ds_read_b64_tr_b16
+// One workgroup computes a BI x BJ tile in steps of SK k.  Both operand tiles of a step go global -> LDS by
+// global_load_lds_dwordx4 (1 KiB a wave and instruction, no registers) into one of NS buffers while another one is
+// multiplied; one barrier a step.  Operands come in two layouts:
+//   row-major  A(i, k) = A[i * ld + k]: LDS rows of 64 k = 128 bytes, two buffers, a fragment is one ds_read_b128
+//   k-major    A(i, k) = A[k * ld + i]: LDS rows of BI elements, four buffers of 32 k, a fragment is two transposing
+//              ds_read_b64_tr_b16
+// (Four buffers of 32 k give a copy three steps of time instead of three quarters of a longer one: k-major 1209 against 1178
+// TFLOP/s on random operands at 768 x 21760 x 16384 and 1854 against 1567 on zeros, which the power limit leaves alone.
+// Row-major rows of 32 k are 64 bytes, half a cache line: 1142 against 1195.)
 // 16-byte chunks are permuted through the source address of the copy (row-major: chunk ^ (row / 2) % 8; k-major: the
-// 64-byte groups ^ k % 4), which spreads the lanes of a fragment read over the banks.
+// 64-byte groups ^ k % 4), which spreads the lanes of a fragment read over the banks: no conflict is counted.
+// What bounds the loop is power: at 70 % of its issue slots the matrix pipe runs at 1.5-1.6 GHz on real operands, and the
+// vendor's own kernel, at 94 %, at 1.44 (1340-1375 TFLOP/s at 8192^3; this loop 1292).
 //
-// fp32 operands are split into two fp16 planes: x / s = h1 + h2 / 2048, s a power of two that brings the largest magnitude
-// into [2^13, 2^14).  h1 holds 11 bits, h2 the next 11 (and more where h1 is subnormal), so h1 + h2 / 2048 has 22 bits for
-// values down to 2^-27 of the largest and a fixed 2^-49 of it below.  The product is three passes over k,
-// (h2 h1' + h1 h2') / 2048 + h1 h1', the cross terms first; the dropped h2 h2' is 2^-24 of the product at most.  Every
-// product of two fp16 values is exact in the matrix pipe, sums are fp32: the result carries the error of an fp32 product
-// at a third of the 16-bit rate, which is 5 times the fp32 matrix rate.
+// fp32 operands are split into fp16 planes: v / s = h1 + h2, s a power of two that brings the largest magnitude into
+// [2^14, 2^15).  h1 holds 11 bits and h2 the next 11: 22 bits for values down to 2^-17 of the largest, a fixed 2^-39 of it
+// below (fp16 ends at 2^-24).  The product is three passes over k, h2 h1' + h1 h2' + h1 h1', the small terms first; the
+// dropped h2 h2' is 2^-22 of the product at most.  Every product of two fp16 values is exact in the matrix pipe, sums are
+// fp32: the result carries the error of an fp32 product at a third of the 16-bit rate, 5 times the fp32 matrix rate.
+// G, whose entries are probabilities and span many more powers of two, is split as h1 + h2 / 2048: 22 bits down to 2^-28 of
+// the largest and a fixed 2^-50 of it below; the pass with its h2 reads a plane h1' / 2048 of the other operand.
 #pragma once
+#include <type_traits>
+
 #include "tsc_internal.h"
 
 namespace unembed_gemm {
@@ -25,47 +34,66 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef const __attribute__((address_space(1))) void *gptr_t;
 typedef __attribute__((address_space(3))) void *lptr_t;
 
-constexpr int BK = 64;
+constexpr int BK = 64;  // k are counted and padded in multiples of this
 
 template <int WI_, int WJ_, int VI_, int VJ_> struct Tile {  // 32 x 32 blocks of a wave, waves of a workgroup
     static constexpr int WI = WI_, WJ = WJ_, VI = VI_, VJ = VJ_, NW = VI * VJ, NT = 64 * NW;
     static constexpr int BI = VI * WI * 32, BJ = VJ * WJ * 32;
-    static constexpr int PA = BI / 8 / NW, PB = BJ / 8 / NW;  // 1-KiB pieces of a k-step and wave
-    static_assert(PA * NW * 8 == BI && PB * NW * 8 == BJ, "whole pieces a wave");
+    static constexpr int OCC = 2;  // waves a SIMD at least
 };
-typedef Tile<4, 2, 2, 4> TileLarge;   // 256 x 256, 8 waves
-typedef Tile<2, 2, 2, 2> TileMedium;  // 128 x 128, 4 waves
-typedef Tile<1, 2, 4, 1> TileTall;    // 128 x 64, 4 waves: few tokens, the vocabulary streams
+// (LARGE as four waves of 128 x 128, one a SIMD with its 256 sums in accumulator registers, has 2/3 of the LDS reads and a
+// loop without a spill; alone it measured 1195 TFLOP/s against 1292 of eight waves of 128 x 64 at 8192^3, and its epilogue
+// overlaps with nothing: loss of 65536 rows 6.55 ms against 4.47)
+typedef Tile<4, 2, 2, 4> TileLarge;   // 256 x 256, one workgroup a CU
+typedef Tile<2, 2, 2, 2> TileMedium;  // 128 x 128, two
+typedef Tile<1, 2, 4, 1> TileTall;    // 128 x 64: few tokens, the vocabulary streams
 typedef Tile<2, 1, 1, 4> TileWide;    // 64 x 128: the same with the operands exchanged
 
 struct Operand {
     const short *p;
-    long long ld;     // elements between rows (row-major) or between k (k-major)
-    long long plane;  // elements from plane h1 to plane h2
+    long long ld;             // elements between rows (row-major) or between k (k-major)
+    long long first, second;  // elements from plane h1 to the plane that the first (the second) of three passes reads
     int rows;         // valid i (j); the tile's others read copies of valid ones
 };
+
+// 16 bytes a lane, global -> LDS: base + off (of the lane) to LDS address at + 16 * lane.  Written out, and not through the
+// builtin, because the compiler would wait for every copy in flight before the next LDS read, whichever buffer that reads;
+// Gemm::run waits by itself, once a step.  (m0 is the compiler's only next to an instruction that takes it; none here does.)
+__device__ __forceinline__ void copy16(const char *base, unsigned off, unsigned at) {
+    const unsigned long long b = (unsigned long long)base;  // (uniform; said again for where the compiler lost sight of it)
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)b), hi = __builtin_amdgcn_readfirstlane((unsigned)(b >> 32));
+    const unsigned long long u = (unsigned long long)hi << 32 | lo;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(u));
+}
 
 // One tile of a workgroup's stream: first rows of both operands.
 struct TileAt {
     int i0, j0;
 };
 
-// The product of a stream of tiles.  All k-steps of all tiles of a workgroup form one stream: step s + 1 is in LDS and step
-// s + 2 on its way while step s is multiplied, also across the end of a tile, so that only the first tile waits for memory.
+// The product of a stream of tiles.  All steps of all tiles of a workgroup form one stream: step s + 1 is in LDS and steps up
+// to s + NS on their way while step s is multiplied, also across the end of a tile, so that only the first tile waits for
+// memory.
 //
-//   step s:  MFMA k 0-15 | 16-31 | 32-47, each while the fragments of the next group are read
-//            wait: own fragments of 48-63 are in registers, own copies of step s + 1 have landed; barrier
-//            MFMA k 48-63 while the first fragments of step s + 1 are read and the copies of step s + 2 are issued
+//   step s:  products of all but the last 16 k, each group while the fragments of the next are read
+//            wait: own fragments of the last group are in registers, own copies of step s + 1 have landed; barrier
+//            products of the last group while the first fragments of step s + 1 are read and the copies of step s + NS issued
 //
 // Behind the barrier nobody reads the buffer of step s any more and everybody's part of step s + 1 is there.
 template <class C, bool KMAJOR, bool F16> struct Gemm {
-    static constexpr int ABYTES = C::BI * BK * 2, BBYTES = C::BJ * BK * 2, STAGE = ABYTES + BBYTES;
-    static constexpr int LDS_BYTES = 2 * STAGE;
+    static constexpr int SK = KMAJOR ? 32 : 64, NS = KMAJOR ? 4 : 2, KK = SK / 16;
+    static constexpr int ABYTES = C::BI * SK * 2, BBYTES = C::BJ * SK * 2, STAGE = ABYTES + BBYTES;
+    static constexpr int LDS_BYTES = NS * STAGE;
+    static constexpr int PA = ABYTES / 1024 / C::NW, PB = BBYTES / 1024 / C::NW, P = PA + PB;  // 1-KiB pieces of a step and wave
+    static_assert(P * C::NW * 1024 == STAGE, "whole pieces a wave");
 
     // byte offsets of this lane's part of the PIECES 1-KiB pieces of this wave, relative to the tile's base
     template <int ROWS, int PIECES>
@@ -90,14 +118,14 @@ template <class C, bool KMAJOR, bool F16> struct Gemm {
     static __device__ __forceinline__ const char *base(const Operand &o, int row0, int k0) {
         return (const char *)(o.p + (KMAJOR ? (long long)k0 * BK * o.ld + row0 : (long long)row0 * o.ld + (long long)k0 * BK));
     }
-    static __device__ __forceinline__ long long step_bytes(const Operand &o) { return KMAJOR ? 2ll * BK * o.ld : 2ll * BK; }
+    static __device__ __forceinline__ long long step_bytes(const Operand &o) { return KMAJOR ? 2ll * SK * o.ld : 2ll * SK; }
 
     template <int ROWS> struct Frag {  // fragment reads of one operand: one LDS address for each of a step's four groups of 16 k
-        unsigned at[4];
+        unsigned at[KK];
         __device__ __forceinline__ Frag(int row0, int extra) {
             const int lane = threadIdx.x & 63;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
+            for (int kk = 0; kk < KK; ++kk) {
                 if constexpr (KMAJOR) {
                     const int l = lane & 15, g = lane >> 4;
                     const int i = row0 + (g & 1) * 16 + (l & 3) * 4, k = kk * 16 + (g >> 1) * 8 + (l >> 2);
@@ -108,22 +136,17 @@ template <class C, bool KMAJOR, bool F16> struct Gemm {
                 }
             }
         }
-        // rows row0 + 32 * block of k group kk: lane l holds row l % 32, k = 8 * (l / 32) + 0..7
-        template <int N> __device__ __forceinline__ void read(const char *lds, unsigned buf, int kk, s16x8 (&f)[N]) const {
+        // rows row0 + 32 * b of k group kk: lane l holds row l % 32, k = 8 * (l / 32) + 0..7
+        __device__ __forceinline__ s16x8 read(const char *lds, unsigned buf, int kk, int b) const {
             if constexpr (KMAJOR) {
                 // the chunk permutation acts on the 64-byte groups, so a block's distance of 64 bytes is an exclusive or too
-#pragma unroll
-                for (int b = 0; b < N; ++b) {
-                    typedef __attribute__((address_space(3))) s16x4 *p4;
-                    const char *p = lds + (at[kk] ^ (b * 64)) + buf;
-                    const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lptr_t)p);
-                    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lptr_t)(p + 4 * ROWS * 2));
-                    f[b] = __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
-                }
+                typedef __attribute__((address_space(3))) s16x4 *p4;
+                const char *p = lds + (at[kk] ^ (b * 64)) + buf;
+                const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lptr_t)p);
+                const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lptr_t)(p + 4 * ROWS * 2));
+                return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
             } else {
-                const char *p = lds + at[kk] + buf;
-#pragma unroll
-                for (int b = 0; b < N; ++b) f[b] = *(const s16x8 *)(p + b * 4096);
+                return *(const s16x8 *)(lds + at[kk] + buf + b * 4096);
             }
         }
     };
@@ -140,7 +163,7 @@ template <class C, bool KMAJOR, bool F16> struct Gemm {
     static __device__ __forceinline__ void run(const Operand &A, const Operand &B, int n_tiles, At tile, int k0, int k1, int passes,
                                                char *lds, Begin begin, Done done) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const int n = k1 - k0, total = n * passes;
+        const int n = (k1 - k0) * (BK / SK), total = n * passes;
         f32x16 acc[C::WI][C::WJ];
         if (n_tiles <= 0) return;
         if (n <= 0) {  // (a part of the k-steps behind their end)
@@ -152,31 +175,31 @@ template <class C, bool KMAJOR, bool F16> struct Gemm {
         }
         const Frag<C::BI> ra((wave / C::VJ) * (C::WI * 32), 0);
         const Frag<C::BJ> rb((wave % C::VJ) * (C::WJ * 32), ABYTES);
-        unsigned offa[C::PA], offb[C::PB];
+        unsigned offa[PA], offb[PB];
         // the producer: the next step to copy
-        int pt = 0, pp = passes == 1 ? 2 : 0, ps = 0;  // tile, pass (0: h2 h1', 1: h1 h2', 2: h1 h1'), step of the pass
+        int pt = 0, pp = passes == 1 ? 2 : 0, ps = 0;  // tile, pass (of one-plane operands: the last), step of the pass
         unsigned pbuf = 0;
         const char *a0, *b0, *pa, *pb;
         const long long da = step_bytes(A), db = step_bytes(B);
         auto set_pass = [&]() {
-            pa = a0 + (pp == 0 ? A.plane * 2 : 0);
-            pb = b0 + (pp == 1 ? B.plane * 2 : 0);
+            pa = a0 + (pp == 0 ? A.first : pp == 1 ? A.second : 0) * 2;
+            pb = b0 + (pp == 0 ? B.first : pp == 1 ? B.second : 0) * 2;
         };
         auto set_tile = [&]() {
             const TileAt at = tile(pt);
-            offsets<C::BI, C::PA>(A, at.i0, offa);
-            offsets<C::BJ, C::PB>(B, at.j0, offb);
+            offsets<C::BI, PA>(A, at.i0, offa);
+            offsets<C::BJ, PB>(B, at.j0, offb);
             a0 = base(A, at.i0, k0);
             b0 = base(B, at.j0, k0);
             set_pass();
         };
+        const unsigned l0 = (unsigned)(size_t)(lptr_t)lds, la = l0 + wave * PA * 1024, lb = l0 + ABYTES + wave * PB * 1024;
         auto piece = [&](int q) {
-            char *dst = lds + pbuf + (q < C::PA ? (wave * C::PA + q) * 1024 : ABYTES + (wave * C::PB + q - C::PA) * 1024);
-            const char *src = q < C::PA ? pa + offa[q < C::PA ? q : 0] : pb + offb[q < C::PA ? 0 : q - C::PA];
-            __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)dst, 16, 0, 0);
+            if (q < PA) copy16(pa, offa[q < PA ? q : 0], la + pbuf + q * 1024);
+            else copy16(pb, offb[q < PA ? 0 : q - PA], lb + pbuf + (q - PA) * 1024);
         };
         auto advance = [&]() {
-            pbuf ^= STAGE;
+            pbuf = pbuf + STAGE == LDS_BYTES ? 0 : pbuf + STAGE;
             if (++ps < n) {
                 pa += da;
                 pb += db;
@@ -193,57 +216,55 @@ template <class C, bool KMAJOR, bool F16> struct Gemm {
                 set_tile();
             }  // else: the stream is at its end, its last step is copied again (twice, unread: no branch in the loop)
         };
-        constexpr int P = C::PA + C::PB;
         set_tile();
+        for (int i = 0; i < NS; ++i) {
 #pragma unroll
-        for (int q = 0; q < P; ++q) piece(q);
-        advance();
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-        for (int q = 0; q < P; ++q) piece(q);
-        advance();
+            for (int q = 0; q < P; ++q) piece(q);
+            advance();
+        }
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1) * P) : "memory");
         s16x8 fa[2][C::WI], fb[2][C::WJ];
         unsigned buf = 0;
-        ra.read(lds, 0, 0, fa[0]);
-        rb.read(lds, 0, 0, fb[0]);
+        // a group of 16 k: products of the fragments `now`, and between them the reads of group kk of the buffer at `from` into
+        // the other set and (COPY) the step's copies -- one behind each product, in this order: a burst of either would leave
+        // the matrix pipe idle, and so would the compiler's own order
+        auto group = [&](auto now_, auto copy_, int kk, unsigned from) {
+            constexpr int NOW = decltype(now_)::value, G = C::WI * C::WJ, R = C::WI + C::WJ;
+            constexpr bool COPY = decltype(copy_)::value;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int a = g / C::WJ, b = a & 1 ? C::WJ - 1 - g % C::WJ : g % C::WJ;  // (back and forth: one operand stays)
+                acc[a][b] = mfma(fa[NOW][a], fb[NOW][b], acc[a][b]);
+                __builtin_amdgcn_sched_barrier(0);
+                // the reads end with the first half of the products (one more for the copies' group: their own come first)
+#pragma unroll
+                for (int r = g * 2 * R / G; r < (g + 1) * 2 * R / G && r < R; ++r) {
+                    if (r < C::WJ) fb[NOW ^ 1][r < C::WJ ? r : 0] = rb.read(lds, from, kk, r);
+                    else fa[NOW ^ 1][r < C::WJ ? 0 : r - C::WJ] = ra.read(lds, from, kk, r - C::WJ);
+                }
+                if (COPY)
+#pragma unroll
+                    for (int q = g * P / G; q < (g + 1) * P / G; ++q) piece(q);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+#pragma unroll
+        for (int r = 0; r < C::WJ; ++r) fb[0][r] = rb.read(lds, 0, 0, r);
+#pragma unroll
+        for (int r = 0; r < C::WI; ++r) fa[0][r] = ra.read(lds, 0, 0, r);
+        const std::integral_constant<int, 0> even;
+        const std::integral_constant<int, 1> odd;
         for (int t = 0; t < n_tiles; ++t) {
             begin(t, acc);
             for (int s = 0; s < total; ++s) {
-                if (passes == 3 && s == 2 * n)
-#pragma unroll
-                    for (int a = 0; a < C::WI; ++a)
-#pragma unroll
-                        for (int b = 0; b < C::WJ; ++b)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) acc[a][b][r] *= 1.f / 2048.f;
-#pragma unroll
-                for (int kk = 0; kk < 3; ++kk) {
-                    ra.read(lds, buf, kk + 1, fa[(kk + 1) & 1]);
-                    rb.read(lds, buf, kk + 1, fb[(kk + 1) & 1]);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int a = 0; a < C::WI; ++a)
-#pragma unroll
-                        for (int b = 0; b < C::WJ; ++b) acc[a][b] = mfma(fa[kk & 1][a], fb[kk & 1][b], acc[a][b]);
-                    __builtin_amdgcn_sched_barrier(0);
+                if constexpr (KK == 4) {
+                    group(even, std::false_type(), 1, buf);
+                    group(odd, std::false_type(), 2, buf);
                 }
-                buf ^= STAGE;
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                // (behind the last step of the last tile these fragments are not used)
-                ra.read(lds, buf, 0, fa[0]);
-                rb.read(lds, buf, 0, fb[0]);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int a = 0; a < C::WI; ++a)
-#pragma unroll
-                    for (int b = 0; b < C::WJ; ++b) {
-                        acc[a][b] = mfma(fa[1][a], fb[1][b], acc[a][b]);
-                        __builtin_amdgcn_sched_barrier(0);
-                        constexpr int G = C::WI * C::WJ;
-#pragma unroll
-                        for (int q = (a * C::WJ + b) * P / G; q < (a * C::WJ + b + 1) * P / G; ++q) piece(q);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
+                group(even, std::false_type(), KK - 1, buf);
+                buf = buf + STAGE == LDS_BYTES ? 0 : buf + STAGE;
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * P) : "memory");
+                group(odd, std::true_type(), 0, buf);  // (behind the last step of the last tile these fragments are not used)
                 advance();
             }
             done(t, acc);
