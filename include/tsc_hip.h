@@ -438,8 +438,8 @@ int tsc_layer_norm_backward(int elem, const tsc_rows_t *dy, const tsc_rows_t *x,
  * the unembedding is passed as its transpose: stride_d 1, stride_v d_model), the other one at least as long as the axis it
  * steps over.  bias [d_vocab] in bias_elem or NULL; an entry below -1e38 takes that token out
  * (probability 0; a row for which none is left has the loss NaN).  Both are borrowed.
- * The handle owns what the matrix pipe reads: W in both orders, padded, in 16 bits -- for TSC_ELEM_F32 as fp16 planes
- * that hold 22 bits of every weight down to 2^-17 of the largest and a fixed 2^-39 of it below -- 2 x 77 MB (fp32: 154 + 232)
+ * The handle owns what the matrix pipe reads: W in both orders, padded, in 16 bits -- for TSC_ELEM_F32 as two fp16 planes
+ * that hold 22 bits of every weight down to 2^-17 of the largest and a fixed 2^-39 of it below -- 2 x 77 MB (fp32: 2 x 154)
  * at 768 x 50257.  After an in-place change of W or bias call tsc_unembed_refresh, in order with the calls that use the
  * handle.  d_model <= 32768, d_vocab <= 2^20.  One handle may be used from several streams.
  */

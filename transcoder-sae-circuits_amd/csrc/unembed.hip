@@ -45,16 +45,13 @@ __device__ __forceinline__ void split(float v, short &h1, short &h2) {
     h1 = bits(a);
     h2 = fabsf((float)a) < __builtin_inff() ? bits((_Float16)(v - (float)a)) : (short)0;
 }
-// the planes of a value: one in 16 bits, or h1, h2 and (three planes) h1 / 2048, Cp elements apart
-__device__ __forceinline__ void store_planes(short *o, int Cp, float v, int elem, int planes) {
+// element e of a row of 16-bit values, or of two planes
+__device__ __forceinline__ void store_value(short *row, long long e, float v, int elem) {
     if (elem == TSC_ELEM_F32) {
-        short h1, h2;
-        split(v, h1, h2);
-        o[0] = h1;
-        o[Cp] = h2;
-        if (planes == 3) o[2 * Cp] = bits((_Float16)((float)__builtin_bit_cast(_Float16, h1) * (1.f / 2048.f)));
+        short *o = row + (e >> 5) * 64 + (e & 31);
+        split(v, o[0], o[32]);
     } else {
-        o[0] = elem == TSC_ELEM_BF16 ? bits((__bf16)v) : bits((_Float16)v);
+        row[e] = elem == TSC_ELEM_BF16 ? bits((__bf16)v) : bits((_Float16)v);
     }
 }
 
@@ -90,9 +87,9 @@ __global__ void bias_kernel(const void *b, int elem, int V, int n, float *out) {
     out[v] = x < -1e38f ? -__builtin_inff() : x;
 }
 
-// out[r][c] = in[r * sr + c * sc], c < C, zero up to the pitch (of a plane); one of sr, sc is 1
+// out[r][c] = in[r * sr + c * sc], c < C, zero up to the pitch Cp; one of sr, sc is 1
 __global__ __launch_bounds__(256) void pack_w_kernel(const void *in, int elem, long long sr, long long sc, int R, int C, int Cp,
-                                                     int planes, const float *wscale, short *out) {
+                                                     const float *wscale, short *out) {
     __shared__ float t[64][65];
     const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, a = threadIdx.x & 63, b = threadIdx.x >> 6;
     for (int i = b; i < 64; i += 4) {
@@ -101,10 +98,11 @@ __global__ __launch_bounds__(256) void pack_w_kernel(const void *in, int elem, l
         t[sc == 1 ? i : a][sc == 1 ? a : i] = v;
     }
     __syncthreads();
+    const int planes = elem == TSC_ELEM_F32 ? 2 : 1;
     const float inv = elem == TSC_ELEM_F32 ? 1.f / wscale[0] : 1.f;
     for (int i = b; i < 64; i += 4) {
         const int r = r0 + i, c = c0 + a;
-        if (r < R && c < Cp) store_planes(out + (long long)r * planes * Cp + c, Cp, t[i][a] * inv, elem, planes);
+        if (r < R && c < Cp) store_value(out + (long long)r * planes * Cp, c, t[i][a] * inv, elem);
     }
 }
 
@@ -113,11 +111,11 @@ __device__ __forceinline__ long long row_at(const TscRows &r, long long row) {
 }
 
 // One wave a row: x[m] / s_m in planes of Dp elements, rows behind M (up to Mp) and rows without a loss zero; s_m to xscale.
-__global__ __launch_bounds__(256) void pack_x_kernel(const TscRows x, int elem, int M, int Mp, int D, int Dp, int planes,
+__global__ __launch_bounds__(256) void pack_x_kernel(const TscRows x, int elem, int M, int Mp, int D, int Dp,
                                                      const long long *targets, long long ignore, short *out, float *xscale) {
     const int m = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (m >= Mp) return;
-    short *o = out + (long long)m * planes * Dp;
+    short *o = out + (long long)m * (elem == TSC_ELEM_F32 ? 2 : 1) * Dp;
     const bool live = m < M && (!targets || targets[m] != ignore);
     const long long at = live ? row_at(x, m) : 0;
     float s = 1.f;
@@ -135,7 +133,7 @@ __global__ __launch_bounds__(256) void pack_x_kernel(const TscRows x, int elem, 
     const float inv = 1.f / s;
     for (int d = lane; d < Dp; d += 64) {
         const bool in = live && d < D;
-        if (elem == TSC_ELEM_F32) store_planes(o + d, Dp, in ? ((const float *)x.data)[at + d] * inv : 0.f, elem, planes);
+        if (elem == TSC_ELEM_F32) store_value(o, d, in ? ((const float *)x.data)[at + d] * inv : 0.f, elem);
         else o[d] = in ? ((const short *)x.data)[at + d] : (short)0;
     }
 }
@@ -191,7 +189,7 @@ __device__ __forceinline__ float2 merge(float2 a, float2 b) {
 
 struct LogitArgs {
     Operand W, x;
-    int nk, passes;
+    int nk;
     int nm, ns, nv, v0;  // blocks of rows, streams of a block, tiles of the vocabulary (counted from entry v0)
     int M, V;
     const float *bias;                  // -inf behind V
@@ -203,8 +201,8 @@ struct LogitArgs {
     float *hit;          // [M]
     // backward
     const float *lse, *rowf;
-    short *G;            // [Mp][ldg], second plane at gplane
-    long long ldg, gplane;
+    short *G;            // [Mp][PLANES * ldg]
+    long long ldg;
     int Mp;
     float *dbias;        // [parts of the rows][ldg] or null
 };
@@ -215,7 +213,7 @@ struct LogitArgs {
 // are, as long as nothing overflows (the tile is then repeated with its own maximum) -- what underflows is below 2^-126 of a
 // term that is already in the sum.
 template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::OCC) void loss_logits_kernel(const LogitArgs a) {
-    typedef Gemm<C, false, F16> G;
+    typedef Gemm<C, false, F16, SPLIT ? 2 : 1> G;
     __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
     int bj, st;
     tile_of(blockIdx.x, a.nm, a.ns, bj, st);
@@ -303,7 +301,7 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
             }
         }
     };
-    G::run(a.W, a.x, (a.nv - st + a.ns - 1) / a.ns, tile, 0, a.nk, a.passes, lds, begin, done);
+    G::run(a.W, a.x, (a.nv - st + a.ns - 1) / a.ns, tile, 0, a.nk, lds, begin, done);
     __syncthreads();  // the operand tiles are no longer read: their place takes the waves' parts
     float2 *sm = (float2 *)lds;
 #pragma unroll
@@ -324,7 +322,7 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
 // Backward, i = m, j = v: a lane holds one entry of the vocabulary and 16 WI rows of it, so db is a sum over its registers,
 // and two neighbouring lanes exchange halves to store two entries of a row each.  The rows' constants lie in LDS.
 template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::OCC) void grad_logits_kernel(const LogitArgs a) {
-    typedef Gemm<C, false, F16> G;
+    typedef Gemm<C, false, F16, SPLIT ? 2 : 1> G;
     __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
     __shared__ __attribute__((aligned(16))) float r_lse[C::BI], r_f[C::BI], r_sc[SPLIT ? C::BI : 4], r_inv[SPLIT ? C::BI : 4];
     __shared__ __attribute__((aligned(16))) int r_t[C::BI];
@@ -370,11 +368,12 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
                 hot |= ((unsigned)m ? 1u << (q * C::WI + i / 32) : 0u) | (i + 32 < C::WI * 32 && (m >> 32) ? 2u << (q * C::WI + i / 32) : 0u);
             }
         }
-        long long ld2 = a.ldg * 2;
+        constexpr int PL = SPLIT ? 2 : 1;
+        long long ld2 = a.ldg * 2 * PL;
         asm volatile("" : "+s"(ld2));  // (else the distances of all rows are computed once and spilled)
         // a lane stores row (lane & 1) of a pair of rows, columns col & ~1 and the next
-        char *base = (char *)(a.G + (long long)(i0 + wr) * a.ldg + v);
-        const unsigned lane_at = (unsigned)((4 * lh + (lane & 1)) * (int)a.ldg + (li & ~1)) * 2u;
+        char *base = (char *)(a.G + ((long long)(i0 + wr) * a.ldg + v) * PL);
+        const unsigned lane_at = (unsigned)((4 * lh + (lane & 1)) * (int)a.ldg * PL + (li & ~1)) * 2u;
         float db[C::WJ], b2[C::WJ];
 #pragma unroll
         for (int q = 0; q < C::WJ; ++q) {
@@ -409,7 +408,7 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
                 for (int e = 0; e < 4; e += 2) {
                     auto put = [&](unsigned own, char *to) __attribute__((always_inline)) {
                         const unsigned other = __builtin_amdgcn_update_dpp(0, own, 0xB1, 0xF, 0xF, true);  // lane ^ 1
-                        *(unsigned *)(to + e * ld2 + q * 64 + lane_at) = __builtin_amdgcn_perm(other, own, sel);
+                        *(unsigned *)(to + e * ld2 + q * 64 * PL + lane_at) = __builtin_amdgcn_perm(other, own, sel);
                     };
                     const f32x2 pair = {w[e], w[e + 1]};
                     if constexpr (F16) {
@@ -417,7 +416,7 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
                         put(__builtin_bit_cast(unsigned, h), row);
                         if constexpr (SPLIT) {  // h2 is held times 2048
                             const f32x2 r = {fmaf((float)h[0], -2048.f, pair[0] * 2048.f), fmaf((float)h[1], -2048.f, pair[1] * 2048.f)};
-                            put(__builtin_bit_cast(unsigned, __builtin_convertvector(r, f16x2)), row + a.gplane * 2);
+                            put(__builtin_bit_cast(unsigned, __builtin_convertvector(r, f16x2)), row + 64);
                         }
                     } else {
                         put(__builtin_bit_cast(unsigned, __builtin_convertvector(pair, bf16x2)), row);
@@ -449,7 +448,7 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
                 if (lh == 0) a.dbias[(long long)(bi * C::VI + wi) * a.ldg + v + q * 32 + li] = db[q];
             }
     };
-    G::run(a.x, a.W, (a.nv - st + a.ns - 1) / a.ns, tile, 0, a.nk, a.passes, lds, begin, done);
+    G::run(a.x, a.W, (a.nv - st + a.ns - 1) / a.ns, tile, 0, a.nk, lds, begin, done);
 }
 
 // lse and loss of the rows from the tiles' parts: one wave a row
@@ -469,19 +468,19 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2 *part, int n, in
 
 struct SumArgs {  // C[z][i][j] = (or +=) the z-th part of the k-steps
     Operand A, B;
-    int nk, per, passes, ti, tj, I, J, add;
+    int nk, per, ti, tj, I, J, add;
     float *out;
 };
 struct OutArgs {  // C[i][j] * post, in the elements' type
     Operand A, B;
-    int nk, passes, ti, tj, I, J;
+    int nk, ti, tj, I, J;
     const float *post;
     void *out;
     long long ld;
     int elem;
 };
-template <class C, bool KMAJOR, bool F16> __global__ __launch_bounds__(C::NT, C::OCC) void sum_kernel(const SumArgs a) {
-    typedef Gemm<C, KMAJOR, F16> G;
+template <class C, bool KMAJOR, bool F16, int PLANES, int SCALED> __global__ __launch_bounds__(C::NT, C::OCC) void sum_kernel(const SumArgs a) {
+    typedef Gemm<C, KMAJOR, F16, PLANES, SCALED> G;
     __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
     int bi, bj;
     tile_of(blockIdx.x, a.ti, a.tj, bi, bj);
@@ -507,10 +506,10 @@ template <class C, bool KMAJOR, bool F16> __global__ __launch_bounds__(C::NT, C:
                     *to = a.add ? *to + acc[p][q][r] : acc[p][q][r];
                 }
     };
-    G::run(a.A, a.B, 1, [&](int) { return TileAt{bi * C::BI, bj * C::BJ}; }, k0, k1, a.passes, lds, begin, done);
+    G::run(a.A, a.B, 1, [&](int) { return TileAt{bi * C::BI, bj * C::BJ}; }, k0, k1, lds, begin, done);
 }
-template <class C, bool F16> __global__ __launch_bounds__(C::NT, C::OCC) void out_kernel(const OutArgs a) {
-    typedef Gemm<C, true, F16> G;
+template <class C, bool F16, int PLANES, int SCALED> __global__ __launch_bounds__(C::NT, C::OCC) void out_kernel(const OutArgs a) {
+    typedef Gemm<C, true, F16, PLANES, SCALED> G;
     __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
     int bi, bj;
     tile_of(blockIdx.x, a.ti, a.tj, bi, bj);
@@ -534,7 +533,7 @@ template <class C, bool F16> __global__ __launch_bounds__(C::NT, C::OCC) void ou
                     if (wi0 + p * 32 + block_row(r, lh) < a.I && wj0 + q * 32 + li < a.J)
                         write_elem(a.out, a.elem, at + (long long)(p * 32 + block_row(r, 0)) * a.ld + q * 32, acc[p][q][r] * post);
     };
-    G::run(a.A, a.B, 1, [&](int) { return TileAt{bi * C::BI, bj * C::BJ}; }, 0, a.nk, a.passes, lds, begin, done);
+    G::run(a.A, a.B, 1, [&](int) { return TileAt{bi * C::BI, bj * C::BJ}; }, 0, a.nk, lds, begin, done);
 }
 // C = sum over z of the parts, for a dW whose k-steps were split
 __global__ __launch_bounds__(256) void join_kernel(const float *part, int n, int I, int J, const float *post, void *out, long long ld, int elem) {
@@ -578,10 +577,10 @@ constexpr long long PIECE_BYTES = 3ll << 29;  // G of one piece of the vocabular
 }  // namespace
 
 struct tsc_unembed {
-    int D, V, elem, belem, planes, wplanes, Dp, Vp, Vb;  // paddings: 64 for a product's k, 256 for the bias a tile reads
+    int D, V, elem, belem, planes, Dp, Vp, Vb;  // paddings: 64 for a product's k, 256 for the bias a tile reads
     long long sd, sv;                    // strides of W (elements): one of them is 1
     const void *W, *bias;                // borrowed
-    short *Wt, *Wd;                      // [V][planes of Dp] and [D][wplanes of Vp]
+    short *Wt, *Wd;                      // [V][planes * Dp] and [D][planes * Vp]
     float *bias32, *wscale;
 };
 
@@ -606,8 +605,8 @@ int tsc_unembed_refresh_(tsc_unembed *h, hipStream_t s) {
         hipLaunchKernelGGL(absmax_kernel, dim3((int)(rows < 1024 ? rows : 1024)), dim3(1024), 0, s, (const float *)h->W, rows, cols, ld, (unsigned *)h->wscale);
         hipLaunchKernelGGL(wscale_kernel, dim3(1), dim3(1), 0, s, h->wscale);
     }
-    hipLaunchKernelGGL(pack_w_kernel, dim3(h->Dp / 64, cdiv(h->V, 64)), dim3(256), 0, s, h->W, h->elem, h->sv, h->sd, h->V, h->D, h->Dp, h->planes, h->wscale, h->Wt);
-    hipLaunchKernelGGL(pack_w_kernel, dim3(h->Vp / 64, cdiv(h->D, 64)), dim3(256), 0, s, h->W, h->elem, h->sd, h->sv, h->D, h->V, h->Vp, h->wplanes, h->wscale, h->Wd);
+    hipLaunchKernelGGL(pack_w_kernel, dim3(h->Dp / 64, cdiv(h->V, 64)), dim3(256), 0, s, h->W, h->elem, h->sv, h->sd, h->V, h->D, h->Dp, h->wscale, h->Wt);
+    hipLaunchKernelGGL(pack_w_kernel, dim3(h->Vp / 64, cdiv(h->D, 64)), dim3(256), 0, s, h->W, h->elem, h->sd, h->sv, h->D, h->V, h->Vp, h->wscale, h->Wd);
     TSC_HIP_CHECK(hipGetLastError());
     return TSC_OK;
 }
@@ -615,11 +614,11 @@ int tsc_unembed_refresh_(tsc_unembed *h, hipStream_t s) {
 int tsc_unembed_create_(tsc_unembed **out, int D, int V, int elem, const void *W, long long sd, long long sv, const void *bias, int belem, hipStream_t s) {
     tsc_unembed *h = new (std::nothrow) tsc_unembed();
     if (!h) return tsc_fail(TSC_ERR_HIP, "out of host memory");
-    h->D = D; h->V = V; h->elem = elem; h->belem = belem; h->planes = elem == TSC_ELEM_F32 ? 2 : 1; h->wplanes = elem == TSC_ELEM_F32 ? 3 : 1;
+    h->D = D; h->V = V; h->elem = elem; h->belem = belem; h->planes = elem == TSC_ELEM_F32 ? 2 : 1;
     h->Dp = (int)up(D, BK); h->Vp = (int)up(V, 256); h->Vb = h->Vp + 256;
     h->sd = sd; h->sv = sv; h->W = W; h->bias = bias;
     hipError_t e = hipMalloc((void **)&h->Wt, (size_t)V * h->planes * h->Dp * 2);
-    if (e == hipSuccess) e = hipMalloc((void **)&h->Wd, (size_t)D * h->wplanes * h->Vp * 2);
+    if (e == hipSuccess) e = hipMalloc((void **)&h->Wd, (size_t)D * h->planes * h->Vp * 2);
     if (e == hipSuccess) e = hipMalloc((void **)&h->bias32, (size_t)h->Vb * 4);
     if (e == hipSuccess) e = hipMalloc((void **)&h->wscale, 256);
     int rc = e == hipSuccess ? tsc_unembed_refresh_(h, s) : tsc_fail(TSC_ERR_HIP, "hipMalloc of the unembedding's operands failed: %s", hipGetErrorString(e));
@@ -727,7 +726,7 @@ Plan plan(const tsc_unembed *h, long long M, bool backward, bool want_x, bool wa
     p.st = streams(M, nv);
     long long at = 0;
     auto take = [&](long long n) { const long long q = at; at = up(at + n, 256); return q; };
-    p.xp = take(2ll * (backward ? h->wplanes : h->planes) * p.Mp * h->Dp);
+    p.xp = take(2ll * h->planes * p.Mp * h->Dp);
     p.xscale = take(4 * M);
     if (!backward) {
         p.part = take(8ll * p.st.ns * M);
@@ -773,12 +772,11 @@ template <bool GRAD> int logits(const tsc_unembed *h, const Streams &st, const L
            : h->elem == TSC_ELEM_BF16 ? launch_logits<false, false, GRAD>(st, a, s)
                                       : launch_logits<true, false, GRAD>(st, a, s);
 }
-LogitArgs logit_args(const tsc_unembed *h, const Plan &p, char *ws, int xplanes, int M, const long long *targets, long long ignore) {
+LogitArgs logit_args(const tsc_unembed *h, const Plan &p, char *ws, int M, const long long *targets, long long ignore) {
     LogitArgs a{};
-    // x W: h2 h1', h1 h2', h1 h1'
-    a.W = {h->Wt, (long long)h->planes * h->Dp, 0, h->Dp, h->V};
-    a.x = {(const short *)(ws + p.xp), (long long)xplanes * h->Dp, h->Dp, 0, M};
-    a.nk = h->Dp / BK; a.passes = h->planes == 2 ? 3 : 1;
+    a.W = {h->Wt, (long long)h->planes * h->Dp, h->V};
+    a.x = {(const short *)(ws + p.xp), (long long)h->planes * h->Dp, M};
+    a.nk = h->Dp / BK;
     a.nm = p.st.nm; a.ns = p.st.ns; a.nv = p.st.nv; a.M = M; a.V = h->V;
     a.bias = h->bias32;
     a.wscale = h->planes == 2 ? h->wscale : nullptr;
@@ -786,32 +784,46 @@ LogitArgs logit_args(const tsc_unembed *h, const Plan &p, char *ws, int xplanes,
     a.targets = targets; a.ignore = ignore;
     return a;
 }
-template <bool KMAJOR> int launch_sum(const Split &w, bool f16, SumArgs &q, hipStream_t s) {
+// (elements of the operands; SCALED: the operand that is G, where it has two planes)
+#define TSC_BY_ELEM(KERNEL, TILE, SCALED, ...)                                                                                  \
+    {                                                                                                                           \
+        if (elem == TSC_ELEM_F32) hipLaunchKernelGGL((KERNEL<TILE, __VA_ARGS__ true, 2, SCALED>), grid, dim3(TILE::NT), 0, s, q);     \
+        else if (elem == TSC_ELEM_BF16) hipLaunchKernelGGL((KERNEL<TILE, __VA_ARGS__ false, 1, 0>), grid, dim3(TILE::NT), 0, s, q);   \
+        else hipLaunchKernelGGL((KERNEL<TILE, __VA_ARGS__ true, 1, 0>), grid, dim3(TILE::NT), 0, s, q);                               \
+    }
+#define TSC_COMMA ,
+int launch_dx(const Split &w, int elem, SumArgs &q, hipStream_t s) {
+    q.per = w.per; q.ti = w.ti; q.tj = w.tj;
+    const dim3 grid(w.ti * w.tj, w.z);
+    if (w.s.kind == LARGE) TSC_BY_ELEM(sum_kernel, TileLarge, 1, false TSC_COMMA)
+    else TSC_BY_ELEM(sum_kernel, TileMedium, 1, false TSC_COMMA)
+    TSC_HIP_CHECK(hipGetLastError());
+    return TSC_OK;
+}
+int launch_dw_parts(const Split &w, int elem, bool by_d, SumArgs &q, hipStream_t s) {
     q.per = w.per; q.ti = w.ti; q.tj = w.tj;
     const dim3 grid(w.ti * w.tj, w.z);
     if (w.s.kind == LARGE) {
-        if (f16) hipLaunchKernelGGL((sum_kernel<TileLarge, KMAJOR, true>), grid, dim3(TileLarge::NT), 0, s, q);
-        else hipLaunchKernelGGL((sum_kernel<TileLarge, KMAJOR, false>), grid, dim3(TileLarge::NT), 0, s, q);
+        if (by_d) TSC_BY_ELEM(sum_kernel, TileLarge, 2, true TSC_COMMA) else TSC_BY_ELEM(sum_kernel, TileLarge, 1, true TSC_COMMA)
     } else {
-        if (f16) hipLaunchKernelGGL((sum_kernel<TileMedium, KMAJOR, true>), grid, dim3(TileMedium::NT), 0, s, q);
-        else hipLaunchKernelGGL((sum_kernel<TileMedium, KMAJOR, false>), grid, dim3(TileMedium::NT), 0, s, q);
+        if (by_d) TSC_BY_ELEM(sum_kernel, TileMedium, 2, true TSC_COMMA) else TSC_BY_ELEM(sum_kernel, TileMedium, 1, true TSC_COMMA)
     }
     TSC_HIP_CHECK(hipGetLastError());
     return TSC_OK;
 }
-int launch_out(const Split &w, bool f16, OutArgs &q, hipStream_t s) {
+int launch_dw(const Split &w, int elem, bool by_d, OutArgs &q, hipStream_t s) {
     q.ti = w.ti; q.tj = w.tj;
     const dim3 grid(w.ti * w.tj);
     if (w.s.kind == LARGE) {
-        if (f16) hipLaunchKernelGGL((out_kernel<TileLarge, true>), grid, dim3(TileLarge::NT), 0, s, q);
-        else hipLaunchKernelGGL((out_kernel<TileLarge, false>), grid, dim3(TileLarge::NT), 0, s, q);
+        if (by_d) TSC_BY_ELEM(out_kernel, TileLarge, 2, ) else TSC_BY_ELEM(out_kernel, TileLarge, 1, )
     } else {
-        if (f16) hipLaunchKernelGGL((out_kernel<TileMedium, true>), grid, dim3(TileMedium::NT), 0, s, q);
-        else hipLaunchKernelGGL((out_kernel<TileMedium, false>), grid, dim3(TileMedium::NT), 0, s, q);
+        if (by_d) TSC_BY_ELEM(out_kernel, TileMedium, 2, ) else TSC_BY_ELEM(out_kernel, TileMedium, 1, )
     }
     TSC_HIP_CHECK(hipGetLastError());
     return TSC_OK;
 }
+#undef TSC_COMMA
+#undef TSC_BY_ELEM
 
 }  // namespace
 
@@ -822,9 +834,9 @@ size_t tsc_unembed_workspace_(const tsc_unembed *h, long long M, int backward, i
 int tsc_launch_unembed_loss(const tsc_unembed *h, const TscRows &x, int M, const long long *targets, long long ignore, float *loss,
                             float *lse, char *ws, hipStream_t s) {
     const Plan p = plan(h, M, false, false, false, false);
-    hipLaunchKernelGGL(pack_x_kernel, dim3(cdiv(p.Mp, 4)), dim3(256), 0, s, x, h->elem, M, p.Mp, h->D, h->Dp, h->planes, (const long long *)nullptr, ignore,
+    hipLaunchKernelGGL(pack_x_kernel, dim3(cdiv(p.Mp, 4)), dim3(256), 0, s, x, h->elem, M, p.Mp, h->D, h->Dp, (const long long *)nullptr, ignore,
                        (short *)(ws + p.xp), (float *)(ws + p.xscale));
-    LogitArgs a = logit_args(h, p, ws, h->planes, M, targets, ignore);
+    LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
     a.part = (float2 *)(ws + p.part);
     a.hit = (float *)(ws + p.hit);
     const int rc = logits<false>(h, p.st, a, s);
@@ -837,7 +849,6 @@ int tsc_launch_unembed_loss(const tsc_unembed *h, const TscRows &x, int M, const
 int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscRows &x, int M, const long long *targets, long long ignore,
                                 const float *lse, void *dx, void *dW, void *db, char *ws, hipStream_t s) {
     const bool f16 = h->elem != TSC_ELEM_BF16;
-    const int passes = h->planes == 2 ? 3 : 1;
     if (M == 0) {
         if (dW) hipLaunchKernelGGL(zero_elem_kernel, dim3(cdiv((long long)h->D * h->V, 256)), dim3(256), 0, s, dW, h->elem, (long long)h->D * h->V);
         if (db) hipLaunchKernelGGL(zero_elem_kernel, dim3(cdiv(h->V, 256)), dim3(256), 0, s, db, h->belem, (long long)h->V);
@@ -847,12 +858,12 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
     const Plan p = plan(h, M, true, dx != nullptr, dW != nullptr, db != nullptr);
     short *xp = (short *)(ws + p.xp), *G = (short *)(ws + p.g);
     float *xscale = (float *)(ws + p.xscale), *rowf = (float *)(ws + p.rowf), *post = (float *)(ws + p.post), *dxp = (float *)(ws + p.dxp);
-    hipLaunchKernelGGL(pack_x_kernel, dim3(cdiv(p.Mp, 4)), dim3(256), 0, s, x, h->elem, M, p.Mp, h->D, h->Dp, h->wplanes, targets, ignore, xp, xscale);
+    hipLaunchKernelGGL(pack_x_kernel, dim3(cdiv(p.Mp, 4)), dim3(256), 0, s, x, h->elem, M, p.Mp, h->D, h->Dp, targets, ignore, xp, xscale);
     hipLaunchKernelGGL(row_factor_kernel, dim3(1), dim3(1024), 0, s, g, xscale, targets, ignore, h->V, M, f16, rowf, post);
-    LogitArgs a = logit_args(h, p, ws, h->wplanes, M, targets, ignore);
-    a.lse = lse; a.rowf = rowf; a.G = G; a.ldg = p.Vc; a.gplane = (long long)p.Mp * p.Vc; a.Mp = p.Mp;
+    LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
+    a.lse = lse; a.rowf = rowf; a.G = G; a.ldg = p.Vc; a.Mp = p.Mp;
     a.dbias = db ? (float *)(ws + p.db) : nullptr;
-    const long long xld = (long long)h->wplanes * h->Dp;
+    const long long xld = (long long)h->planes * h->Dp;
     const int db_parts = p.st.nm * (p.st.s.kind == FEW ? 1 : 2);  // waves of a tile's rows
     for (int c = 0; c < p.pieces; ++c) {
         const int v0 = c * p.Vc, nv = h->V - v0 < p.Vc ? h->V - v0 : p.Vc;
@@ -864,17 +875,16 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
         if (db) hipLaunchKernelGGL(dbias_kernel, dim3(cdiv(nv, 256)), dim3(256), 0, s, a.dbias, db_parts, a.ldg, nv, post, h->belem, db, (long long)v0);
         if (dx) {
             SumArgs q{};
-            // G W^T: h2 (2048 of it) by h1' / 2048, h1 by h2', h1 by h1'
-            q.A = {G, p.Vc, a.gplane, 0, M};
-            q.B = {h->Wd + v0, (long long)h->wplanes * h->Vp, 2ll * h->Vp, h->Vp, h->D};
-            q.nk = cdiv(nv, BK); q.passes = passes; q.I = M; q.J = h->D; q.add = c > 0; q.out = dxp;
+            q.A = {G, (long long)h->planes * p.Vc, M};
+            q.B = {h->Wd + (long long)h->planes * v0, (long long)h->planes * h->Vp, h->D};
+            q.nk = cdiv(nv, BK); q.I = M; q.J = h->D; q.add = c > 0; q.out = dxp;
             Split w = p.dx;
             if (c > 0) w.per = cdiv(q.nk, w.z);  // the same parts, shorter
-            rc = launch_sum<false>(w, f16, q, s);
+            rc = launch_dx(w, h->elem, q, s);
             if (rc) return rc;
         }
         if (dW) {
-            const Operand X = {xp, xld, 2 * h->Dp, h->Dp, h->D}, Gk = {G, p.Vc, a.gplane, 0, nv};
+            const Operand X = {xp, xld, h->D}, Gk = {G, (long long)h->planes * p.Vc, nv};
             const bool by_d = h->sv == 1;  // dW is dense in W's order: [D][V] or [V][D]
             const Split w = dw_split(h, p.Mp, nv);
             const int I = by_d ? h->D : nv, J = by_d ? nv : h->D;
@@ -884,14 +894,14 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
                 OutArgs q{};
                 q.A = by_d ? X : Gk;
                 q.B = by_d ? Gk : X;
-                q.nk = p.Mp / BK; q.passes = passes; q.I = I; q.J = J; q.post = post; q.elem = h->elem; q.ld = ld; q.out = out;
-                rc = launch_out(w, f16, q, s);
+                q.nk = p.Mp / BK; q.I = I; q.J = J; q.post = post; q.elem = h->elem; q.ld = ld; q.out = out;
+                rc = launch_dw(w, h->elem, by_d, q, s);
             } else {
                 SumArgs q{};
                 q.A = by_d ? X : Gk;
                 q.B = by_d ? Gk : X;
-                q.nk = p.Mp / BK; q.passes = passes; q.I = I; q.J = J; q.out = (float *)(ws + p.dwp);
-                rc = launch_sum<true>(w, f16, q, s);
+                q.nk = p.Mp / BK; q.I = I; q.J = J; q.out = (float *)(ws + p.dwp);
+                rc = launch_dw_parts(w, h->elem, by_d, q, s);
                 if (!rc) hipLaunchKernelGGL(join_kernel, dim3(cdiv((long long)I * J, 256)), dim3(256), 0, s, q.out, w.z, I, J, post, out, ld, h->elem);
             }
             if (rc) return rc;

@@ -16,13 +16,16 @@
 // What bounds the loop is power: at 70 % of its issue slots the matrix pipe runs at 1.5-1.6 GHz on real operands, and the
 // vendor's own kernel, at 94 %, at 1.44 (1340-1375 TFLOP/s at 8192^3; this loop 1292).
 //
-// fp32 operands are split into fp16 planes: v / s = h1 + h2, s a power of two that brings the largest magnitude into
+// fp32 operands are split into two fp16 planes: v / s = h1 + h2, s a power of two that brings the largest magnitude into
 // [2^14, 2^15).  h1 holds 11 bits and h2 the next 11: 22 bits for values down to 2^-17 of the largest, a fixed 2^-39 of it
-// below (fp16 ends at 2^-24).  The product is three passes over k, h2 h1' + h1 h2' + h1 h1', the small terms first; the
-// dropped h2 h2' is 2^-22 of the product at most.  Every product of two fp16 values is exact in the matrix pipe, sums are
-// fp32: the result carries the error of an fp32 product at a third of the 16-bit rate, 5 times the fp32 matrix rate.
+// below (fp16 ends at 2^-24).  The product is h1 h1' + h1 h2' + h2 h1'; the dropped h2 h2' is 2^-22 of it at most.  Every
+// product of two fp16 values is exact in the matrix pipe, sums are fp32: the result carries the error of an fp32 product at
+// a third of the 16-bit rate, 5 times the fp32 matrix rate.
 // G, whose entries are probabilities and span many more powers of two, is split as h1 + h2 / 2048: 22 bits down to 2^-28 of
-// the largest and a fixed 2^-50 of it below; the pass with its h2 reads a plane h1' / 2048 of the other operand.
+// the largest and a fixed 2^-50 of it below; the other operand's h1 is divided by 2048 in registers before it meets that h2.
+// The planes of 32 neighbouring elements lie next to each other, element e's h1 at e / 32 * 64 + e % 32 and its h2 32 behind
+// it: a cache line holds both, and a step brings both planes of half as many k through LDS for three products, where one
+// pass a product would bring each plane three times in two.
 #pragma once
 #include <type_traits>
 
@@ -59,9 +62,8 @@ typedef Tile<2, 1, 1, 4> TileWide;    // 64 x 128: the same with the operands ex
 
 struct Operand {
     const short *p;
-    long long ld;             // elements between rows (row-major) or between k (k-major)
-    long long first, second;  // elements from plane h1 to the plane that the first (the second) of three passes reads
-    int rows;         // valid i (j); the tile's others read copies of valid ones
+    long long ld;  // 16-bit elements (of both planes) between rows (row-major) or between k (k-major)
+    int rows;      // valid i (j); the tile's others read copies of valid ones
 };
 
 // 16 bytes a lane, global -> LDS: base + off (of the lane) to LDS address at + 16 * lane.  Written out, and not through the
@@ -88,9 +90,11 @@ struct TileAt {
 //            products of the last group while the first fragments of step s + 1 are read and the copies of step s + NS issued
 //
 // Behind the barrier nobody reads the buffer of step s any more and everybody's part of step s + 1 is there.
-template <class C, bool KMAJOR, bool F16> struct Gemm {
-    static constexpr int SK = KMAJOR ? 32 : 64, NS = KMAJOR ? 4 : 2, KK = SK / 16;
-    static constexpr int ABYTES = C::BI * SK * 2, BBYTES = C::BJ * SK * 2, STAGE = ABYTES + BBYTES;
+// SCALED (two planes): the operand whose h2 is held times 2048 -- 0: none, 1: A, 2: B.
+template <class C, bool KMAJOR, bool F16, int PLANES, int SCALED = 0> struct Gemm {
+    static_assert(PLANES == 1 || F16, "planes are fp16");
+    static constexpr int SK = (KMAJOR ? 32 : 64) / PLANES, NS = KMAJOR ? 4 : 2, KK = SK / 16;
+    static constexpr int ABYTES = C::BI * SK * PLANES * 2, BBYTES = C::BJ * SK * PLANES * 2, STAGE = ABYTES + BBYTES;
     static constexpr int LDS_BYTES = NS * STAGE;
     static constexpr int PA = ABYTES / 1024 / C::NW, PB = BBYTES / 1024 / C::NW, P = PA + PB;  // 1-KiB pieces of a step and wave
     static_assert(P * C::NW * 1024 == STAGE, "whole pieces a wave");
@@ -103,9 +107,9 @@ template <class C, bool KMAJOR, bool F16> struct Gemm {
         for (int q = 0; q < PIECES; ++q) {
             const int piece = wave * PIECES + q;
             if (KMAJOR) {
-                constexpr int CH = ROWS / 8;  // 16-byte chunks of a k
+                constexpr int CH = ROWS * PLANES / 8;  // 16-byte chunks of a k
                 const int at = piece * 64 + lane, k = at / CH, c = (at % CH) ^ (((k & 3) << 2) & (CH - 1));
-                const int last = (o.rows + 7) / 8 * 8 - 8 - row0;
+                const int last = (PLANES == 2 ? (o.rows + 31) / 32 * 64 : (o.rows + 7) / 8 * 8) - 8 - row0 * PLANES;
                 const int i = c * 8 < last ? c * 8 : last;  // (last >= 0: a tile has at least one row)
                 off[q] = (unsigned)(k * (int)o.ld + i) * 2u;
             } else {
@@ -116,37 +120,39 @@ template <class C, bool KMAJOR, bool F16> struct Gemm {
         }
     }
     static __device__ __forceinline__ const char *base(const Operand &o, int row0, int k0) {
-        return (const char *)(o.p + (KMAJOR ? (long long)k0 * BK * o.ld + row0 : (long long)row0 * o.ld + (long long)k0 * BK));
+        return (const char *)(o.p + (KMAJOR ? (long long)k0 * BK * o.ld + row0 * PLANES : (long long)row0 * o.ld + (long long)k0 * BK * PLANES));
     }
-    static __device__ __forceinline__ long long step_bytes(const Operand &o) { return KMAJOR ? 2ll * SK * o.ld : 2ll * SK; }
+    static __device__ __forceinline__ long long step_bytes(const Operand &o) { return KMAJOR ? 2ll * SK * o.ld : 128; }
 
-    template <int ROWS> struct Frag {  // fragment reads of one operand: one LDS address for each of a step's four groups of 16 k
-        unsigned at[KK];
+    template <int ROWS> struct Frag {  // fragment reads of one operand
+        static constexpr int PITCH = ROWS * PLANES * 2;   // k-major: bytes of a k
+        unsigned at[KMAJOR ? KK : KK * PLANES];           // LDS address of block 0: of each 16 k, row-major also of each plane
         __device__ __forceinline__ Frag(int row0, int extra) {
-            const int lane = threadIdx.x & 63;
+            const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5;
+            if constexpr (KMAJOR) {
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
-                if constexpr (KMAJOR) {
-                    const int l = lane & 15, g = lane >> 4;
-                    const int i = row0 + (g & 1) * 16 + (l & 3) * 4, k = kk * 16 + (g >> 1) * 8 + (l >> 2);
-                    at[kk] = extra + k * ROWS * 2 + (((i >> 3) ^ (((k & 3) << 2) & (ROWS / 8 - 1))) << 4) + (i & 4) * 2;
-                } else {
-                    const int li = lane & 31, lh = lane >> 5;
-                    at[kk] = extra + (row0 + li) * 128 + (((kk * 2 + lh) ^ ((li >> 1) & 7)) << 4);
+                for (int kk = 0; kk < KK; ++kk) {
+                    const int l = lane & 15, g = lane >> 4, k = kk * 16 + (g >> 1) * 8 + (l >> 2);
+                    const int i = (g & 1) * 16 + (l & 3) * 4;  // of the block
+                    const int chunk = row0 * PLANES / 8 + (i >> 3);
+                    at[kk] = extra + k * PITCH + ((chunk ^ (((k & 3) << 2) & (ROWS * PLANES / 8 - 1))) << 4) + (i & 4) * 2;
                 }
+            } else {
+#pragma unroll
+                for (int c = 0; c < KK * PLANES; ++c) at[c] = extra + (row0 + li) * 128 + (((c * 2 + lh) ^ ((li >> 1) & 7)) << 4);
             }
         }
-        // rows row0 + 32 * b of k group kk: lane l holds row l % 32, k = 8 * (l / 32) + 0..7
-        __device__ __forceinline__ s16x8 read(const char *lds, unsigned buf, int kk, int b) const {
+        // rows row0 + 32 * b, 16 k number kk, a plane: lane l holds row l % 32, k = 8 * (l / 32) + 0..7
+        __device__ __forceinline__ s16x8 read(const char *lds, unsigned buf, int kk, int plane, int b) const {
             if constexpr (KMAJOR) {
-                // the chunk permutation acts on the 64-byte groups, so a block's distance of 64 bytes is an exclusive or too
+                // the chunk permutation acts on the 64-byte groups, so a block's distance, 64 bytes a plane, is an exclusive or too
                 typedef __attribute__((address_space(3))) s16x4 *p4;
-                const char *p = lds + (at[kk] ^ (b * 64)) + buf;
+                const char *p = lds + (at[kk] ^ ((b * PLANES + plane) * 64)) + buf;
                 const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lptr_t)p);
-                const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lptr_t)(p + 4 * ROWS * 2));
+                const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lptr_t)(p + 4 * PITCH));
                 return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
             } else {
-                return *(const s16x8 *)(lds + at[kk] + buf + b * 4096);
+                return *(const s16x8 *)(lds + at[plane * KK + kk] + buf + b * 4096);
             }
         }
     };
@@ -157,13 +163,17 @@ template <class C, bool KMAJOR, bool F16> struct Gemm {
             return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
 
-    // tiles t = 0 .. n_tiles - 1 at tile(t); k-steps [k0, k1) in passes 1 (16-bit operands) or 3 (split fp32).
-    // begin(t, acc) sets a tile's accumulators, done(t, acc) takes its sums.  LDS of the stages: lds[0 .. LDS_BYTES).
+    static __device__ __forceinline__ s16x8 smaller(s16x8 h) {  // h1 / 2048
+        return __builtin_bit_cast(s16x8, __builtin_bit_cast(f16x8, h) * (_Float16)(1.f / 2048.f));
+    }
+
+    // tiles t = 0 .. n_tiles - 1 at tile(t), k from k0 * BK to k1 * BK.  begin(t, acc) sets a tile's accumulators,
+    // done(t, acc) takes its sums.  LDS of the stages: lds[0 .. LDS_BYTES).
     template <class At, class Begin, class Done>
-    static __device__ __forceinline__ void run(const Operand &A, const Operand &B, int n_tiles, At tile, int k0, int k1, int passes,
-                                               char *lds, Begin begin, Done done) {
+    static __device__ __forceinline__ void run(const Operand &A, const Operand &B, int n_tiles, At tile, int k0, int k1, char *lds,
+                                               Begin begin, Done done) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const int n = (k1 - k0) * (BK / SK), total = n * passes;
+        const int n = (k1 - k0) * (BK / SK);
         f32x16 acc[C::WI][C::WJ];
         if (n_tiles <= 0) return;
         if (n <= 0) {  // (a part of the k-steps behind their end)
@@ -177,21 +187,16 @@ template <class C, bool KMAJOR, bool F16> struct Gemm {
         const Frag<C::BJ> rb((wave % C::VJ) * (C::WJ * 32), ABYTES);
         unsigned offa[PA], offb[PB];
         // the producer: the next step to copy
-        int pt = 0, pp = passes == 1 ? 2 : 0, ps = 0;  // tile, pass (of one-plane operands: the last), step of the pass
+        int pt = 0, ps = 0;
         unsigned pbuf = 0;
-        const char *a0, *b0, *pa, *pb;
+        const char *pa, *pb;
         const long long da = step_bytes(A), db = step_bytes(B);
-        auto set_pass = [&]() {
-            pa = a0 + (pp == 0 ? A.first : pp == 1 ? A.second : 0) * 2;
-            pb = b0 + (pp == 0 ? B.first : pp == 1 ? B.second : 0) * 2;
-        };
         auto set_tile = [&]() {
             const TileAt at = tile(pt);
             offsets<C::BI, PA>(A, at.i0, offa);
             offsets<C::BJ, PB>(B, at.j0, offb);
-            a0 = base(A, at.i0, k0);
-            b0 = base(B, at.j0, k0);
-            set_pass();
+            pa = base(A, at.i0, k0);
+            pb = base(B, at.j0, k0);
         };
         const unsigned l0 = (unsigned)(size_t)(lptr_t)lds, la = l0 + wave * PA * 1024, lb = l0 + ABYTES + wave * PB * 1024;
         auto piece = [&](int q) {
@@ -205,16 +210,11 @@ template <class C, bool KMAJOR, bool F16> struct Gemm {
                 pb += db;
                 return;
             }
-            if (pp < 2) {
-                ps = 0;
-                ++pp;
-                set_pass();
-            } else if (pt + 1 < n_tiles) {
+            if (pt + 1 < n_tiles) {
                 ps = 0;
                 ++pt;
-                pp = passes == 1 ? 2 : 0;
                 set_tile();
-            }  // else: the stream is at its end, its last step is copied again (twice, unread: no branch in the loop)
+            }  // else: the stream is at its end, its last step is copied again (NS times, unread: no branch in the loop)
         };
         set_tile();
         for (int i = 0; i < NS; ++i) {
@@ -225,47 +225,94 @@ template <class C, bool KMAJOR, bool F16> struct Gemm {
         asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1) * P) : "memory");
         s16x8 fa[2][C::WI], fb[2][C::WJ];
         unsigned buf = 0;
-        // a group of 16 k: products of the fragments `now`, and between them the reads of group kk of the buffer at `from` into
-        // the other set and (COPY) the step's copies -- one behind each product, in this order: a burst of either would leave
-        // the matrix pipe idle, and so would the compiler's own order
-        auto group = [&](auto now_, auto copy_, int kk, unsigned from) {
-            constexpr int NOW = decltype(now_)::value, G = C::WI * C::WJ, R = C::WI + C::WJ;
+        constexpr int G = C::WI * C::WJ;
+        // all products of fragments x and y, and behind each of them a part of the `reads` fragment reads read(r) and (COPY) of
+        // the step's copies, in this order: a burst of either would leave the matrix pipe idle, and so would the compiler's
+        // own order.  The reads end with the first half of the products.
+        auto group = [&](const s16x8(&x)[C::WI], const s16x8(&y)[C::WJ], auto copy_, auto reads_, auto read) __attribute__((always_inline)) {
+            constexpr int R = decltype(reads_)::value;
             constexpr bool COPY = decltype(copy_)::value;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const int a = g / C::WJ, b = a & 1 ? C::WJ - 1 - g % C::WJ : g % C::WJ;  // (back and forth: one operand stays)
-                acc[a][b] = mfma(fa[NOW][a], fb[NOW][b], acc[a][b]);
+                acc[a][b] = mfma(x[a], y[b], acc[a][b]);
                 __builtin_amdgcn_sched_barrier(0);
-                // the reads end with the first half of the products (one more for the copies' group: their own come first)
 #pragma unroll
-                for (int r = g * 2 * R / G; r < (g + 1) * 2 * R / G && r < R; ++r) {
-                    if (r < C::WJ) fb[NOW ^ 1][r < C::WJ ? r : 0] = rb.read(lds, from, kk, r);
-                    else fa[NOW ^ 1][r < C::WJ ? 0 : r - C::WJ] = ra.read(lds, from, kk, r - C::WJ);
-                }
+                for (int r = g * 2 * R / G; r < (g + 1) * 2 * R / G && r < R; ++r) read(r);
                 if (COPY)
 #pragma unroll
                     for (int q = g * P / G; q < (g + 1) * P / G; ++q) piece(q);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
+        const std::false_type no;
+        const std::true_type yes;
+        const std::integral_constant<int, C::WI> wi;
+        const std::integral_constant<int, C::WJ> wj;
+        const std::integral_constant<int, C::WI + C::WJ> both;
+        auto next_step = [&]() __attribute__((always_inline)) {  // own reads of this step's buffer are done, the next step is there
+            buf = buf + STAGE == LDS_BYTES ? 0 : buf + STAGE;
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * P) : "memory");
+        };
+        // reads of the 16 k number kk: both operands' h1 into sets sa and sb
+        auto first = [&](int kk, int sa, int sb) {
+            return [&, kk, sa, sb](int r) __attribute__((always_inline)) {
+                if (r < C::WJ) fb[sb][r < C::WJ ? r : 0] = rb.read(lds, buf, kk, 0, r);
+                else fa[sa][r < C::WJ ? 0 : r - C::WJ] = ra.read(lds, buf, kk, 0, r - C::WJ);
+            };
+        };
+        // Two planes: the three products of 16 k.  The set that is free before the last product takes the next h1 of its operand,
+        // so one operand's h1 changes between the sets from one 16 k to the next (PAR).
+        //   SCALED 0, 1: h1 h1', h1 h2', h2 h1' -- B's h1 in set PAR;     SCALED 2: h1 h1', h2 h1', h1 h2' -- A's h1 in set PAR
+        auto three = [&](auto par_, auto last_, int kk, int kk_next) __attribute__((always_inline)) {
+            constexpr int PAR = decltype(par_)::value;
+            constexpr bool LAST = decltype(last_)::value;  // of its step
+            if constexpr (SCALED == 2) {
+                group(fa[PAR], fb[0], no, wi, [&](int r) __attribute__((always_inline)) { fa[PAR ^ 1][r] = ra.read(lds, buf, kk, 1, r); });
+                group(fa[PAR ^ 1], fb[0], no, wj, [&](int r) __attribute__((always_inline)) { fb[1][r] = rb.read(lds, buf, kk, 1, r); });
 #pragma unroll
-        for (int r = 0; r < C::WJ; ++r) fb[0][r] = rb.read(lds, 0, 0, r);
+                for (int a = 0; a < C::WI; ++a) fa[PAR][a] = smaller(fa[PAR][a]);
+                if constexpr (LAST) next_step();
+                group(fa[PAR], fb[1], last_, both, first(kk_next, PAR ^ 1, 0));
+            } else {
+                group(fa[0], fb[PAR], no, wj, [&](int r) __attribute__((always_inline)) { fb[PAR ^ 1][r] = rb.read(lds, buf, kk, 1, r); });
+                group(fa[0], fb[PAR ^ 1], no, wi, [&](int r) __attribute__((always_inline)) { fa[1][r] = ra.read(lds, buf, kk, 1, r); });
+                if constexpr (SCALED == 1) {
 #pragma unroll
-        for (int r = 0; r < C::WI; ++r) fa[0][r] = ra.read(lds, 0, 0, r);
+                    for (int b = 0; b < C::WJ; ++b) fb[PAR][b] = smaller(fb[PAR][b]);
+                }
+                if constexpr (LAST) next_step();
+                group(fa[1], fb[PAR], last_, both, first(kk_next, 0, PAR ^ 1));
+            }
+            if constexpr (LAST) advance();
+        };
         const std::integral_constant<int, 0> even;
         const std::integral_constant<int, 1> odd;
+#pragma unroll
+        for (int r = 0; r < C::WI + C::WJ; ++r) first(0, 0, 0)(r);
         for (int t = 0; t < n_tiles; ++t) {
             begin(t, acc);
-            for (int s = 0; s < total; ++s) {
-                if constexpr (KK == 4) {
-                    group(even, std::false_type(), 1, buf);
-                    group(odd, std::false_type(), 2, buf);
+            if constexpr (PLANES == 1) {
+                for (int s = 0; s < n; ++s) {
+                    if constexpr (KK == 4) {
+                        group(fa[0], fb[0], no, both, first(1, 1, 1));
+                        group(fa[1], fb[1], no, both, first(2, 0, 0));
+                    }
+                    group(fa[0], fb[0], no, both, first(KK - 1, 1, 1));
+                    next_step();
+                    group(fa[1], fb[1], yes, both, first(0, 0, 0));  // (behind the last tile's last step these are not used)
+                    advance();
                 }
-                group(even, std::false_type(), KK - 1, buf);
-                buf = buf + STAGE == LDS_BYTES ? 0 : buf + STAGE;
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * P) : "memory");
-                group(odd, std::true_type(), 0, buf);  // (behind the last step of the last tile these fragments are not used)
-                advance();
+            } else if constexpr (KK == 2) {
+                for (int s = 0; s < n; ++s) {
+                    three(even, no, 0, 1);
+                    three(odd, yes, 1, 0);
+                }
+            } else {
+                for (int s = 0; s < n; s += 2) {  // (n is a multiple of 4)
+                    three(even, yes, 0, 0);
+                    three(odd, yes, 0, 0);
+                }
             }
             done(t, acc);
         }
