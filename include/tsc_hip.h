@@ -438,7 +438,8 @@ int tsc_layer_norm_backward(int elem, const tsc_rows_t *dy, const tsc_rows_t *x,
  * the unembedding is passed as its transpose: stride_d 1, stride_v d_model), the other one at least as long as the axis it
  * steps over.  bias [d_vocab] in bias_elem or NULL; an entry below -1e38 takes that token out
  * (probability 0; a row for which none is left has the loss NaN).  Both are borrowed.
- * The handle owns what the matrix pipe reads: W in both orders, padded, in 16 bits -- for TSC_ELEM_F32 as two fp16 planes
+ * The handle owns what the matrix pipe reads: W in both orders, padded, in 16 bits (an order that a 16-bit W has already, at
+ * 16-byte alignment and with an inner axis that is a multiple of 64, is read in place) -- for TSC_ELEM_F32 as two fp16 planes
  * that hold 22 bits of every weight down to 2^-17 of the largest and a fixed 2^-39 of it below -- 2 x 77 MB (fp32: 2 x 154)
  * at 768 x 50257.  After an in-place change of W or bias call tsc_unembed_refresh, in order with the calls that use the
  * handle.  d_model <= 32768, d_vocab <= 2^20.  One handle may be used from several streams.
@@ -469,7 +470,7 @@ int tsc_unembed_loss(const tsc_unembed_t *head, const tsc_rows_t *x, int64_t row
  *   G[m][v] = dloss[m] (exp(l[m][v] - lse[m]) - [v = targets[m]]),  dx = G W^T,  dW = x^T G,  dbias = sum over rows of G.
  * dx [rows, d_model] dense; dW dense in W's order ([d_model, d_vocab] where stride_v is 1, else [d_vocab, d_model]); dbias
  * [d_vocab] in bias_elem; each may be NULL = not wanted.  Ignored rows have a zero dx and add nothing, whatever they hold; a
- * target outside the vocabulary makes its row's dx and all of dW NaN.  G is made in pieces of the vocabulary (1.5 GiB of
+ * target outside the vocabulary makes its row's dx and all of dW NaN.  G is made in pieces of the vocabulary (2 GiB of
  * workspace) and rounded to 16 bits as the operand of the two products (fp32: two planes, 22 bits down to 2^-28 of the
  * largest and a fixed 2^-50 of it below; fp16: 11 bits down to 2^-28, a fixed 2^-39 below; the largest: of |dloss|, for fp32
  * of |dloss| times the row's largest |x|).  dbias sums unrounded values.

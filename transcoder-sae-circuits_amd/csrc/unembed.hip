@@ -45,16 +45,6 @@ __device__ __forceinline__ void split(float v, short &h1, short &h2) {
     h1 = bits(a);
     h2 = fabsf((float)a) < __builtin_inff() ? bits((_Float16)(v - (float)a)) : (short)0;
 }
-// element e of a row of 16-bit values, or of two planes
-__device__ __forceinline__ void store_value(short *row, long long e, float v, int elem) {
-    if (elem == TSC_ELEM_F32) {
-        short *o = row + (e >> 5) * 64 + (e & 31);
-        split(v, o[0], o[32]);
-    } else {
-        row[e] = elem == TSC_ELEM_BF16 ? bits((__bf16)v) : bits((_Float16)v);
-    }
-}
-
 // ------------------------------------------------------------------------------------------------ operands
 __global__ __launch_bounds__(1024) void absmax_kernel(const float *w, long long rows, long long cols, long long ld, unsigned *top) {
     float m = 0.f;
@@ -87,22 +77,50 @@ __global__ void bias_kernel(const void *b, int elem, int V, int n, float *out) {
     out[v] = x < -1e38f ? -__builtin_inff() : x;
 }
 
-// out[r][c] = in[r * sr + c * sc], c < C, zero up to the pitch Cp; one of sr, sc is 1
-__global__ __launch_bounds__(256) void pack_w_kernel(const void *in, int elem, long long sr, long long sc, int R, int C, int Cp,
-                                                     const float *wscale, short *out) {
-    __shared__ float t[64][65];
-    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, a = threadIdx.x & 63, b = threadIdx.x >> 6;
-    for (int i = b; i < 64; i += 4) {
-        const int r = sc == 1 ? r0 + i : r0 + a, c = sc == 1 ? c0 + a : c0 + i;
-        const float v = r < R && c < C ? read_elem(in, elem, r * sr + c * sc) : 0.f;
-        t[sc == 1 ? i : a][sc == 1 ? a : i] = v;
+// 16 bytes of elements at an element's alignment
+template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Vec { T e[16 / sizeof(T)]; };
+
+// out[r][c] = in[r * sr + c * sc], c < C, zero up to the pitch Cp; one of sr, sc is 1.  64 x 64 elements a workgroup, 16 bytes
+// a lane on both sides.  T: float (two planes) or the bits of a 16-bit type.
+template <class T> __global__ __launch_bounds__(256) void pack_w_kernel(const T *in, long long sr, long long sc, int R, int C, int Cp,
+                                                                        const float *wscale, short *out) {
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int VE = 16 / sizeof(T), PER = 64 / VE;
+    __shared__ T t[64][64 + 4 / sizeof(T)];
+    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+    for (int i = threadIdx.x; i < 64 * PER; i += 256) {
+        const int line = i / PER, at = i % PER * VE;  // along the axis of stride 1
+        const int r = r0 + (sc == 1 ? line : at), c = c0 + (sc == 1 ? at : line);
+        const T *p = in + r * sr + c * sc;
+        if (sc == 1 ? r < R && c + VE <= C : c < C && r + VE <= R) {
+            const Vec<T> v = *(const Vec<T> *)p;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) t[sc == 1 ? line : at + e][sc == 1 ? at + e : line] = v.e[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                const bool ok = sc == 1 ? r < R && c + e < C : c < C && r + e < R;
+                t[sc == 1 ? line : at + e][sc == 1 ? at + e : line] = ok ? p[e] : (T)0;
+            }
+        }
     }
     __syncthreads();
-    const int planes = elem == TSC_ELEM_F32 ? 2 : 1;
-    const float inv = elem == TSC_ELEM_F32 ? 1.f / wscale[0] : 1.f;
-    for (int i = b; i < 64; i += 4) {
-        const int r = r0 + i, c = c0 + a;
-        if (r < R && c < Cp) store_value(out + (long long)r * planes * Cp, c, t[i][a] * inv, elem);
+    const float inv = SPLIT ? 1.f / wscale[0] : 1.f;
+    for (int i = threadIdx.x; i < 64 * 8; i += 256) {  // 8 elements of a row (Cp is a multiple of 64)
+        const int line = i / 8, at = i % 8 * 8, r = r0 + line, c = c0 + at;
+        if (r >= R) continue;
+        s16x8 h1, h2;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            short x, y = 0;
+            if constexpr (SPLIT) split(t[line][at + e] * inv, x, y);
+            else x = t[line][at + e];
+            h1[e] = x;
+            h2[e] = y;
+        }
+        short *o = out + (SPLIT ? (long long)r * 2 * Cp + (c >> 5) * 64 + (c & 31) : (long long)r * Cp + c);
+        *(s16x8 *)o = h1;
+        if constexpr (SPLIT) *(s16x8 *)(o + 32) = h2;
     }
 }
 
@@ -110,61 +128,77 @@ __device__ __forceinline__ long long row_at(const TscRows &r, long long row) {
     return (row / r.inner) * r.outer_stride + (row % r.inner) * r.inner_stride;
 }
 
-// One wave a row: x[m] / s_m in planes of Dp elements, rows behind M (up to Mp) and rows without a loss zero; s_m to xscale.
-__global__ __launch_bounds__(256) void pack_x_kernel(const TscRows x, int elem, int M, int Mp, int D, int Dp,
-                                                     const long long *targets, long long ignore, short *out, float *xscale) {
-    const int m = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (m >= Mp) return;
-    short *o = out + (long long)m * (elem == TSC_ELEM_F32 ? 2 : 1) * Dp;
-    const bool live = m < M && (!targets || targets[m] != ignore);
-    const long long at = live ? row_at(x, m) : 0;
-    float s = 1.f;
-    if (elem == TSC_ELEM_F32) {
-        float top = 0.f;
-        if (live)
-            for (int d = lane; d < D; d += 64) {
-                const float v = fabsf(((const float *)x.data)[at + d]);
-                top = v < __builtin_inff() ? fmaxf(top, v) : top;
+// One wave a row, n rows one after the other: x[m] / s_m, pitch Dp, rows behind M (up to Mp) and rows without a loss zero; s_m
+// to xscale (fp32).  With gtop: it takes the largest |g_m| s_m, from which G is scaled (a maximum does not depend on the order
+// of the atomics; one a workgroup, only where it raises the value).
+template <class T> __global__ __launch_bounds__(256) void pack_x_kernel(const TscRows x, int M, int Mp, int D, int Dp, int n, const long long *targets,
+                                                                        long long ignore, const float *g, short *out, float *xscale, unsigned *gtop) {
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int VE = 16 / sizeof(T);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float most = 0.f;
+    for (int m = (blockIdx.x * 4 + wave) * n, end = m + n < Mp ? m + n : Mp; m < end; ++m) {
+        short *o = out + (long long)m * (SPLIT ? 2 : 1) * Dp;
+        const bool live = m < M && (!targets || targets[m] != ignore);
+        const T *p = (const T *)x.data + (live ? row_at(x, m) : 0);
+        float s = 1.f;
+        if constexpr (SPLIT) {
+            float top = 0.f;
+            if (live)
+                for (int d = lane * VE; d < D; d += 64 * VE)
+                    if (d + VE <= D) {
+                        const Vec<T> v = *(const Vec<T> *)(p + d);
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) top = fabsf(v.e[e]) < __builtin_inff() ? fmaxf(top, fabsf(v.e[e])) : top;
+                    } else {
+                        for (int e = d; e < D; ++e) top = fabsf(p[e]) < __builtin_inff() ? fmaxf(top, fabsf(p[e])) : top;
+                    }
+            for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
+            s = pow2_scale(top);
+            if (lane == 0 && m < M) xscale[m] = s;
+        }
+        if (gtop && live) {
+            const float v = fabsf(g[m] * s);
+            most = v < __builtin_inff() ? fmaxf(most, v) : most;
+        }
+        const float inv = 1.f / s;
+        for (int d = lane * VE; d < Dp; d += 64 * VE) {
+            Vec<T> v;
+            if (live && d + VE <= D) {
+                v = *(const Vec<T> *)(p + d);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) v.e[e] = live && d + e < D ? p[d + e] : (T)0;
             }
-        for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
-        s = pow2_scale(top);
+            if constexpr (SPLIT) {
+                s16x4 h1, h2;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    short a, b;
+                    split(v.e[e] * inv, a, b);
+                    h1[e] = a;
+                    h2[e] = b;
+                }
+                short *q = o + (d >> 5) * 64 + (d & 31);
+                *(s16x4 *)q = h1;
+                *(s16x4 *)(q + 32) = h2;
+            } else {
+                *(Vec<T> *)(o + d) = v;
+            }
+        }
     }
-    if (lane == 0 && m < M) xscale[m] = s;
-    const float inv = 1.f / s;
-    for (int d = lane; d < Dp; d += 64) {
-        const bool in = live && d < D;
-        if (elem == TSC_ELEM_F32) store_value(o, d, in ? ((const float *)x.data)[at + d] * inv : 0.f, elem);
-        else o[d] = in ? ((const short *)x.data)[at + d] : (short)0;
-    }
+    if (!gtop) return;
+    __shared__ float all[4];
+    if (lane == 0) all[wave] = most;
+    __syncthreads();
+    if (threadIdx.x) return;
+    most = fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3]));
+    if (__float_as_uint(most) > __atomic_load_n(gtop, __ATOMIC_RELAXED)) atomicMax(gtop, __float_as_uint(most));
 }
 
-// rowf[m] = g_m s_m S (0 without a loss, NaN with a target outside the vocabulary), post[0] = 1 / S.  S = 1 for bf16, whose
-// range is fp32's; for the fp16 planes the power of two that keeps |G'| = |rowf (p - [v = t])| below 2^15.
-__global__ __launch_bounds__(1024) void row_factor_kernel(const float *g, const float *xscale, const long long *targets, long long ignore,
-                                                          int V, int M, int f16, float *rowf, float *post) {
-    __shared__ float s[17];
-    float top = 0.f;
-    if (f16)
-        for (int m = threadIdx.x; m < M; m += 1024)
-            if (targets[m] != ignore) {
-                const float v = fabsf(g[m] * xscale[m]);
-                top = v < __builtin_inff() ? fmaxf(top, v) : top;
-            }
-    for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-        const float q = f16 ? pow2_scale(top) : 1.f;
-        s[16] = 1.f / q;
-        post[0] = q;
-    }
-    __syncthreads();
-    for (int m = threadIdx.x; m < M; m += 1024) {
-        const long long t = targets[m];
-        rowf[m] = t == ignore ? 0.f : t < 0 || t >= V ? __builtin_nanf("") : g[m] * xscale[m] * s[16];
-    }
-}
+// G' = G s_m S in 16 bits: S is 1 for bf16, whose range is fp32's, and for the fp16 planes the power of two that keeps |G'| =
+// |g_m| s_m S |p - [v = t]| below 2^15.  This is 1 / S.
+__device__ __forceinline__ float g_unit(const unsigned *gtop) { return gtop ? pow2_scale(__uint_as_float(*gtop)) : 1.f; }
 
 // ------------------------------------------------------------------------------------------------ products
 // Tiles of a launch: workgroups b and b + 8 share an XCD, so each XCD gets a run of neighbouring tiles, and within a run
@@ -200,7 +234,8 @@ struct LogitArgs {
     float2 *part;        // [ns][M]: reference, sum of 2^(l log2 e - reference)
     float *hit;          // [M]
     // backward
-    const float *lse, *rowf;
+    const float *lse, *g;    // of the rows: kept, and d(loss)
+    const unsigned *gtop;    // g_unit
     short *G;            // [Mp][PLANES * ldg]
     long long ldg;
     int Mp;
@@ -331,14 +366,16 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
     const int i0 = bi * C::BI;
     const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave / C::VJ, wr = wi * (C::WI * 32), wj = (wave % C::VJ) * (C::WJ * 32);
+    const float unit = 1.f / g_unit(a.gtop);
     for (int i = threadIdx.x; i < C::BI; i += C::NT) {
         const int m = i0 + i, mc = m < a.M ? m : a.M - 1;
         const long long t = a.targets[mc];
         const bool live = m < a.M && t != a.ignore;
         // rows without a loss: every exponential is 2^-inf = 0
         r_lse[i] = live ? a.lse[mc] * LOG2E : __builtin_inff();
-        r_f[i] = live ? a.rowf[mc] : 0.f;
-        r_t[i] = live && t >= 0 && t < a.V ? (int)t - a.v0 : -1;
+        const bool known = t >= 0 && t < a.V;
+        r_f[i] = !live ? 0.f : known ? a.g[mc] * (SPLIT ? a.xscale[mc] : 1.f) * unit : __builtin_nanf("");
+        r_t[i] = live && known ? (int)t - a.v0 : -1;
         if (SPLIT) {
             r_sc[i] = a.xscale[mc] * a.wscale[0] * LOG2E;
             r_inv[i] = 1.f / a.xscale[mc];
@@ -471,10 +508,10 @@ struct SumArgs {  // C[z][i][j] = (or +=) the z-th part of the k-steps
     int nk, per, ti, tj, I, J, add;
     float *out;
 };
-struct OutArgs {  // C[i][j] * post, in the elements' type
+struct OutArgs {  // C[i][j] * g_unit, in the elements' type
     Operand A, B;
     int nk, ti, tj, I, J;
-    const float *post;
+    const unsigned *gtop;
     void *out;
     long long ld;
     int elem;
@@ -515,7 +552,7 @@ template <class C, bool F16, int PLANES, int SCALED> __global__ __launch_bounds_
     tile_of(blockIdx.x, a.ti, a.tj, bi, bj);
     const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5, wave = threadIdx.x >> 6;
     const int wi0 = bi * C::BI + (wave / C::VJ) * (C::WI * 32), wj0 = bj * C::BJ + (wave % C::VJ) * (C::WJ * 32);
-    const float post = a.post[0];
+    const float post = g_unit(a.gtop);
     auto begin = [&](int, f32x16 (&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
 #pragma unroll
         for (int p = 0; p < C::WI; ++p)
@@ -535,34 +572,70 @@ template <class C, bool F16, int PLANES, int SCALED> __global__ __launch_bounds_
     };
     G::run(a.A, a.B, 1, [&](int) { return TileAt{bi * C::BI, bj * C::BJ}; }, 0, a.nk, lds, begin, done);
 }
-// C = sum over z of the parts, for a dW whose k-steps were split
-__global__ __launch_bounds__(256) void join_kernel(const float *part, int n, int I, int J, const float *post, void *out, long long ld, int elem) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long long)I * J) return;
-    float v = 0.f;
-    for (int z = 0; z < n; ++z) v += part[(long long)z * I * J + i];
-    write_elem(out, elem, i / J * ld + i % J, v * post[0]);
+// C[i][j] = sum over z of part[z][i][j] times g_unit, 4 elements a lane: a dW whose k-steps were split
+__global__ __launch_bounds__(256) void join_kernel(const float *part, int n, int I, int J, const unsigned *gtop, void *out, long long ld, int elem) {
+    const int i = blockIdx.x, j = (blockIdx.y * 256 + threadIdx.x) * 4;
+    const float unit = g_unit(gtop);
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (j + 4 <= J) {
+        for (int z = 0; z < n; ++z) {
+            const Vec<float> u = *(const Vec<float> *)(part + ((long long)z * I + i) * J + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += u.e[e];
+        }
+    } else {
+        for (int e = 0; j + e < J; ++e)
+            for (int z = 0; z < n; ++z) v[e] += part[((long long)z * I + i) * J + j + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (j + e < J) write_elem(out, elem, i * ld + j + e, v[e] * unit);
 }
-// dx[m][d] = sum over z, with the scales undone
+// dx[m][d] = sum over z, with the scales undone: 256 elements of a row a workgroup, its waves share the parts
 __global__ __launch_bounds__(256) void dx_kernel(const float *part, int n, int M, int D, const float *wscale, const float *xscale,
-                                                 const float *post, const long long *targets, long long ignore, int elem, void *dx) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long long)M * D) return;
-    const int m = (int)(i / D);
-    float v = 0.f;
-    for (int z = 0; z < n; ++z) v += part[(long long)z * M * D + i];
-    v *= post[0];
-    if (wscale) v = v * wscale[0] / xscale[m];
-    write_elem(dx, elem, i, targets[m] == ignore ? 0.f : v);
+                                                 const unsigned *gtop, const long long *targets, long long ignore, int elem, void *dx) {
+    __shared__ float red[3][256];
+    const int m = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = blockIdx.y * 256 + lane * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    const float *p = part + (long long)m * D + d;
+    if (d + 4 <= D) {
+#pragma unroll 4
+        for (int z = wave; z < n; z += 4) {
+            const Vec<float> u = *(const Vec<float> *)(p + (long long)z * M * D);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += u.e[e];
+        }
+    } else {
+        for (int e = 0; d + e < D; ++e)
+            for (int z = wave; z < n; z += 4) v[e] += p[(long long)z * M * D + e];
+    }
+    if (wave)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[wave - 1][e * 64 + lane] = v[e];
+    __syncthreads();
+    if (wave) return;
+    const bool live = targets[m] != ignore;
+    const float unit = g_unit(gtop), ws = wscale ? wscale[0] : 1.f, xs = wscale ? 1.f / xscale[m] : 1.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float all = (v[e] + red[0][e * 64 + lane]) + (red[1][e * 64 + lane] + red[2][e * 64 + lane]);
+        if (d + e < D) write_elem(dx, elem, (long long)m * D + d + e, live ? all * unit * ws * xs : 0.f);
+    }
 }
-
-__global__ __launch_bounds__(256) void dbias_kernel(const float *part, int n, long long ld, int J, const float *post, int elem, void *out,
-                                                    long long at) {
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    if (j >= J) return;
+// db[at + j] = sum over the parts, 64 columns x 16 parts a workgroup
+__global__ __launch_bounds__(1024) void dbias_kernel(const float *part, int n, long long ld, int J, const unsigned *gtop, int elem, void *out,
+                                                     long long at) {
+    __shared__ float red[16][64];
+    const int c = threadIdx.x & 63, p = threadIdx.x >> 6, j = blockIdx.x * 64 + c;
     float v = 0.f;
-    for (int i = 0; i < n; ++i) v += part[i * ld + j];
-    write_elem(out, elem, at + j, v * post[0]);
+    if (j < J)
+        for (int i = p; i < n; i += 16) v += part[i * ld + j];
+    red[p][c] = v;
+    __syncthreads();
+    if (p || j >= J) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) v += red[i][c];
+    write_elem(out, elem, at + j, v * g_unit(gtop));
 }
 __global__ void zero_elem_kernel(void *p, int elem, long long n) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -572,7 +645,8 @@ __global__ void zero_elem_kernel(void *p, int elem, long long n) {
 inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 inline long long up(long long a, long long b) { return (a + b - 1) / b * b; }
 
-constexpr long long PIECE_BYTES = 3ll << 29;  // G of one piece of the vocabulary
+constexpr long long PIECE_BYTES = 1ll << 31;  // G of one piece of the vocabulary
+constexpr long long MAX_LD = 1 << 22;         // a tile's 256 rows lie within 2^31 bytes
 
 }  // namespace
 
@@ -580,15 +654,17 @@ struct tsc_unembed {
     int D, V, elem, belem, planes, Dp, Vp, Vb;  // paddings: 64 for a product's k, 256 for the bias a tile reads
     long long sd, sv;                    // strides of W (elements): one of them is 1
     const void *W, *bias;                // borrowed
-    short *Wt, *Wd;                      // [V][planes * Dp] and [D][planes * Vp]
+    const short *Wt, *Wd;                // [V][planes * Dp] and [D][planes * Vp], or W itself where it can be read as it is
+    long long wt_ld, wd_ld;
+    bool own_t, own_d;
     float *bias32, *wscale;
 };
 
 // ------------------------------------------------------------------------------------------------ handle
 int tsc_unembed_destroy_(tsc_unembed *h) {
     if (!h) return TSC_OK;
-    if (h->Wt) (void)hipFree(h->Wt);
-    if (h->Wd) (void)hipFree(h->Wd);
+    if (h->own_t && h->Wt) (void)hipFree((void *)h->Wt);
+    if (h->own_d && h->Wd) (void)hipFree((void *)h->Wd);
     if (h->bias32) (void)hipFree(h->bias32);
     if (h->wscale) (void)hipFree(h->wscale);
     delete h;
@@ -605,8 +681,13 @@ int tsc_unembed_refresh_(tsc_unembed *h, hipStream_t s) {
         hipLaunchKernelGGL(absmax_kernel, dim3((int)(rows < 1024 ? rows : 1024)), dim3(1024), 0, s, (const float *)h->W, rows, cols, ld, (unsigned *)h->wscale);
         hipLaunchKernelGGL(wscale_kernel, dim3(1), dim3(1), 0, s, h->wscale);
     }
-    hipLaunchKernelGGL(pack_w_kernel, dim3(h->Dp / 64, cdiv(h->V, 64)), dim3(256), 0, s, h->W, h->elem, h->sv, h->sd, h->V, h->D, h->Dp, h->wscale, h->Wt);
-    hipLaunchKernelGGL(pack_w_kernel, dim3(h->Vp / 64, cdiv(h->D, 64)), dim3(256), 0, s, h->W, h->elem, h->sd, h->sv, h->D, h->V, h->Vp, h->wscale, h->Wd);
+    auto pack = [&](long long sr, long long sc, int R, int C, int Cp, short *out) {
+        const dim3 grid(Cp / 64, cdiv(R, 64));
+        if (h->elem == TSC_ELEM_F32) hipLaunchKernelGGL((pack_w_kernel<float>), grid, dim3(256), 0, s, (const float *)h->W, sr, sc, R, C, Cp, h->wscale, out);
+        else hipLaunchKernelGGL((pack_w_kernel<short>), grid, dim3(256), 0, s, (const short *)h->W, sr, sc, R, C, Cp, (const float *)nullptr, out);
+    };
+    if (h->own_t) pack(h->sv, h->sd, h->V, h->D, h->Dp, (short *)h->Wt);
+    if (h->own_d) pack(h->sd, h->sv, h->D, h->V, h->Vp, (short *)h->Wd);
     TSC_HIP_CHECK(hipGetLastError());
     return TSC_OK;
 }
@@ -617,8 +698,17 @@ int tsc_unembed_create_(tsc_unembed **out, int D, int V, int elem, const void *W
     h->D = D; h->V = V; h->elem = elem; h->belem = belem; h->planes = elem == TSC_ELEM_F32 ? 2 : 1;
     h->Dp = (int)up(D, BK); h->Vp = (int)up(V, 256); h->Vb = h->Vp + 256;
     h->sd = sd; h->sv = sv; h->W = W; h->bias = bias;
-    hipError_t e = hipMalloc((void **)&h->Wt, (size_t)V * h->planes * h->Dp * 2);
-    if (e == hipSuccess) e = hipMalloc((void **)&h->Wd, (size_t)D * h->planes * h->Vp * 2);
+    // 16-bit weights in the order and at the alignment that a product reads are read where they are
+    const bool plain = elem != TSC_ELEM_F32 && (uintptr_t)W % 16 == 0;
+    h->own_t = !(plain && sd == 1 && D % BK == 0 && sv % 8 == 0 && sv <= MAX_LD);
+    h->own_d = !(plain && sv == 1 && V % BK == 0 && sd % 8 == 0 && sd <= MAX_LD);
+    h->wt_ld = h->own_t ? (long long)h->planes * h->Dp : sv;
+    h->wd_ld = h->own_d ? (long long)h->planes * h->Vp : sd;
+    hipError_t e = hipSuccess;
+    if (!h->own_t) h->Wt = (const short *)W;
+    else e = hipMalloc((void **)&h->Wt, (size_t)V * h->planes * h->Dp * 2);
+    if (!h->own_d) h->Wd = (const short *)W;
+    else if (e == hipSuccess) e = hipMalloc((void **)&h->Wd, (size_t)D * h->planes * h->Vp * 2);
     if (e == hipSuccess) e = hipMalloc((void **)&h->bias32, (size_t)h->Vb * 4);
     if (e == hipSuccess) e = hipMalloc((void **)&h->wscale, 256);
     int rc = e == hipSuccess ? tsc_unembed_refresh_(h, s) : tsc_fail(TSC_ERR_HIP, "hipMalloc of the unembedding's operands failed: %s", hipGetErrorString(e));
@@ -664,12 +754,14 @@ Streams streams(long long M, long long V) {
 }
 
 // A product of I x J with nk k-steps: tiles and the parts that its k-steps are split into, by the time of the slowest CU
-// (k-steps of a LARGE tile cost 4 units, of a MEDIUM one, two of which share a CU, 2.5) plus the traffic of the fp32 parts.
+// (64 k of a LARGE tile take 1.8 us, of a MEDIUM one, two of which share a CU, 1.1; three times that with two planes; a
+// tile begins and ends in 4) plus the traffic of the fp32 parts.
 struct Split {
     Shape s;
     int ti, tj, z, per;
+    double cost;
 };
-Split split_of(long long I, long long J, int nk, int passes, bool always_parts) {
+Split split_of(long long I, long long J, int nk, int planes, bool always_parts) {
     Split best{};
     double least = 0;
     for (int kind : {LARGE, MEDIUM}) {
@@ -677,13 +769,13 @@ Split split_of(long long I, long long J, int nk, int passes, bool always_parts) 
         r.s = shape_of(kind);
         r.ti = cdiv(I, r.s.bi);
         r.tj = cdiv(J, r.s.bj);
-        const double step = kind == LARGE ? 1.6e-6 : 1.0e-6, part = (double)I * J * 8 / 4e12;
+        const double step = (kind == LARGE ? 1.8e-6 : 1.1e-6) * (planes == 2 ? 3 : 1), start = 4e-6, part = (double)I * J * 8 / 5e12;
         for (int z = 1; z <= 64 && z <= nk; ++z) {
             r.per = cdiv(nk, z);
             r.z = cdiv(nk, r.per);
-            const double cost = (double)cdiv((long long)r.ti * r.tj * r.z, r.s.slots) * (r.per * passes + 3) * step +
+            const double cost = (double)cdiv((long long)r.ti * r.tj * r.z, r.s.slots) * (r.per * step + start) +
                                 (r.z > 1 || always_parts ? r.z * part : 0);
-            if (least == 0 || cost < least) least = cost, best = r;
+            if (least == 0 || cost < least) least = r.cost = cost, best = r;
         }
     }
     return best;
@@ -695,30 +787,31 @@ struct Plan {
     Streams st;
     int Vc, pieces;  // backward: entries of a piece
     Split dx;        // of a whole piece
-    long long xp, xscale, part, hit, rowf, post, g, db, dxp, dwp, bytes;
+    long long xp, xscale, part, hit, gtop, g, db, dxp, dwp, bytes;
 };
-Split dw_split(const tsc_unembed *h, long long Mp, int nv) {
-    return h->sv == 1 ? split_of(h->D, nv, (int)(Mp / BK), h->planes == 2 ? 3 : 1, false)
-                      : split_of(nv, h->D, (int)(Mp / BK), h->planes == 2 ? 3 : 1, false);
+// dW of nv entries of the vocabulary: as many of them as fill whole rounds of the chip in one piece, the rest (or all of them,
+// where that is cheaper) with their k-steps split.
+struct DwPlan {
+    int n[2];  // entries of each part
+    Split w[2];
+};
+DwPlan dw_plan(const tsc_unembed *h, long long Mp, int nv) {
+    const int nk = (int)(Mp / BK), dt = cdiv(h->D, 256);
+    auto of = [&](int n) { return h->sv == 1 ? split_of(h->D, n, nk, h->planes, false) : split_of(n, h->D, nk, h->planes, false); };
+    DwPlan r{{nv, 0}, {of(nv), {}}};
+    const int rounds = (int)((long long)dt * cdiv(nv, 256) / CUS), main = rounds * CUS / dt * 256;
+    if (rounds < 1 || main >= nv) return r;
+    const DwPlan two{{main, nv - main}, {of(main), of(nv - main)}};
+    return two.w[0].cost + two.w[1].cost < r.w[0].cost ? two : r;
 }
 Plan plan(const tsc_unembed *h, long long M, bool backward, bool want_x, bool want_w, bool want_b) {
     Plan p{};
     p.Mp = (int)up(M, BK);
     int nv = h->V;
     if (backward) {
-        // tiles of a piece: what fits PIECE_BYTES, and of that the number whose dW fills whole rounds of the chip best
-        const int all = cdiv(h->V, 256), dt = cdiv(h->D, 256);
-        long long fit = PIECE_BYTES / (2ll * h->planes * p.Mp * 256);
-        int vt = (int)(fit < 1 ? 1 : fit < all ? fit : all);
-        if (vt < all) {
-            double best = 0;
-            int pick = vt;
-            for (int t = vt; t > vt / 2; --t) {
-                const double full = (double)t * dt / (CUS * cdiv((long long)t * dt, CUS));
-                if (full > best + 0.01) best = full, pick = t;
-            }
-            vt = pick;
-        }
+        const int all = cdiv(h->V, 256);
+        const long long fit = PIECE_BYTES / (2ll * h->planes * p.Mp * 256);
+        const int vt = (int)(fit < 1 ? 1 : fit < all ? fit : all);
         p.Vc = vt * 256;
         p.pieces = cdiv(h->V, p.Vc);
         if (p.Vc < nv) nv = p.Vc;
@@ -732,19 +825,19 @@ Plan plan(const tsc_unembed *h, long long M, bool backward, bool want_x, bool wa
         p.part = take(8ll * p.st.ns * M);
         p.hit = take(4 * M);
     } else {
-        p.rowf = take(4 * M);
-        p.post = take(4);
+        p.gtop = take(4);
         p.g = take(2ll * h->planes * p.Mp * p.Vc);
         if (want_b) p.db = take(4ll * 2 * p.st.nm * p.Vc);
         if (want_x) {
-            p.dx = split_of(M, h->D, cdiv(nv, BK), h->planes == 2 ? 3 : 1, true);
+            p.dx = split_of(M, h->D, cdiv(nv, BK), h->planes, true);
             p.dxp = take(4ll * p.dx.z * M * h->D);
         }
-        if (want_w) {  // a piece's dW and the last, shorter one's may be split differently
+        if (want_w) {  // the parts of a piece's dW and of the last, shorter one's
             long long most = 0;
             for (int n : {nv, h->V - (p.pieces - 1) * p.Vc}) {
-                const Split w = dw_split(h, p.Mp, n);
-                if (w.z > 1 && (long long)w.z * n > most) most = (long long)w.z * n;
+                const DwPlan w = dw_plan(h, p.Mp, n);
+                for (int i = 0; i < 2; ++i)
+                    if (w.n[i] && w.w[i].z > 1 && (long long)w.w[i].z * w.n[i] > most) most = (long long)w.w[i].z * w.n[i];
             }
             p.dwp = take(4ll * most * h->D);
         }
@@ -774,7 +867,7 @@ template <bool GRAD> int logits(const tsc_unembed *h, const Streams &st, const L
 }
 LogitArgs logit_args(const tsc_unembed *h, const Plan &p, char *ws, int M, const long long *targets, long long ignore) {
     LogitArgs a{};
-    a.W = {h->Wt, (long long)h->planes * h->Dp, h->V};
+    a.W = {h->Wt, h->wt_ld, h->V};
     a.x = {(const short *)(ws + p.xp), (long long)h->planes * h->Dp, M};
     a.nk = h->Dp / BK;
     a.nm = p.st.nm; a.ns = p.st.ns; a.nv = p.st.nv; a.M = M; a.V = h->V;
@@ -827,6 +920,20 @@ int launch_dw(const Split &w, int elem, bool by_d, OutArgs &q, hipStream_t s) {
 
 }  // namespace
 
+namespace {
+void pack_x(const tsc_unembed *h, const Plan &p, const TscRows &x, int M, const long long *targets, long long ignore, const float *g, char *ws,
+            unsigned *gtop, hipStream_t s) {
+    short *out = (short *)(ws + p.xp);
+    float *xscale = (float *)(ws + p.xscale);
+    const int n = p.Mp >= 16384 ? 4 : 1;  // (a full chip of waves first)
+    const dim3 grid(cdiv(p.Mp, 4 * n));
+    if (h->elem == TSC_ELEM_F32)
+        hipLaunchKernelGGL((pack_x_kernel<float>), grid, dim3(256), 0, s, x, M, p.Mp, h->D, h->Dp, n, targets, ignore, g, out, xscale, gtop);
+    else
+        hipLaunchKernelGGL((pack_x_kernel<short>), grid, dim3(256), 0, s, x, M, p.Mp, h->D, h->Dp, n, targets, ignore, g, out, xscale, gtop);
+}
+}  // namespace
+
 size_t tsc_unembed_workspace_(const tsc_unembed *h, long long M, int backward, int want_x, int want_w, int want_b) {
     return M < 1 ? 0 : (size_t)plan(h, M, backward, want_x, want_w, want_b).bytes;
 }
@@ -834,9 +941,12 @@ size_t tsc_unembed_workspace_(const tsc_unembed *h, long long M, int backward, i
 int tsc_launch_unembed_loss(const tsc_unembed *h, const TscRows &x, int M, const long long *targets, long long ignore, float *loss,
                             float *lse, char *ws, hipStream_t s) {
     const Plan p = plan(h, M, false, false, false, false);
-    hipLaunchKernelGGL(pack_x_kernel, dim3(cdiv(p.Mp, 4)), dim3(256), 0, s, x, h->elem, M, p.Mp, h->D, h->Dp, (const long long *)nullptr, ignore,
-                       (short *)(ws + p.xp), (float *)(ws + p.xscale));
     LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
+    const bool one_stride = x.inner_stride * x.inner == x.outer_stride;
+    if (h->elem != TSC_ELEM_F32 && one_stride && h->D % BK == 0 && x.inner_stride % 8 == 0 && x.inner_stride <= MAX_LD && (uintptr_t)x.data % 16 == 0)
+        a.x = {(const short *)x.data, x.inner_stride, M};  // rows that a product can read where they are
+    else
+        pack_x(h, p, x, M, nullptr, ignore, nullptr, ws, nullptr, s);
     a.part = (float2 *)(ws + p.part);
     a.hit = (float *)(ws + p.hit);
     const int rc = logits<false>(h, p.st, a, s);
@@ -857,11 +967,12 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
     }
     const Plan p = plan(h, M, true, dx != nullptr, dW != nullptr, db != nullptr);
     short *xp = (short *)(ws + p.xp), *G = (short *)(ws + p.g);
-    float *xscale = (float *)(ws + p.xscale), *rowf = (float *)(ws + p.rowf), *post = (float *)(ws + p.post), *dxp = (float *)(ws + p.dxp);
-    hipLaunchKernelGGL(pack_x_kernel, dim3(cdiv(p.Mp, 4)), dim3(256), 0, s, x, h->elem, M, p.Mp, h->D, h->Dp, targets, ignore, xp, xscale);
-    hipLaunchKernelGGL(row_factor_kernel, dim3(1), dim3(1024), 0, s, g, xscale, targets, ignore, h->V, M, f16, rowf, post);
+    float *dxp = (float *)(ws + p.dxp);
+    unsigned *gtop = f16 ? (unsigned *)(ws + p.gtop) : nullptr;
+    if (gtop) hipLaunchKernelGGL(fill_kernel, dim3(1), dim3(256), 0, s, (float *)gtop, 0.f, 1ll);
+    pack_x(h, p, x, M, targets, ignore, g, ws, gtop, s);
     LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
-    a.lse = lse; a.rowf = rowf; a.G = G; a.ldg = p.Vc; a.Mp = p.Mp;
+    a.lse = lse; a.g = g; a.gtop = gtop; a.G = G; a.ldg = p.Vc; a.Mp = p.Mp;
     a.dbias = db ? (float *)(ws + p.db) : nullptr;
     const long long xld = (long long)h->planes * h->Dp;
     const int db_parts = p.st.nm * (p.st.s.kind == FEW ? 1 : 2);  // waves of a tile's rows
@@ -872,11 +983,11 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
         a.ns = p.st.ns < a.nv ? p.st.ns : a.nv;
         int rc = logits<true>(h, p.st, a, s);
         if (rc) return rc;
-        if (db) hipLaunchKernelGGL(dbias_kernel, dim3(cdiv(nv, 256)), dim3(256), 0, s, a.dbias, db_parts, a.ldg, nv, post, h->belem, db, (long long)v0);
+        if (db) hipLaunchKernelGGL(dbias_kernel, dim3(cdiv(nv, 64)), dim3(1024), 0, s, a.dbias, db_parts, a.ldg, nv, gtop, h->belem, db, (long long)v0);
         if (dx) {
             SumArgs q{};
             q.A = {G, (long long)h->planes * p.Vc, M};
-            q.B = {h->Wd + (long long)h->planes * v0, (long long)h->planes * h->Vp, h->D};
+            q.B = {h->Wd + (long long)h->planes * v0, h->wd_ld, h->D};
             q.nk = cdiv(nv, BK); q.I = M; q.J = h->D; q.add = c > 0; q.out = dxp;
             Split w = p.dx;
             if (c > 0) w.per = cdiv(q.nk, w.z);  // the same parts, shorter
@@ -884,32 +995,34 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
             if (rc) return rc;
         }
         if (dW) {
-            const Operand X = {xp, xld, h->D}, Gk = {G, (long long)h->planes * p.Vc, nv};
             const bool by_d = h->sv == 1;  // dW is dense in W's order: [D][V] or [V][D]
-            const Split w = dw_split(h, p.Mp, nv);
-            const int I = by_d ? h->D : nv, J = by_d ? nv : h->D;
-            const long long first = by_d ? v0 : (long long)v0 * h->D, ld = by_d ? h->V : h->D;
-            void *out = (char *)dW + first * (h->elem == TSC_ELEM_F32 ? 4 : 2);
-            if (w.z == 1) {
-                OutArgs q{};
-                q.A = by_d ? X : Gk;
-                q.B = by_d ? Gk : X;
-                q.nk = p.Mp / BK; q.I = I; q.J = J; q.post = post; q.elem = h->elem; q.ld = ld; q.out = out;
-                rc = launch_dw(w, h->elem, by_d, q, s);
-            } else {
-                SumArgs q{};
-                q.A = by_d ? X : Gk;
-                q.B = by_d ? Gk : X;
-                q.nk = p.Mp / BK; q.I = I; q.J = J; q.out = (float *)(ws + p.dwp);
-                rc = launch_dw_parts(w, h->elem, by_d, q, s);
-                if (!rc) hipLaunchKernelGGL(join_kernel, dim3(cdiv((long long)I * J, 256)), dim3(256), 0, s, q.out, w.z, I, J, post, out, ld, h->elem);
+            const DwPlan parts = dw_plan(h, p.Mp, nv);
+            for (int i = 0, at = 0; i < 2 && parts.n[i]; at += parts.n[i++]) {
+                const Split &w = parts.w[i];
+                const Operand X = {xp, xld, h->D}, Gk = {G + (long long)h->planes * at, (long long)h->planes * p.Vc, parts.n[i]};
+                const int I = by_d ? h->D : parts.n[i], J = by_d ? parts.n[i] : h->D;
+                const long long first = by_d ? v0 + at : (long long)(v0 + at) * h->D, ld = by_d ? h->V : h->D;
+                void *out = (char *)dW + first * (h->elem == TSC_ELEM_F32 ? 4 : 2);
+                if (w.z == 1) {
+                    OutArgs q{};
+                    q.A = by_d ? X : Gk;
+                    q.B = by_d ? Gk : X;
+                    q.nk = p.Mp / BK; q.I = I; q.J = J; q.gtop = gtop; q.elem = h->elem; q.ld = ld; q.out = out;
+                    rc = launch_dw(w, h->elem, by_d, q, s);
+                } else {
+                    SumArgs q{};
+                    q.A = by_d ? X : Gk;
+                    q.B = by_d ? Gk : X;
+                    q.nk = p.Mp / BK; q.I = I; q.J = J; q.out = (float *)(ws + p.dwp);
+                    rc = launch_dw_parts(w, h->elem, by_d, q, s);
+                    if (!rc) hipLaunchKernelGGL(join_kernel, dim3(I, cdiv(J, 1024)), dim3(256), 0, s, q.out, w.z, I, J, gtop, out, ld, h->elem);
+                }
+                if (rc) return rc;
             }
-            if (rc) return rc;
         }
         TSC_HIP_CHECK(hipGetLastError());
     }
-    if (dx) hipLaunchKernelGGL(dx_kernel, dim3(cdiv((long long)M * h->D, 256)), dim3(256), 0, s, dxp, p.dx.z, M, h->D,
-                               a.wscale, a.xscale, post, targets, ignore, h->elem, dx);
+    if (dx) hipLaunchKernelGGL(dx_kernel, dim3(M, cdiv(h->D, 256)), dim3(256), 0, s, dxp, p.dx.z, M, h->D, a.wscale, a.xscale, gtop, targets, ignore, h->elem, dx);
     TSC_HIP_CHECK(hipGetLastError());
     return TSC_OK;
 }
