@@ -47,7 +47,8 @@ def reference_backward(dy, x, mean, scale, w, eps_u=U):
     err = (6 * U * dn.abs() + (K + 6) * U * dn.abs().mean(-1, keepdim=True)
            + xh.abs() * (K + 12) * U * (dn * xh).abs().mean(-1, keepdim=True)) / scale
     rows = x.numel() // D
-    # a thread's own rows one after the other, at most 32 groups of a workgroup, 512 / 32 and 32 partial sums
+    # a thread's own rows one after the other (256 workgroups; at the sizes with more than 37 rows here each has two or more
+    # groups of threads), at most 128 groups of a workgroup by halves, 256 / 32 and 32 partial sums
     n = (rows + 511) // 512 + 100
     flat = dy.reshape(-1, D), (dy * xh).reshape(-1, D)
     dw, db = flat[1].sum(0), flat[0].sum(0)
