@@ -896,11 +896,27 @@ def _elem(t: torch.Tensor, name: str) -> int:
     return _ELEM[t.dtype]
 
 
+def _launch(device: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of ``device``, which is made the current device where it is not (the two
+    lookups of a call whose device is current already cost 1 us, the guard and ``current_stream()`` 6)."""
+    i = device.index
+    if torch._C._cuda_getDevice() == i:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc != 0:
+        _check(rc)
+
+
 def _rows(t: torch.Tensor, name: str) -> _RowsStruct:
     """``tsc_rows_t`` of a ``[..., D]`` tensor: its last axis is dense, the leading ones step with at most two strides
     (``x[:, :-1]`` of a dense ``[B, T, D]``, a slice of one position, an expanded gradient)."""
     if t.dim() < 1:
         raise TscError(f"{name} must have a last axis")
+    if t.is_contiguous():
+        d = t.shape[-1]
+        return _RowsStruct(t.data_ptr(), 1, d, d)
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise TscError(f"{name}: the elements of a row must be contiguous (stride {t.stride(-1)})")
     levels = []  # (size, stride), outermost first
@@ -950,6 +966,10 @@ def _ptr(t: Optional[torch.Tensor]):
     return t.data_ptr() if t is not None else None
 
 
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``tsc_layer_norm`` over the last axis of ``x`` (float32, bfloat16 or float16; leading axes with at most two strides):
@@ -960,12 +980,11 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         raise TscError("layer norm of rows without elements")
     pe = _norm_params(x, weight, bias)
     _same_device(x.device, weight=weight, bias=bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     scale = torch.empty_like(mean)
-    with torch.cuda.device(x.device):
-        _check(lib().tsc_layer_norm(elem, ctypes.byref(rows), mean.numel(), x.shape[-1], _ptr(weight), _ptr(bias), pe, float(eps),
-                                    y.data_ptr(), mean.data_ptr(), scale.data_ptr(), _stream()))
+    _launch(x.device, lib().tsc_layer_norm, elem, ctypes.byref(rows), mean.numel(), x.shape[-1], _ptr(weight), _ptr(bias), pe,
+            float(eps), y.data_ptr(), mean.data_ptr(), scale.data_ptr())
     return y, mean, scale
 
 
@@ -985,14 +1004,13 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, s
             raise TscError(f"{name} must be {tuple(x.shape[:-1])} (got {tuple(t.shape)})")
     _same_device(x.device, dy=dy, mean=mean, scale=scale, weight=weight, bias=bias)
     n, d = mean.numel(), x.shape[-1]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _dense_like(x)
     dw = torch.empty_like(weight) if weight is not None else None
     db = torch.empty_like(bias) if bias is not None else None
     nws = lib().tsc_layer_norm_workspace_bytes(n, d) if dw is not None or db is not None else 0
     ws = torch.empty(nws // 4, dtype=torch.float32, device=x.device) if nws else None
-    with torch.cuda.device(x.device):
-        _check(lib().tsc_layer_norm_backward(elem, ctypes.byref(dr), ctypes.byref(xr), mean.data_ptr(), scale.data_ptr(), n, d,
-                                             _ptr(weight), pe, dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), nws, _stream()))
+    _launch(x.device, lib().tsc_layer_norm_backward, elem, ctypes.byref(dr), ctypes.byref(xr), mean.data_ptr(), scale.data_ptr(),
+            n, d, _ptr(weight), pe, dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), nws)
     return dx, dw, db
 
 
@@ -1078,10 +1096,9 @@ class UnembedHead:
         self.refresh_if_modified()
         loss = torch.empty(targets.shape, dtype=torch.float32, device=self.device)
         lse = torch.empty_like(loss)
-        with torch.cuda.device(self.device):
-            ws, n = self._workspace(m, 0, 0, 0, 0)
-            _check(lib().tsc_unembed_loss(self._handle, ctypes.byref(rows), m, targets.data_ptr(), int(ignore_index),
-                                          loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), n, _stream()))
+        ws, n = self._workspace(m, 0, 0, 0, 0)
+        _launch(self.device, lib().tsc_unembed_loss, self._handle, ctypes.byref(rows), m, targets.data_ptr(), int(ignore_index),
+                loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), n)
         return loss, lse
 
     def loss_backward(self, dloss: torch.Tensor, x: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
@@ -1095,15 +1112,13 @@ class UnembedHead:
                 raise TscError(f"{name} must be {tuple(targets.shape)} (got {tuple(t.shape)})")
             _same_device(self.device, **{name: t})
         self.refresh_if_modified()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=self.device) if want_x else None
+        dx = _dense_like(x) if want_x else None
         dW = None
         if want_weight:
             dW = torch.empty((self.d_model, self.d_vocab) if self._by_d else (self.d_vocab, self.d_model), dtype=x.dtype,
                              device=self.device)
         db = torch.empty_like(self.b_U) if want_bias and self.b_U is not None else None
-        with torch.cuda.device(self.device):
-            ws, n = self._workspace(m, 1, int(dx is not None), int(dW is not None), int(db is not None))
-            _check(lib().tsc_unembed_loss_backward(self._handle, dloss.data_ptr(), ctypes.byref(rows), m, targets.data_ptr(),
-                                                   int(ignore_index), lse.data_ptr(), _ptr(dx), _ptr(dW), _ptr(db), ws.data_ptr(),
-                                                   n, _stream()))
+        ws, n = self._workspace(m, 1, int(dx is not None), int(dW is not None), int(db is not None))
+        _launch(self.device, lib().tsc_unembed_loss_backward, self._handle, dloss.data_ptr(), ctypes.byref(rows), m,
+                targets.data_ptr(), int(ignore_index), lse.data_ptr(), _ptr(dx), _ptr(dW), _ptr(db), ws.data_ptr(), n)
         return dx, dW if dW is None or self._by_d else dW.t(), db
