@@ -1,0 +1,144 @@
+"""The end of a language model as differentiable operators: layer norm, and the cross entropy behind the unembedding without
+the ``[rows, d_vocab]`` logits (``tsc_layer_norm*``, ``tsc_unembed_*`` through ``tsc_hip``).
+
+    head = tsc_hip.UnembedHead(W_U, b_U)
+    loss = unembed_loss(layer_norm(resid, w, b), targets, head)      # mean over the rows whose target counts
+    loss.backward()                                                  # resid, w, b, W_U and b_U
+
+Gradients are first-order (a second derivative raises) and the same call gives the same bits.  Both may be captured into a
+HIP graph, the backward pass too.  A captured pass whose weights learn lays them out again on every replay; a capture while
+an eager pass over the same leaves is alive is refused (``_mark_leaves``).
+"""
+from __future__ import annotations
+
+import weakref
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+from torch.autograd.graph import get_gradient_edge
+
+import tsc_hip
+
+_MARK = "tsc_eager_stream"
+
+
+def _mark_leaves(*tensors) -> list:
+    """A leaf has one gradient accumulator for as long as any pass over it lives, and the accumulator belongs to the stream
+    of the first.  A backward pass that is captured on another stream would wait for that stream inside the capture, which
+    ends the process: so an eager pass leaves its stream at the accumulator (gone with the pass), and a capture that finds
+    another stream's there refuses.  The caller holds what is returned until the pass itself holds the accumulators."""
+    held = []
+    for t in tensors:
+        if t is None or not t.requires_grad or not t.is_leaf or not t.is_cuda:
+            continue
+        stream = torch.cuda.current_stream(t.device).cuda_stream
+        held.append(get_gradient_edge(t).node)
+        note = held[-1].metadata
+        if not torch.cuda.is_current_stream_capturing():
+            note.setdefault(_MARK, stream)
+        elif note.get(_MARK, stream) != stream:
+            raise tsc_hip.TscError(
+                "an eager pass over the same leaf is alive (its loss or an output is still referenced) while this one is "
+                "captured into a graph on another stream: delete its outputs first, or run it on the capture's stream")
+    return held
+
+
+def _as_rows(t: torch.Tensor) -> torch.Tensor:
+    """A gradient may arrive broadcast or transposed: a copy where its rows are no ``tsc_rows_t``."""
+    try:
+        tsc_hip._rows(t, "t")
+        return t
+    except tsc_hip.TscError:
+        return t.contiguous()
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, scale = tsc_hip.layer_norm(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, bias, mean, scale)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, mean, scale = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx, dw, db = tsc_hip.layer_norm_backward(_as_rows(dy), x, mean, scale, weight, bias if need_b else None, want_weight=need_w)
+        return dx if need_x else None, dw, db, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last axis (:func:`tsc_hip.layer_norm`: types, strides and
+    refusals), differentiable in ``x``, ``weight`` and ``bias``."""
+    held = _mark_leaves(x, weight, bias) if torch.is_grad_enabled() else None  # noqa: F841
+    return _LayerNorm.apply(x, weight, bias, eps)
+
+
+class _UnembedLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, W_U, b_U, targets, head, ignore_index):
+        loss, lse = head.loss(x, targets, ignore_index)
+        # (the weights are saved for their version: a change in place between the two passes is an error, not a wrong gradient)
+        ctx.save_for_backward(x, W_U, b_U, targets, lse)
+        ctx.head, ctx.ignore_index = head, ignore_index
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        x, _, _, targets, lse = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx, dw, db = ctx.head.loss_backward(dloss.contiguous(), x, targets, lse, ctx.ignore_index, want_x=need_x,
+                                            want_weight=need_w, want_bias=need_b)
+        return dx, dw, db, None, None, None
+
+
+def _total(v: torch.Tensor) -> torch.Tensor:
+    """Sum of all elements in rows of 1024: no reduction over several blocks, which clears its counters with a memset node
+    in a captured graph."""
+    v = v.reshape(-1)
+    while v.numel() > 1024:
+        n = -(-v.numel() // 1024)
+        v = torch.nn.functional.pad(v, (0, n * 1024 - v.numel())).view(n, 1024).sum(1)
+    return v.sum()
+
+
+def unembed_loss(x: torch.Tensor, targets: torch.Tensor, head: "tsc_hip.UnembedHead", ignore_index: int = -100,
+                 reduction: str = "mean") -> torch.Tensor:
+    """Cross entropy of ``x @ head.W_U + head.b_U`` with ``targets`` (:meth:`tsc_hip.UnembedHead.loss`), differentiable in
+    ``x``, ``head.W_U`` and ``head.b_U``.  ``reduction``: ``"none"`` -- float32 of shape ``x.shape[:-1]``; ``"sum"``;
+    ``"mean"`` -- over the rows whose target is not ``ignore_index`` (NaN where there are none)."""
+    if reduction not in ("none", "sum", "mean"):
+        raise tsc_hip.TscError(f"reduction must be 'none', 'sum' or 'mean' (got {reduction!r})")
+    if torch.is_grad_enabled():
+        held = _mark_leaves(x, head.W_U, head.b_U)  # noqa: F841
+        if torch.cuda.is_current_stream_capturing() and any(p is not None and p.requires_grad for p in (head.W_U, head.b_U)):
+            head.refresh()  # part of the graph: a replay finds the weights that the step before it left
+    rows = _UnembedLoss.apply(x, head.W_U, head.b_U, targets, head, ignore_index)
+    if reduction == "none":
+        return rows
+    total = _total(rows)
+    return total if reduction == "sum" else total / _total((targets != ignore_index).double()).float()
+
+
+_heads: "weakref.WeakKeyDictionary" = weakref.WeakKeyDictionary()
+
+
+def model_head(model) -> "tsc_hip.UnembedHead":
+    """The :class:`tsc_hip.UnembedHead` of ``model.W_U`` and ``model.b_U``, laid out once for as long as the model keeps these
+    tensors (a change in place lays it out again)."""
+    key = tuple((t.data_ptr(), t.dtype, t.shape, t.stride()) for t in (model.W_U, model.b_U))
+    entry = _heads.get(model)
+    if entry is None or entry[0] != key:
+        entry = _heads[model] = (key, tsc_hip.UnembedHead(model.W_U.detach(), model.b_U.detach()))
+    return entry[1]
+
+
+def next_token_loss(normalized: torch.Tensor, tokens: torch.Tensor, head: "tsc_hip.UnembedHead",
+                    per_token: bool = False) -> torch.Tensor:
+    """A model's training loss from its final normalised residual ``[batch, n, d_model]``: the cross entropy of token
+    ``t + 1`` at position ``t``, as mean or ``[batch, n - 1]`` (padding counts like any token)."""
+    return unembed_loss(normalized[:, :-1], tokens[:, 1:].contiguous(), head, reduction="none" if per_token else "mean")

@@ -6,8 +6,8 @@ is_sparse_connection, use_ghost_grads, hook_point, hook_point_layer``), same par
 shapes (:70-99), ``encode(x)`` (:194-213) and ``forward(x)`` returning the 6-tuple ``(sae_out,
 feature_acts, loss, mse_loss, l1_loss, mse_loss_ghost_resid)`` (:108-192).  ``encode`` runs the
 hand-written fp32-MFMA kernel through the C-ABI; the decoder half of ``forward`` is a plain library
-GEMM.  Training helpers (resampling, ghost grads, ``get_test_loss``, ``save_model``) are out of scope
- and absent.
+GEMM.  ``get_test_loss`` runs a model with the dictionary in the place of what it replaces.  Training helpers
+(resampling, ghost grads, ``save_model``) are out of scope and absent.
 """
 from __future__ import annotations
 
@@ -94,6 +94,29 @@ class SparseTranscoder(HipDictionaryMixin, nn.Module):
         l1_loss = self.l1_coefficient * sparsity
         loss = mse_loss + l1_loss + mse_loss_ghost_resid
         return sae_out, feature_acts, loss, mse_loss, l1_loss, mse_loss_ghost_resid
+
+    @torch.no_grad()
+    def get_test_loss(self, batch_tokens, model):
+        """Mean next-token loss of ``model`` on ``batch_tokens [batch, n]`` with the dictionary's output in the place of what
+        it reconstructs: the layer's MLP output for a transcoder (computed from the activation at ``cfg.hook_point``), the
+        activation itself otherwise.  Compare with ``model(batch_tokens, return_type="loss")``."""
+        if getattr(self.cfg, "hook_point_head_index", None) is not None:
+            raise NotImplementedError("a dictionary of one attention head is outside the accelerated analysis path")
+
+        def reconstruct(act):
+            return self.forward(act.reshape(-1, act.shape[-1]))[0].to(act.dtype).reshape(*act.shape[:-1], self.d_out)
+
+        if not self.cfg.is_transcoder:
+            hooks = [(self.cfg.hook_point, lambda act, hook: reconstruct(act))]
+        else:
+            seen = {}
+
+            def read(act, hook):
+                seen["in"] = act
+
+            hooks = [(self.cfg.hook_point, read),
+                     (f"blocks.{self.cfg.hook_point_layer}.hook_mlp_out", lambda act, hook: reconstruct(seen["in"]))]
+        return model.run_with_hooks(batch_tokens, return_type="loss", fwd_hooks=hooks)
 
     # ------------------------------------------------------------------ loaders (local files only)
     @classmethod

@@ -13,7 +13,8 @@ W_Q/W_K/W_V/OV``, ``blocks[l].mlp``, ``tokenizer.decode``, ``to_str_tokens`` -- 
 ``normalized = (x - mean) / scale``.
 
 It is upstream of the accelerated path (the model forward stays
-PyTorch); nothing in here is a HIP kernel.
+PyTorch); the one HIP operator in here is the loss behind the unembedding of a model on a GPU
+(``return_type="loss"``), which the dictionaries' ``get_test_loss`` ends in.
 """
 from __future__ import annotations
 
@@ -198,6 +199,7 @@ class SyntheticHookedTransformer(nn.Module):
         return_type: Optional[str] = "logits",
         names_filter: Union[None, str, Sequence[str], Callable[[str], bool]] = None,
         stop_at_layer: Optional[int] = None,
+        loss_per_token: bool = False,
     ):
         if names_filter is None:
             keep = lambda n: True  # noqa: E731
@@ -216,12 +218,12 @@ class SyntheticHookedTransformer(nn.Module):
                 cache[name] = value
             return value
 
-        out = self._forward(tokens, put, return_type, stop_at_layer)
+        out = self._forward(tokens, put, return_type, stop_at_layer, loss_per_token)
         return out, cache
 
     @torch.no_grad()
     def run_with_hooks(self, tokens: torch.Tensor, return_type: Optional[str] = "logits", fwd_hooks=(),
-                       stop_at_layer: Optional[int] = None, **_ignored):
+                       stop_at_layer: Optional[int] = None, loss_per_token: bool = False, **_ignored):
         """TransformerLens' ``run_with_hooks`` for forward hooks: ``fwd_hooks = [(name or name-filter, fn)]``,
         ``fn(activation, hook=<object with .name>)``; a tensor returned by ``fn`` replaces the activation."""
         table = []
@@ -236,9 +238,19 @@ class SyntheticHookedTransformer(nn.Module):
                         value = res
             return value
 
-        return self._forward(tokens, put, return_type, stop_at_layer)
+        return self._forward(tokens, put, return_type, stop_at_layer, loss_per_token)
 
-    def _forward(self, tokens, put, return_type, stop_at_layer):
+    def _loss(self, final: torch.Tensor, tokens: torch.Tensor, per_token: bool) -> torch.Tensor:
+        """Next-token cross entropy: without the ``[batch, n, d_vocab]`` logits on a GPU, plainly on the CPU."""
+        if final.is_cuda:
+            from lm_head import model_head, next_token_loss
+
+            return next_token_loss(final, tokens, model_head(self), per_token)
+        logits = (final[:, :-1] @ self.W_U + self.b_U).float()
+        loss = logits.logsumexp(-1) - logits.gather(-1, tokens[:, 1:, None])[..., 0]
+        return loss if per_token else loss.mean()
+
+    def _forward(self, tokens, put, return_type, stop_at_layer, loss_per_token=False):
         cfg = self.cfg
         tokens = torch.as_tensor(tokens).to(self.device)
         if tokens.dim() == 1:
@@ -275,7 +287,13 @@ class SyntheticHookedTransformer(nn.Module):
         final = put("ln_final.hook_normalized", final)
         if return_type is None:
             return None
-        return final @ self.W_U + self.b_U
+        if return_type == "loss":
+            return self._loss(final, tokens, loss_per_token)
+        logits = final @ self.W_U + self.b_U
+        return (logits, self._loss(final, tokens, loss_per_token)) if return_type == "both" else logits
 
-    def forward(self, tokens, return_type="logits"):
-        return self.run_with_cache(tokens, return_type=return_type, names_filter=lambda n: False)[0]
+    def forward(self, tokens, return_type="logits", loss_per_token=False):
+        """Logits, the next-token loss (``return_type="loss"``; ``loss_per_token``: ``[batch, n - 1]`` instead of the mean),
+        ``"both"`` or None."""
+        return self.run_with_cache(tokens, return_type=return_type, names_filter=lambda n: False,
+                                   loss_per_token=loss_per_token)[0]

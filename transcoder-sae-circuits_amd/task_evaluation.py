@@ -14,6 +14,8 @@ from typing import Callable, List, Optional
 
 import torch
 
+import lm_head
+import tsc_hip
 from circuit_lens import BatchedCircuitLens
 from load_model_and_encoders import get_model_encoders
 
@@ -74,10 +76,47 @@ class TaskEvaluation:
             self._batched = BatchedCircuitLens(self.str_prompts, positions=pos)
         return self._batched
 
-    def contribution_decomposition(self, k: int = 10, positions="eval"):
-        """Per prompt, at ``eval_index``: every component's normalised contribution to the prompt's logit-difference
-        direction and the top-``k`` of them (``BatchedCircuitLens.direction_lens``)."""
-        return self.batched_lens(positions).direction_lens(self.logit_difference_directions(), k=k)
+    def contribution_decomposition(self, k: int = 10, positions="eval", directions: Optional[torch.Tensor] = None):
+        """Per prompt, at ``eval_index``: every component's normalised contribution to the prompt's direction (its
+        logit difference, or ``directions [n_prompts, d_model]``, e.g. ``loss_directions()``) and the top-``k`` of them
+        (``BatchedCircuitLens.direction_lens``)."""
+        if directions is None:
+            directions = self.logit_difference_directions()
+        return self.batched_lens(positions).direction_lens(directions, k=k)
+
+    # ------------------------------------------------------------------ the answer's loss (new)
+    @torch.no_grad()
+    def _answer_rows(self):
+        """Every prompt's final residual at ``eval_index`` of its own length (as ``BatchedCircuitLens``: padding sits behind
+        it), normalised, and its answer's last token."""
+        model = self.model
+        if any(p["correct"] is None for p in self.prompts):
+            raise ValueError("Prompt does not have correct token")
+        name = f"blocks.{model.cfg.n_layers - 1}.hook_resid_post"
+        cache = model.run_with_cache(self.tokens, return_type=None, names_filter=[name])[1]
+        pos = [self.eval_index % int(model.to_tokens(t).shape[1]) for t in self.str_prompts]
+        resid = cache[name][torch.arange(len(pos), device=self.tokens.device), torch.tensor(pos, device=self.tokens.device)]
+        answers = torch.cat([model.to_tokens(p["correct"])[0, -1:] for p in self.prompts]).to(resid.device)
+        return resid, tsc_hip.layer_norm(resid, eps=model.cfg.eps), answers, lm_head.model_head(model)
+
+    @torch.no_grad()
+    def answer_loss(self) -> torch.Tensor:
+        """``[n_prompts]``: the cross entropy of every prompt's correct answer (its last token) at ``eval_index``."""
+        _, (normalized, _, _), answers, head = self._answer_rows()
+        return head.loss(normalized, answers)[0]
+
+    @torch.no_grad()
+    def loss_directions(self, at: str = "normalized") -> torch.Tensor:
+        """``[n_prompts, d_model]``: the direction that lowers each prompt's ``answer_loss`` fastest.  ``at="normalized"``:
+        the negative gradient at the final normalised residual, ``W_U[:, correct] - sum_v p_v W_U[:, v]`` -- what
+        ``logit_difference_directions`` is with the model's own distribution in the counter token's place;
+        ``at="resid"``: the negative gradient at the residual before the layer norm."""
+        if at not in ("normalized", "resid"):
+            raise ValueError(f"at must be 'normalized' or 'resid' (got {at!r})")
+        resid, (normalized, mean, scale), answers, head = self._answer_rows()
+        lse = head.loss(normalized, answers)[1]
+        down = head.loss_backward(torch.full_like(lse, -1.0), normalized, answers, lse, want_weight=False, want_bias=False)[0]
+        return down if at == "normalized" else tsc_hip.layer_norm_backward(down, resid, mean, scale)[0]
 
     # ------------------------------------------------------------------ out of scope
     def _out_of_scope(self, *a, **k):

@@ -989,10 +989,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, scale: torch.Tensor,
-                        weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None):
+                        weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, want_weight: bool = True):
     """``tsc_layer_norm_backward``: ``(dx, dweight, dbias)`` from the ``mean`` and ``scale`` that :func:`layer_norm` returned.
-    ``dweight`` (``dbias``) is None where ``weight`` (``bias``) is; else it has that parameter's type.  The same call gives
-    the same bits."""
+    ``dweight`` (``dbias``) is None where ``weight`` (``bias``) is, ``dweight`` also where it is not wanted (the weight enters
+    dx); else it has that parameter's type.  The same call gives the same bits."""
     elem, xr, dr = _elem(x, "x"), _rows(x, "x"), _rows(dy, "dy")
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise TscError(f"dy must be {x.dtype} {tuple(x.shape)} like x (got {dy.dtype} {tuple(dy.shape)})")
@@ -1005,7 +1005,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, s
     _same_device(x.device, dy=dy, mean=mean, scale=scale, weight=weight, bias=bias)
     n, d = mean.numel(), x.shape[-1]
     dx = _dense_like(x)
-    dw = torch.empty_like(weight) if weight is not None else None
+    dw = torch.empty_like(weight) if weight is not None and want_weight else None
     db = torch.empty_like(bias) if bias is not None else None
     nws = lib().tsc_layer_norm_workspace_bytes(n, d) if dw is not None or db is not None else 0
     ws = torch.empty(nws // 4, dtype=torch.float32, device=x.device) if nws else None

@@ -77,6 +77,19 @@ class ZSAE(HipDictionaryMixin, nn.Module):
             l1 = l1.mean(dim=0)
         return l2 + l1, x_reconstruct, acts, l2, l1
 
+    @torch.no_grad()
+    def get_test_loss(self, batch_tokens, model, layer=None):
+        """Mean next-token loss of ``model`` on ``batch_tokens [batch, n]`` with every head's ``hook_z`` of ``layer`` (default:
+        ``cfg["layer"]``) replaced by the reconstruction."""
+        layer = self.cfg.get("layer") if layer is None else layer
+        if layer is None:
+            raise ValueError("which layer's hook_z?  cfg names none: pass layer=")
+
+        def replace(z, hook):
+            return self.forward(z.reshape(-1, self.W_enc.shape[0]))[1].to(z.dtype).reshape(z.shape)
+
+        return model.run_with_hooks(batch_tokens, return_type="loss", fwd_hooks=[(f"blocks.{layer}.attn.hook_z", replace)])
+
     @classmethod
     def load_from_files(cls, cfg_json: str, weights_pt: str, device=None):
         """Local ``<run>_cfg.json`` + ``<run>.pt`` pair (what reference :85-88 downloads)."""
