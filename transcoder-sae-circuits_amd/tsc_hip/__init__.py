@@ -896,14 +896,13 @@ def _elem(t: torch.Tensor, name: str) -> int:
     return _ELEM[t.dtype]
 
 
-def _launch(device: torch.device, fn, *args) -> None:
-    """``fn(*args, stream)`` on the current stream of ``device``, which is made the current device where it is not (the two
+def _launch(i: int, fn, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of device ``i``, which is made the current device where it is not (the two
     lookups of a call whose device is current already cost 1 us, the guard and ``current_stream()`` 6)."""
-    i = device.index
     if torch._C._cuda_getDevice() == i:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(i):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     if rc != 0:
         _check(rc)
@@ -937,14 +936,14 @@ def _rows(t: torch.Tensor, name: str) -> _RowsStruct:
     return _RowsStruct(t.data_ptr(), levels[1][0], levels[0][1], levels[1][1])
 
 
-def _same_device(device, **tensors) -> None:
+def _same_device(index: int, **tensors) -> None:
     for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise TscError(f"{name} lives on {t.device}, the other operands on {device}")
+        if t is not None and t.get_device() != index:
+            raise TscError(f"{name} lives on {t.device}, the other operands on cuda:{index}")
 
 
 def _norm_param(p: Optional[torch.Tensor], x: torch.Tensor, name: str) -> None:
-    if p is None:
+    if p is None or (p.dtype == x.dtype and p.is_cuda and p.dim() == 1 and p.shape[0] == x.shape[-1] and p.is_contiguous()):
         return
     _elem(p, name)
     if p.dtype not in (x.dtype, torch.float32):
@@ -979,11 +978,11 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if x.shape[-1] < 1:
         raise TscError("layer norm of rows without elements")
     pe = _norm_params(x, weight, bias)
-    _same_device(x.device, weight=weight, bias=bias)
+    _same_device(x.get_device(), weight=weight, bias=bias)
     y = _dense_like(x)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     scale = torch.empty_like(mean)
-    _launch(x.device, lib().tsc_layer_norm, elem, ctypes.byref(rows), mean.numel(), x.shape[-1], _ptr(weight), _ptr(bias), pe,
+    _launch(x.get_device(), lib().tsc_layer_norm, elem, ctypes.byref(rows), mean.numel(), x.shape[-1], _ptr(weight), _ptr(bias), pe,
             float(eps), y.data_ptr(), mean.data_ptr(), scale.data_ptr())
     return y, mean, scale
 
@@ -1002,14 +1001,14 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, s
     for name, t in (("mean", mean), ("scale", scale)):
         if _dev(t, torch.float32, name).shape != x.shape[:-1]:
             raise TscError(f"{name} must be {tuple(x.shape[:-1])} (got {tuple(t.shape)})")
-    _same_device(x.device, dy=dy, mean=mean, scale=scale, weight=weight, bias=bias)
+    _same_device(x.get_device(), dy=dy, mean=mean, scale=scale, weight=weight, bias=bias)
     n, d = mean.numel(), x.shape[-1]
     dx = _dense_like(x)
     dw = torch.empty_like(weight) if weight is not None and want_weight else None
     db = torch.empty_like(bias) if bias is not None else None
     nws = lib().tsc_layer_norm_workspace_bytes(n, d) if dw is not None or db is not None else 0
     ws = torch.empty(nws // 4, dtype=torch.float32, device=x.device) if nws else None
-    _launch(x.device, lib().tsc_layer_norm_backward, elem, ctypes.byref(dr), ctypes.byref(xr), mean.data_ptr(), scale.data_ptr(),
+    _launch(x.get_device(), lib().tsc_layer_norm_backward, elem, ctypes.byref(dr), ctypes.byref(xr), mean.data_ptr(), scale.data_ptr(),
             n, d, _ptr(weight), pe, dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), nws)
     return dx, dw, db
 
@@ -1040,7 +1039,7 @@ class UnembedHead:
             _elem(b_U, "b_U")
             if tuple(b_U.shape) != (self.d_vocab,) or not b_U.is_contiguous() or b_U.dtype not in (W_U.dtype, torch.float32):
                 raise TscError(f"b_U must be a contiguous [{self.d_vocab}] tensor of {W_U.dtype} or float32")
-            _same_device(W_U.device, b_U=b_U)
+            _same_device(W_U.get_device(), b_U=b_U)
         self._by_d = sv == 1
         self._keep = [W_U] if b_U is None else [W_U, b_U]
         self.W_U, self.b_U, self.device, self.dtype = W_U, b_U, W_U.device, W_U.dtype
@@ -1081,7 +1080,7 @@ class UnembedHead:
             raise TscError(f"x must be {self.dtype} [..., {self.d_model}] (got {x.dtype} {tuple(x.shape)})")
         if _dev(targets, torch.int64, "targets").shape != x.shape[:-1]:
             raise TscError(f"targets must be {tuple(x.shape[:-1])} (got {tuple(targets.shape)})")
-        _same_device(self.device, x=x, targets=targets)
+        _same_device(self.device.index, x=x, targets=targets)
         return _rows(x, "x"), targets.numel()
 
     def _workspace(self, *shape):
@@ -1097,7 +1096,7 @@ class UnembedHead:
         loss = torch.empty(targets.shape, dtype=torch.float32, device=self.device)
         lse = torch.empty_like(loss)
         ws, n = self._workspace(m, 0, 0, 0, 0)
-        _launch(self.device, lib().tsc_unembed_loss, self._handle, ctypes.byref(rows), m, targets.data_ptr(), int(ignore_index),
+        _launch(self.device.index, lib().tsc_unembed_loss, self._handle, ctypes.byref(rows), m, targets.data_ptr(), int(ignore_index),
                 loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), n)
         return loss, lse
 
@@ -1110,7 +1109,7 @@ class UnembedHead:
         for name, t in (("dloss", dloss), ("lse", lse)):
             if _dev(t, torch.float32, name).shape != targets.shape:
                 raise TscError(f"{name} must be {tuple(targets.shape)} (got {tuple(t.shape)})")
-            _same_device(self.device, **{name: t})
+            _same_device(self.device.index, **{name: t})
         self.refresh_if_modified()
         dx = _dense_like(x) if want_x else None
         dW = None
@@ -1119,6 +1118,6 @@ class UnembedHead:
                              device=self.device)
         db = torch.empty_like(self.b_U) if want_bias and self.b_U is not None else None
         ws, n = self._workspace(m, 1, int(dx is not None), int(dW is not None), int(db is not None))
-        _launch(self.device, lib().tsc_unembed_loss_backward, self._handle, dloss.data_ptr(), ctypes.byref(rows), m,
+        _launch(self.device.index, lib().tsc_unembed_loss_backward, self._handle, dloss.data_ptr(), ctypes.byref(rows), m,
                 targets.data_ptr(), int(ignore_index), lse.data_ptr(), _ptr(dx), _ptr(dW), _ptr(db), ws.data_ptr(), n)
         return dx, dW if dW is None or self._by_d else dW.t(), db
