@@ -8,8 +8,9 @@
 // HBM-bound: one read of every operand and one write of the result, ~10 operations an element.  A row is held in the
 // registers of TPR threads (NV 16-byte vectors each), so both passes over it (mean, then the squared deviations: no
 // cancellation of two large sums) cost no second read.  All statistics and sums are fp32.  Thread groups walk the rows
-// with the stride of the grid; backward they keep their part of dw and db in registers meanwhile.  The parts of a workgroup meet in LDS, those of the grid in the workspace, and a second launch adds them up in a fixed
-// order, so results do not depend on timing.
+// with the stride of the grid; backward they keep their part of dw and db in registers meanwhile.  The parts of a
+// workgroup meet in LDS, those of the grid in the workspace, and a second launch adds them up in a fixed order, so results
+// do not depend on timing.
 #include <type_traits>
 
 #include "tsc_internal.h"
@@ -198,7 +199,7 @@ struct LnArgs {
 
 // Threads a row and 16-byte vectors a thread; thread groups of a workgroup take rows of their own.  The next row is read
 // while this one is reduced.
-// Measured (fresh inputs): 65536 x 768 bf16 40 us = 5.0 TB/s, fp32 68 us = 5.9 TB/s.
+// Measured (fresh inputs): 65536 x 768 bf16 37 us = 5.4 TB/s, fp32 68 us = 5.9 TB/s; 512 x 768 fp32 3.6 us, a launch's own time.
 template <class T, int NV, int TPR, int NT> __global__ __launch_bounds__(NT) void ln_forward_kernel(const LnArgs a) {
     typedef Row<T, NV, TPR> R;
     constexpr int N = NV * R::VE, GROUPS = NT / TPR;
@@ -251,7 +252,8 @@ template <class T, int NV, int TPR, int NT> __global__ __launch_bounds__(NT) voi
 
 // The row's elements stay as they were read and are widened in each of the two passes, and the weight lies in LDS (its place
 // is needed for the sums only at the end), so that 16 waves a CU keep their rows and sums in registers.
-// Measured: 65536 x 768 fp32 125 us = 4.8 TB/s, bf16 79 us = 3.8 TB/s; 16384 x 768 fp32 27 us and 4 for the sums' last step.
+// Measured: 65536 x 768 fp32 125 us = 4.8 TB/s, bf16 80 us = 3.8 TB/s; 16384 x 768 fp32 27 us and 4 for the sums' last step;
+// 1021 x 4099 bf16 16 us.  Reading the next row ahead, as the forward pass does, changed nothing (and spills with two vectors).
 template <class T, int NV, int TPR, int NT> __global__ __launch_bounds__(NT) void ln_backward_kernel(const LnArgs a) {
     typedef RowEnd<T, NV, TPR> R;
     constexpr int N = NV * R::VE, GROUPS = NT / TPR;
@@ -339,12 +341,16 @@ template <class T, int NV, int TPR, int NT> __global__ __launch_bounds__(NT) voi
                 }
             }
         }
-        if (grp == 0)
+        // (through LDS into the order of memory: a thread's vectors lie apart, and so would its stores; 1021 x 4099 bf16 16 us
+        // against 19)
+        __syncthreads();
+        if (grp == 0) {
 #pragma unroll
-            for (int j = 0; j < NV; ++j)
-#pragma unroll
-                for (int e = 0; e < R::VE; ++e)
-                    if (R::at(t, j) + e < D) dst[(long long)blockIdx.x * D + R::at(t, j) + e] = v[j * R::VE + e];
+            for (int i = 0; i < N; i += 4)
+                *(float4 *)&part[R::at(t, i / R::VE) + i % R::VE] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < D; i += NT) dst[(long long)blockIdx.x * D + i] = part[i];
     };
     if (a.part_w) emit(dw, a.part_w);
     if (a.part_b) emit(db, a.part_b);
@@ -419,7 +425,7 @@ __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float *part_w, co
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), p = threadIdx.x >> 5;
     float s = 0.f;
     if (c < D)
-#pragma unroll 4
+#pragma unroll 8
         for (int i = p; i < n_parts; i += 32) s += part[(long long)i * D + c];
     red[p][threadIdx.x & 31] = s;
     __syncthreads();
