@@ -494,7 +494,13 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2 *part, int n, in
     const int m = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (m >= M) return;
     float2 all = make_float2(-__builtin_inff(), 0.f);
-    for (int i = lane; i < n; i += 64) all = merge(all, part[(long long)i * M + m]);
+    for (int i = lane; i < n; i += 512) {  // (the loads of eight parts under way at once)
+        float2 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = i + 64 * k < n ? part[(long long)(i + 64 * k) * M + m] : make_float2(-__builtin_inff(), 0.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) all = merge(all, v[k]);
+    }
     for (int o = 32; o > 0; o >>= 1) all = merge(all, make_float2(__shfl_xor(all.x, o), __shfl_xor(all.y, o)));
     if (lane) return;
     const float l = (all.x + __log2f(all.y)) * LN2;
