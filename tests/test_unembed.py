@@ -4,7 +4,7 @@ Tolerances.  u = 2^-24.  A product of split fp32 operands is off by at most 3 * 
 product of the second planes), plus 2^-39 of either operand's largest times the other operand; 16-bit operands multiply exactly.  Sums: Higham and Mary's
 probabilistic bound 4 sqrt(n) u of the sum of the absolute terms for n additions (a fixed order, so a run repeats itself).
 An error e of a logit is a relative error e of its exponential; G is rounded to 16 bits as an operand (bf16 2^-8, fp16 2^-11,
-fp32 2^-22 and the floors that the header names); results are rounded once to their type."""
+fp32 2^-22 and the floors that the header names; squared where a row's remainder is kept); results are rounded once to their type."""
 import ctypes
 import math
 
@@ -75,10 +75,9 @@ def reference(x, W, b, t, dloss, ignore=-100):
         top = (xd.abs().amax(-1, keepdim=True) * g.abs()).max()
         floor = 2.0 ** -50 * 2 * top / xd.abs().amax(-1, keepdim=True).clamp_min(1e-30)  # 2: the row's scale is a power of two
         rnd = 2.0 ** -22 * out_G.abs() + torch.where(g == 0, 0.0, floor)
-    elif dt == torch.float16:
-        rnd = 2.0 ** -11 * out_G.abs() + 2.0 ** -39 * g.abs().max()
-    else:
-        rnd = 2.0 ** -8 * out_G.abs()
+    else:  # up to 64 rows what the rounding took is kept, rounded itself
+        half = 2.0 ** -11 if dt == torch.float16 else 2.0 ** -8
+        rnd = half * (half if M <= 64 else 1.0) * out_G.abs() + (2.0 ** -39 * g.abs().max() if dt == torch.float16 else 0.0)
     e_op = e_raw + rnd
     passes_rel = 3 * 2.0 ** -22 if dt == torch.float32 else 0.0
     aG, aw = out_G.abs(), wd.abs()

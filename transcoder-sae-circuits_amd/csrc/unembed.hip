@@ -7,7 +7,10 @@
 // Bound by the matrix pipe: 2 M D V operations forward; backward makes the logits again (2 M D V) and adds two products of
 // the same size.  Forward: the tile of logits stays in the accumulators, only its rows' maximum and sum of exponentials leave
 // the workgroup.  Backward, in pieces of the vocabulary: G of a piece goes to the workspace in 16 bits (fp32: two fp16
-// planes), and the two products read it from there.
+// planes), and the two products read it from there.  One entry carries most of a row of G, the target's, so what is lost of
+// it in 16 bits is lost of the row's gradient: as much as the result's own rounding loses on the average of many rows, up to
+// twice that in a single one.  So up to 64 rows of 16-bit elements, whose time is W's way from memory, also keep what the
+// rounding took (rows 2 m: G_m, 2 m + 1: its remainder), and both products run over twice as many rows.
 #include <new>
 #include <type_traits>
 
@@ -17,6 +20,7 @@ using namespace unembed_gemm;
 
 namespace {
 
+constexpr int FEW_ROWS = 64;  // a tile's rows where W's way from memory is what takes the time
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -129,16 +133,16 @@ __device__ __forceinline__ long long row_at(const TscRows &r, long long row) {
 }
 
 // One wave a row, n rows one after the other: x[m] / s_m, pitch Dp, rows behind M (up to Mp) and rows without a loss zero; s_m
-// to xscale (fp32).  With gtop: it takes the largest |g_m| s_m, from which G is scaled (a maximum does not depend on the order
+// to xscale (fp32); `copies` of each row one after the other.  With gtop: it takes the largest |g_m| s_m, from which G is scaled (a maximum does not depend on the order
 // of the atomics; one a workgroup, only where it raises the value).
-template <class T> __global__ __launch_bounds__(256) void pack_x_kernel(const TscRows x, int M, int Mp, int D, int Dp, int n, const long long *targets,
+template <class T> __global__ __launch_bounds__(256) void pack_x_kernel(const TscRows x, int M, int Mp, int D, int Dp, int n, int copies, const long long *targets,
                                                                         long long ignore, const float *g, short *out, float *xscale, unsigned *gtop) {
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int VE = 16 / sizeof(T);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float most = 0.f;
     for (int m = (blockIdx.x * 4 + wave) * n, end = m + n < Mp ? m + n : Mp; m < end; ++m) {
-        short *o = out + (long long)m * (SPLIT ? 2 : 1) * Dp;
+        short *o = out + (long long)m * (SPLIT ? 2 : copies) * Dp;
         const bool live = m < M && (!targets || targets[m] != ignore);
         const T *p = (const T *)x.data + (live ? row_at(x, m) : 0);
         float s = 1.f;
@@ -183,7 +187,7 @@ template <class T> __global__ __launch_bounds__(256) void pack_x_kernel(const Ts
                 *(s16x4 *)q = h1;
                 *(s16x4 *)(q + 32) = h2;
             } else {
-                *(Vec<T> *)(o + d) = v;
+                for (int k = 0; k < copies; ++k) *(Vec<T> *)(o + (long long)k * Dp + d) = v;
             }
         }
     }
@@ -238,6 +242,7 @@ struct LogitArgs {
     const unsigned *gtop;    // g_unit
     short *G;            // [Mp][PLANES * ldg]
     long long ldg;
+    int rest;            // of a row's remainder behind the row (elements); FEW rows of 16-bit elements
     int Mp;
     float *dbias;        // [parts of the rows][ldg] or null
 };
@@ -406,6 +411,7 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
             }
         }
         constexpr int PL = SPLIT ? 2 : 1;
+        constexpr bool REST = !SPLIT && C::BI <= FEW_ROWS;
         long long ld2 = a.ldg * 2 * PL;
         asm volatile("" : "+s"(ld2));  // (else the distances of all rows are computed once and spilled)
         // a lane stores row (lane & 1) of a pair of rows, columns col & ~1 and the next
@@ -454,9 +460,11 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
                         if constexpr (SPLIT) {  // h2 is held times 2048
                             const f32x2 r = {fmaf((float)h[0], -2048.f, pair[0] * 2048.f), fmaf((float)h[1], -2048.f, pair[1] * 2048.f)};
                             put(__builtin_bit_cast(unsigned, __builtin_convertvector(r, f16x2)), row + 64);
-                        }
+                        } else if constexpr (REST) put(__builtin_bit_cast(unsigned, __builtin_convertvector(pair - __builtin_convertvector(h, f32x2), f16x2)), row + 2 * a.rest);
                     } else {
-                        put(__builtin_bit_cast(unsigned, __builtin_convertvector(pair, bf16x2)), row);
+                        const bf16x2 h = __builtin_convertvector(pair, bf16x2);
+                        put(__builtin_bit_cast(unsigned, h), row);
+                        if constexpr (REST) put(__builtin_bit_cast(unsigned, __builtin_convertvector(pair - __builtin_convertvector(h, f32x2), bf16x2)), row + 2 * a.rest);
                     }
                 }
             }
@@ -509,9 +517,9 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2 *part, int n, in
     loss[m] = t == ignore ? 0.f : t < 0 || t >= V ? __builtin_nanf("") : l - hit[m];
 }
 
-struct SumArgs {  // C[z][i][j] = (or +=) the z-th part of the k-steps
+struct SumArgs {  // C[z][i][j] = (or +=) the z-th part of the k-steps; pair: of rows 2 i and 2 i + 1 of A
     Operand A, B;
-    int nk, per, ti, tj, I, J, add;
+    int nk, per, ti, tj, I, J, add, pair;
     float *out;
 };
 struct OutArgs {  // C[i][j] * g_unit, in the elements' type
@@ -538,6 +546,21 @@ template <class C, bool KMAJOR, bool F16, int PLANES, int SCALED> __global__ __l
     };
     auto done = [&](int, f32x16 (&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
         float *o = a.out + ((long long)blockIdx.y * a.I + wi0 + 4 * lh) * a.J + wj0 + li;
+        if (PLANES == 1 && a.pair) {
+            o -= (long long)(wi0 / 2 + 2 * lh) * a.J;
+#pragma unroll
+            for (int p = 0; p < C::WI; ++p)
+#pragma unroll
+                for (int q = 0; q < C::WJ; ++q)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 2) {
+                        if ((wi0 + p * 32 + block_row(r, lh)) / 2 >= a.I || wj0 + q * 32 + li >= a.J) continue;
+                        float *to = o + (long long)((p * 32 + block_row(r, 0)) / 2) * a.J + q * 32;
+                        const float v = acc[p][q][r] + acc[p][q][r + 1];
+                        *to = a.add ? *to + v : v;
+                    }
+            return;
+        }
 #pragma unroll
         for (int p = 0; p < C::WI; ++p)
 #pragma unroll
@@ -747,7 +770,7 @@ struct Streams {
 };
 Streams streams(long long M, long long V) {
     Streams r{};
-    r.s = shape_of(M <= 64 ? FEW : cdiv(M, 256) * (long long)cdiv(V, 256) >= CUS ? LARGE : MEDIUM);
+    r.s = shape_of(M <= FEW_ROWS ? FEW : cdiv(M, 256) * (long long)cdiv(V, 256) >= CUS ? LARGE : MEDIUM);
     r.nm = cdiv(M, r.s.bi);
     r.nv = cdiv(V, r.s.bj);
     long long best = -1;
@@ -790,6 +813,7 @@ Split split_of(long long I, long long J, int nk, int planes, bool always_parts) 
 // What a call keeps in its workspace (each part starts at a multiple of 256 bytes)
 struct Plan {
     int Mp;
+    int copies;      // backward: rows of G a row (2: its remainder too), and of x
     Streams st;
     int Vc, pieces;  // backward: entries of a piece
     Split dx;        // of a whole piece
@@ -801,8 +825,8 @@ struct DwPlan {
     int n[2];  // entries of each part
     Split w[2];
 };
-DwPlan dw_plan(const tsc_unembed *h, long long Mp, int nv) {
-    const int nk = (int)(Mp / BK), dt = cdiv(h->D, 256);
+DwPlan dw_plan(const tsc_unembed *h, long long rows, int nv) {
+    const int nk = (int)(rows / BK), dt = cdiv(h->D, 256);
     auto of = [&](int n) { return h->sv == 1 ? split_of(h->D, n, nk, h->planes, false) : split_of(n, h->D, nk, h->planes, false); };
     DwPlan r{{nv, 0}, {of(nv), {}}};
     const int rounds = (int)((long long)dt * cdiv(nv, 256) / CUS), main = rounds * CUS / dt * 256;
@@ -813,10 +837,12 @@ DwPlan dw_plan(const tsc_unembed *h, long long Mp, int nv) {
 Plan plan(const tsc_unembed *h, long long M, bool backward, bool want_x, bool want_w, bool want_b) {
     Plan p{};
     p.Mp = (int)up(M, BK);
+    p.copies = backward && h->planes == 1 && M <= FEW_ROWS ? 2 : 1;
+    const int rows = p.copies * p.Mp;
     int nv = h->V;
     if (backward) {
         const int all = cdiv(h->V, 256);
-        const long long fit = PIECE_BYTES / (2ll * h->planes * p.Mp * 256);
+        const long long fit = PIECE_BYTES / (2ll * h->planes * rows * 256);
         const int vt = (int)(fit < 1 ? 1 : fit < all ? fit : all);
         p.Vc = vt * 256;
         p.pieces = cdiv(h->V, p.Vc);
@@ -825,23 +851,23 @@ Plan plan(const tsc_unembed *h, long long M, bool backward, bool want_x, bool wa
     p.st = streams(M, nv);
     long long at = 0;
     auto take = [&](long long n) { const long long q = at; at = up(at + n, 256); return q; };
-    p.xp = take(2ll * h->planes * p.Mp * h->Dp);
+    p.xp = take(2ll * h->planes * rows * h->Dp);
     p.xscale = take(4 * M);
     if (!backward) {
         p.part = take(8ll * p.st.ns * M);
         p.hit = take(4 * M);
     } else {
         p.gtop = take(4);
-        p.g = take(2ll * h->planes * p.Mp * p.Vc);
-        if (want_b) p.db = take(4ll * 2 * p.st.nm * p.Vc);
+        p.g = take(2ll * h->planes * rows * p.Vc);
+        if (want_b) p.db = take(4ll * 2 * p.st.nm * p.Vc);  // (two parts a tile of rows, or one of twice the pitch)
         if (want_x) {
-            p.dx = split_of(M, h->D, cdiv(nv, BK), h->planes, true);
+            p.dx = split_of(p.copies * M, h->D, cdiv(nv, BK), h->planes, true);
             p.dxp = take(4ll * p.dx.z * M * h->D);
         }
         if (want_w) {  // the parts of a piece's dW and of the last, shorter one's
             long long most = 0;
             for (int n : {nv, h->V - (p.pieces - 1) * p.Vc}) {
-                const DwPlan w = dw_plan(h, p.Mp, n);
+                const DwPlan w = dw_plan(h, rows, n);
                 for (int i = 0; i < 2; ++i)
                     if (w.n[i] && w.w[i].z > 1 && (long long)w.w[i].z * w.n[i] > most) most = (long long)w.w[i].z * w.n[i];
             }
@@ -934,9 +960,9 @@ void pack_x(const tsc_unembed *h, const Plan &p, const TscRows &x, int M, const 
     const int n = p.Mp >= 16384 ? 4 : 1;  // (a full chip of waves first)
     const dim3 grid(cdiv(p.Mp, 4 * n));
     if (h->elem == TSC_ELEM_F32)
-        hipLaunchKernelGGL((pack_x_kernel<float>), grid, dim3(256), 0, s, x, M, p.Mp, h->D, h->Dp, n, targets, ignore, g, out, xscale, gtop);
+        hipLaunchKernelGGL((pack_x_kernel<float>), grid, dim3(256), 0, s, x, M, p.Mp, h->D, h->Dp, n, p.copies, targets, ignore, g, out, xscale, gtop);
     else
-        hipLaunchKernelGGL((pack_x_kernel<short>), grid, dim3(256), 0, s, x, M, p.Mp, h->D, h->Dp, n, targets, ignore, g, out, xscale, gtop);
+        hipLaunchKernelGGL((pack_x_kernel<short>), grid, dim3(256), 0, s, x, M, p.Mp, h->D, h->Dp, n, p.copies, targets, ignore, g, out, xscale, gtop);
 }
 }  // namespace
 
@@ -978,7 +1004,8 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
     if (gtop) hipLaunchKernelGGL(fill_kernel, dim3(1), dim3(256), 0, s, (float *)gtop, 0.f, 1ll);
     pack_x(h, p, x, M, targets, ignore, g, ws, gtop, s);
     LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
-    a.lse = lse; a.g = g; a.gtop = gtop; a.G = G; a.ldg = p.Vc; a.Mp = p.Mp;
+    a.lse = lse; a.g = g; a.gtop = gtop; a.G = G; a.ldg = (long long)p.copies * p.Vc; a.rest = p.Vc; a.Mp = p.Mp;
+    a.x.ld *= p.copies;
     a.dbias = db ? (float *)(ws + p.db) : nullptr;
     const long long xld = (long long)h->planes * h->Dp;
     const int db_parts = p.st.nm * (p.st.s.kind == FEW ? 1 : 2);  // waves of a tile's rows
@@ -992,9 +1019,9 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
         if (db) hipLaunchKernelGGL(dbias_kernel, dim3(cdiv(nv, 64)), dim3(1024), 0, s, a.dbias, db_parts, a.ldg, nv, gtop, h->belem, db, (long long)v0);
         if (dx) {
             SumArgs q{};
-            q.A = {G, (long long)h->planes * p.Vc, M};
+            q.A = {G, (long long)h->planes * p.Vc, p.copies * M};
             q.B = {h->Wd + (long long)h->planes * v0, h->wd_ld, h->D};
-            q.nk = cdiv(nv, BK); q.I = M; q.J = h->D; q.add = c > 0; q.out = dxp;
+            q.nk = cdiv(nv, BK); q.I = M; q.J = h->D; q.add = c > 0; q.pair = p.copies == 2; q.out = dxp;
             Split w = p.dx;
             if (c > 0) w.per = cdiv(q.nk, w.z);  // the same parts, shorter
             rc = launch_dx(w, h->elem, q, s);
@@ -1002,7 +1029,7 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
         }
         if (dW) {
             const bool by_d = h->sv == 1;  // dW is dense in W's order: [D][V] or [V][D]
-            const DwPlan parts = dw_plan(h, p.Mp, nv);
+            const DwPlan parts = dw_plan(h, (long long)p.copies * p.Mp, nv);
             for (int i = 0, at = 0; i < 2 && parts.n[i]; at += parts.n[i++]) {
                 const Split &w = parts.w[i];
                 const Operand X = {xp, xld, h->D}, Gk = {G + (long long)h->planes * at, (long long)h->planes * p.Vc, parts.n[i]};
@@ -1013,13 +1040,13 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
                     OutArgs q{};
                     q.A = by_d ? X : Gk;
                     q.B = by_d ? Gk : X;
-                    q.nk = p.Mp / BK; q.I = I; q.J = J; q.gtop = gtop; q.elem = h->elem; q.ld = ld; q.out = out;
+                    q.nk = p.copies * p.Mp / BK; q.I = I; q.J = J; q.gtop = gtop; q.elem = h->elem; q.ld = ld; q.out = out;
                     rc = launch_dw(w, h->elem, by_d, q, s);
                 } else {
                     SumArgs q{};
                     q.A = by_d ? X : Gk;
                     q.B = by_d ? Gk : X;
-                    q.nk = p.Mp / BK; q.I = I; q.J = J; q.out = (float *)(ws + p.dwp);
+                    q.nk = p.copies * p.Mp / BK; q.I = I; q.J = J; q.out = (float *)(ws + p.dwp);
                     rc = launch_dw_parts(w, h->elem, by_d, q, s);
                     if (!rc) hipLaunchKernelGGL(join_kernel, dim3(I, cdiv(J, 1024)), dim3(256), 0, s, q.out, w.z, I, J, gtop, out, ld, h->elem);
                 }
