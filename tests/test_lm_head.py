@@ -288,6 +288,12 @@ def test_capture_while_an_eager_pass_lives_is_refused():
                 call()
     want = float(eager)
     del eager, y
+    E = W.detach().t().contiguous().requires_grad_()
+    tied = tsc_hip.UnembedHead(E.t(), bu.detach())
+    with pytest.raises(tsc_hip.TscError, match="view"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            static.add_(0.0)
+            lm_head.unembed_loss(static, t, tied)
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         loss = lm_head.unembed_loss(lm_head.layer_norm(x, w, b), t, head)

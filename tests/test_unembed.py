@@ -355,6 +355,31 @@ def test_captured_and_replayed(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_weights_changed_before_a_capture(dtype):
+    """The capture lays out nothing by itself: an eager call before the first replay sees the change all the same, and so does
+    every replay, also of a change that comes after it."""
+    import tsc_hip
+
+    x, W, b, t, _ = make(20, 64, 300, dtype, seed=23)
+    head = tsc_hip.UnembedHead(W, b)
+    head.loss(x, t)
+    W.mul_(1.5)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = head.loss(x, t)
+    fresh = lambda: tsc_hip.UnembedHead(W.clone(), b).loss(x, t)  # noqa: E731
+    assert all(torch.equal(p, q) for p, q in zip(head.loss(x, t), fresh()))
+    for k in (1.0, 0.5, 1.25):
+        W.mul_(k)
+        want = fresh()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
+        assert all(torch.equal(p, q) for p, q in zip(head.loss(x, t), want))
+
+
+@pytest.mark.gpu
 def test_two_streams_share_a_head():
     import tsc_hip
 

@@ -6,8 +6,10 @@ the ``[rows, d_vocab]`` logits (``tsc_layer_norm*``, ``tsc_unembed_*`` through `
     loss.backward()                                                  # resid, w, b, W_U and b_U
 
 Gradients are first-order (a second derivative raises) and the same call gives the same bits.  Both may be captured into a
-HIP graph, the backward pass too.  A captured pass whose weights learn lays them out again on every replay; a capture while
-an eager pass over the same leaves is alive is refused (``_mark_leaves``).
+HIP graph, the backward pass too.  A captured pass whose weights learn lays them out again on every replay (replays do not
+tell torch that they changed the weights: ``head.refresh()`` before an eager call that follows them); a capture while an eager
+pass over the same leaves is alive is refused (``_mark_leaves``), and so is one whose head is of a view (``W_E.t()``) that
+learns.
 """
 from __future__ import annotations
 
@@ -115,7 +117,11 @@ def unembed_loss(x: torch.Tensor, targets: torch.Tensor, head: "tsc_hip.UnembedH
         raise tsc_hip.TscError(f"reduction must be 'none', 'sum' or 'mean' (got {reduction!r})")
     if torch.is_grad_enabled():
         held = _mark_leaves(x, head.W_U, head.b_U)  # noqa: F841
-        if torch.cuda.is_current_stream_capturing() and any(p is not None and p.requires_grad for p in (head.W_U, head.b_U)):
+        learning = [p for p in (head.W_U, head.b_U) if p is not None and p.requires_grad]
+        if learning and torch.cuda.is_current_stream_capturing():
+            if not all(p.is_leaf for p in learning):
+                raise tsc_hip.TscError("the head's W_U or b_U is a view of the leaf that learns, made before the capture: its "
+                                       "accumulator may belong to another stream; make the head of leaves, or step eagerly")
             head.refresh()  # part of the graph: a replay finds the weights that the step before it left
     rows = _UnembedLoss.apply(x, head.W_U, head.b_U, targets, head, ignore_index)
     if reduction == "none":

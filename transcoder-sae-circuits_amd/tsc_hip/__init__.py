@@ -1020,7 +1020,9 @@ class UnembedHead:
 
     Borrows both tensors and owns 16-bit copies of ``W_U`` in both orders, laid out at construction and again by
     :meth:`refresh`.  :meth:`loss` and :meth:`loss_backward` do that by themselves when torch's version counters say that a
-    tensor was changed in place (inference tensors have none: call :meth:`refresh`)."""
+    tensor was changed in place (inference tensors have none, and the replay of a graph that changes them does not count, nor does a
+    replayed call look: call :meth:`refresh` after the change).  Calls on several streams may run at once; one that lays out again is ordered with the others by
+    the caller, like the change itself."""
 
     def __init__(self, W_U: torch.Tensor, b_U: Optional[torch.Tensor] = None):
         self._handle = ctypes.c_void_p()
@@ -1052,10 +1054,12 @@ class UnembedHead:
         return tuple(0 if t.is_inference() else t._version for t in self._keep)
 
     def refresh(self) -> None:
-        """Lay the weights out again (``tsc_unembed_refresh``)."""
-        with torch.cuda.device(self.device):
-            _check(lib().tsc_unembed_refresh(self._handle, _stream()))
-        self._versions = self._param_versions()
+        """Lay the weights out again (``tsc_unembed_refresh``).  Captured into a graph it is part of every replay."""
+        if not self._handle:
+            raise TscError("this UnembedHead is closed")
+        _launch(self.device.index, lib().tsc_unembed_refresh, self._handle)
+        if not torch.cuda.is_current_stream_capturing():  # (a captured one has laid out nothing yet)
+            self._versions = self._param_versions()
 
     def refresh_if_modified(self) -> None:
         if self._param_versions() != self._versions:
@@ -1088,7 +1092,8 @@ class UnembedHead:
         return torch.empty(n, dtype=torch.uint8, device=self.device), n
 
     def loss(self, x: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100) -> Tuple[torch.Tensor, torch.Tensor]:
-        """``tsc_unembed_loss``: ``(loss, lse)``, float32 of shape ``x.shape[:-1]``: every row's cross entropy (0 where the
+        """``tsc_unembed_loss``: ``(loss, lse)``, float32 of shape ``x.shape[:-1]`` (``targets``: int64 of that shape,
+        contiguous): every row's cross entropy (0 where the
         target is ``ignore_index``, NaN where it is outside the vocabulary otherwise) and the logarithm of its sum of
         exponentials, which :meth:`loss_backward` takes."""
         rows, m = self._operands(x, targets)
@@ -1102,7 +1107,7 @@ class UnembedHead:
 
     def loss_backward(self, dloss: torch.Tensor, x: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
                       ignore_index: int = -100, want_x: bool = True, want_weight: bool = True, want_bias: bool = True):
-        """``tsc_unembed_loss_backward``: ``(dx, dW, db)`` for the gradient ``dloss`` (float32, ``x.shape[:-1]``) of the rows'
+        """``tsc_unembed_loss_backward``: ``(dx, dW, db)`` for the gradient ``dloss`` (float32, ``x.shape[:-1]``, contiguous) of the rows'
         losses, None where not wanted (``db`` also without ``b_U``).  ``dx`` and ``dW`` have x's type, ``dW`` the shape and
         the order of ``W_U``, ``db`` the type of ``b_U``."""
         rows, m = self._operands(x, targets)
