@@ -99,7 +99,7 @@ class SparseTranscoder(HipDictionaryMixin, nn.Module):
     def get_test_loss(self, batch_tokens, model):
         """Mean next-token loss of ``model`` on ``batch_tokens [batch, n]`` with the dictionary's output in the place of what
         it reconstructs: the layer's MLP output for a transcoder (computed from the activation at ``cfg.hook_point``), the
-        activation itself otherwise.  Compare with ``model(batch_tokens, return_type="loss")``."""
+        activation itself otherwise (reference :492-542).  Compare with ``model(batch_tokens, return_type="loss")``."""
         if getattr(self.cfg, "hook_point_head_index", None) is not None:
             raise NotImplementedError("a dictionary of one attention head is outside the accelerated analysis path")
 
