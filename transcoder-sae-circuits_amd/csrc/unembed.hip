@@ -146,17 +146,29 @@ template <class T> __global__ __launch_bounds__(256) void pack_x_kernel(const Ts
         const bool live = m < M && (!targets || targets[m] != ignore);
         const T *p = (const T *)x.data + (live ? row_at(x, m) : 0);
         float s = 1.f;
+        auto load = [&](int d) __attribute__((always_inline)) {
+            Vec<T> v;
+            if (live && d + VE <= D) {
+                v = *(const Vec<T> *)(p + d);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) v.e[e] = live && d + e < D ? p[d + e] : (T)0;
+            }
+            return v;
+        };
+        constexpr int HELD = SPLIT ? 4 : 1;  // vectors a lane that are read once, all at the same time (for few rows that is what counts)
+        Vec<T> held[HELD];
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) held[i] = load((i * 64 + lane) * VE);
         if constexpr (SPLIT) {
             float top = 0.f;
-            if (live)
-                for (int d = lane * VE; d < D; d += 64 * VE)
-                    if (d + VE <= D) {
-                        const Vec<T> v = *(const Vec<T> *)(p + d);
+            auto take = [&](const Vec<T> &v) __attribute__((always_inline)) {
 #pragma unroll
-                        for (int e = 0; e < VE; ++e) top = fabsf(v.e[e]) < __builtin_inff() ? fmaxf(top, fabsf(v.e[e])) : top;
-                    } else {
-                        for (int e = d; e < D; ++e) top = fabsf(p[e]) < __builtin_inff() ? fmaxf(top, fabsf(p[e])) : top;
-                    }
+                for (int e = 0; e < VE; ++e) top = fabsf(v.e[e]) < __builtin_inff() ? fmaxf(top, fabsf(v.e[e])) : top;
+            };
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) take(held[i]);
+            for (int d = (HELD * 64 + lane) * VE; d < D; d += 64 * VE) take(load(d));
             for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
             s = pow2_scale(top);
             if (lane == 0 && m < M) xscale[m] = s;
@@ -166,14 +178,7 @@ template <class T> __global__ __launch_bounds__(256) void pack_x_kernel(const Ts
             most = v < __builtin_inff() ? fmaxf(most, v) : most;
         }
         const float inv = 1.f / s;
-        for (int d = lane * VE; d < Dp; d += 64 * VE) {
-            Vec<T> v;
-            if (live && d + VE <= D) {
-                v = *(const Vec<T> *)(p + d);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VE; ++e) v.e[e] = live && d + e < D ? p[d + e] : (T)0;
-            }
+        auto store = [&](int d, const Vec<T> &v) __attribute__((always_inline)) {
             if constexpr (SPLIT) {
                 s16x4 h1, h2;
 #pragma unroll
@@ -189,7 +194,11 @@ template <class T> __global__ __launch_bounds__(256) void pack_x_kernel(const Ts
             } else {
                 for (int k = 0; k < copies; ++k) *(Vec<T> *)(o + (long long)k * Dp + d) = v;
             }
-        }
+        };
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if ((i * 64 + lane) * VE < Dp) store((i * 64 + lane) * VE, held[i]);
+        for (int d = (HELD * 64 + lane) * VE; d < Dp; d += 64 * VE) store(d, load(d));
     }
     if (!gtop) return;
     __shared__ float all[4];
@@ -496,25 +505,30 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
     G::run(a.x, a.W, (a.nv - st + a.ns - 1) / a.ns, tile, 0, a.nk, lds, begin, done);
 }
 
-// lse and loss of the rows from the tiles' parts: one wave a row
-__global__ __launch_bounds__(256) void loss_kernel(const float2 *part, int n, int M, int V, const float *hit, const long long *targets,
-                                                   long long ignore, float *loss, float *lse) {
-    const int m = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+// lse and loss of the rows from the streams' parts: a wave a row, or (LANE) a lane, whose loads are then whole lines: many rows
+// have few streams (65536 rows of 4: 5 us against 32 as waves)
+template <bool LANE> __global__ __launch_bounds__(256) void loss_kernel(const float2 *part, int n, int M, int V, const float *hit, const long long *targets,
+                                                                        long long ignore, float *loss, float *lse) {
+    const int lane = threadIdx.x & 63, m = LANE ? blockIdx.x * 256 + threadIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6);
     if (m >= M) return;
+    const long long t = targets[m];
+    const float h = hit[m];  // (nothing where the target is no entry)
     float2 all = make_float2(-__builtin_inff(), 0.f);
-    for (int i = lane; i < n; i += 512) {  // (the loads of eight parts under way at once)
+    constexpr int STEP = LANE ? 1 : 64;
+    for (int i = LANE ? 0 : lane; i < n; i += 8 * STEP) {  // (the loads of eight parts under way at once)
         float2 v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = i + 64 * k < n ? part[(long long)(i + 64 * k) * M + m] : make_float2(-__builtin_inff(), 0.f);
+        for (int k = 0; k < 8; ++k) v[k] = i + STEP * k < n ? part[(long long)(i + STEP * k) * M + m] : make_float2(-__builtin_inff(), 0.f);
 #pragma unroll
         for (int k = 0; k < 8; ++k) all = merge(all, v[k]);
     }
-    for (int o = 32; o > 0; o >>= 1) all = merge(all, make_float2(__shfl_xor(all.x, o), __shfl_xor(all.y, o)));
-    if (lane) return;
+    if constexpr (!LANE) {
+        for (int o = 32; o > 0; o >>= 1) all = merge(all, make_float2(__shfl_xor(all.x, o), __shfl_xor(all.y, o)));
+        if (lane) return;
+    }
     const float l = (all.x + __log2f(all.y)) * LN2;
-    const long long t = targets[m];
     lse[m] = l;
-    loss[m] = t == ignore ? 0.f : t < 0 || t >= V ? __builtin_nanf("") : l - hit[m];
+    loss[m] = t == ignore ? 0.f : t < 0 || t >= V ? __builtin_nanf("") : l - h;
 }
 
 struct SumArgs {  // C[z][i][j] = (or +=) the z-th part of the k-steps; pair: of rows 2 i and 2 i + 1 of A
@@ -983,7 +997,8 @@ int tsc_launch_unembed_loss(const tsc_unembed *h, const TscRows &x, int M, const
     a.hit = (float *)(ws + p.hit);
     const int rc = logits<false>(h, p.st, a, s);
     if (rc) return rc;
-    hipLaunchKernelGGL(loss_kernel, dim3(cdiv(M, 4)), dim3(256), 0, s, a.part, p.st.ns, M, h->V, a.hit, targets, ignore, loss, lse);
+    if (p.st.ns <= 16) hipLaunchKernelGGL((loss_kernel<true>), dim3(cdiv(M, 256)), dim3(256), 0, s, a.part, p.st.ns, M, h->V, a.hit, targets, ignore, loss, lse);
+    else hipLaunchKernelGGL((loss_kernel<false>), dim3(cdiv(M, 4)), dim3(256), 0, s, a.part, p.st.ns, M, h->V, a.hit, targets, ignore, loss, lse);
     TSC_HIP_CHECK(hipGetLastError());
     return TSC_OK;
 }
