@@ -252,7 +252,7 @@ struct LogitArgs {
     short *G;            // [Mp][PLANES * ldg]
     long long ldg;
     int rest;            // of a row's remainder behind the row (elements); FEW rows of 16-bit elements
-    int Mp;
+    int Mp;              // rows of G that are wanted (32 at a time are written)
     float *dbias;        // [parts of the rows][ldg] or null
 };
 
@@ -481,7 +481,7 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
         };
 #pragma unroll
         for (int p = 0; p < C::WI; ++p) {
-            if (i0 + wr + p * 32 >= a.Mp) break;  // (Mp is a multiple of 64)
+            if (i0 + wr + p * 32 >= a.Mp) break;
 #pragma unroll
             for (int s = 0; s < 4; ++s) quad(std::false_type(), p, s, 0, C::WJ);
         }
@@ -813,7 +813,7 @@ Split split_of(long long I, long long J, int nk, int planes, bool always_parts) 
         r.ti = cdiv(I, r.s.bi);
         r.tj = cdiv(J, r.s.bj);
         const double step = (kind == LARGE ? 1.8e-6 : 1.1e-6) * (planes == 2 ? 3 : 1), start = 4e-6, part = (double)I * J * 8 / 5e12;
-        for (int z = 1; z <= 64 && z <= nk; ++z) {
+        for (int z = 1; z <= 128 && z <= nk; ++z) {
             r.per = cdiv(nk, z);
             r.z = cdiv(nk, r.per);
             const double cost = (double)cdiv((long long)r.ti * r.tj * r.z, r.s.slots) * (r.per * step + start) +
@@ -1019,7 +1019,8 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
     if (gtop) hipLaunchKernelGGL(fill_kernel, dim3(1), dim3(256), 0, s, (float *)gtop, 0.f, 1ll);
     pack_x(h, p, x, M, targets, ignore, g, ws, gtop, s);
     LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
-    a.lse = lse; a.g = g; a.gtop = gtop; a.G = G; a.ldg = (long long)p.copies * p.Vc; a.rest = p.Vc; a.Mp = p.Mp;
+    a.lse = lse; a.g = g; a.gtop = gtop; a.G = G; a.ldg = (long long)p.copies * p.Vc; a.rest = p.Vc;
+    a.Mp = dW ? p.Mp : M;  // (only dW's k-steps run over the rows behind M)
     a.x.ld *= p.copies;
     a.dbias = db ? (float *)(ws + p.db) : nullptr;
     const long long xld = (long long)h->planes * h->Dp;
