@@ -79,10 +79,14 @@ def reference(x, W, b, t, dloss, ignore=-100):
         half = 2.0 ** -11 if dt == torch.float16 else 2.0 ** -8
         rnd = half * (half if M <= 64 else 1.0) * out_G.abs() + (2.0 ** -39 * g.abs().max() if dt == torch.float16 else 0.0)
     e_op = e_raw + rnd
+    e_dx = e_op  # what the rounding took of the target's entry is added in fp32
+    if dt != torch.float32 and M > 64:
+        e_dx = e_op.clone()
+        e_dx[torch.arange(M, device=x.device), at[:, 0]] = (e_raw + 4 * U * out_G.abs()).gather(1, at)[:, 0]
     passes_rel = 3 * 2.0 ** -22 if dt == torch.float32 else 0.0
     aG, aw = out_G.abs(), wd.abs()
     wt = wd.t().contiguous()
-    out["dx"] = (out_G @ wt, e_op @ aw.t().contiguous() + (4 * math.sqrt(passes * V) * U + passes_rel) * (aG @ aw.t().contiguous())
+    out["dx"] = (out_G @ wt, e_dx @ aw.t().contiguous() + (4 * math.sqrt(passes * V) * U + passes_rel) * (aG @ aw.t().contiguous())
                  + (2 * 2.0 ** -39 * wd.abs().max() * aG.sum(-1, keepdim=True) if dt == torch.float32 else 0.0))
     xt = xd.t().contiguous()
     # (an element of x is held against its row's largest: 2^-39 of that, twice for its h1 / 2048)

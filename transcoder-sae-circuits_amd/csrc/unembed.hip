@@ -9,8 +9,9 @@
 // the workgroup.  Backward, in pieces of the vocabulary: G of a piece goes to the workspace in 16 bits (fp32: two fp16
 // planes), and the two products read it from there.  One entry carries most of a row of G, the target's, so what is lost of
 // it in 16 bits is lost of the row's gradient: as much as the result's own rounding loses on the average of many rows, up to
-// twice that in a single one.  So up to 64 rows of 16-bit elements, whose time is W's way from memory, also keep what the
-// rounding took (rows 2 m: G_m, 2 m + 1: its remainder), and both products run over twice as many rows.
+// twice that in a single one.  So what the rounding took of it is kept as a number a row, and dx adds it times W's row t; and
+// up to 64 rows of 16-bit elements, whose time is W's way from memory, keep what the rounding took of all entries (rows 2 m:
+// G_m, 2 m + 1: its remainder), and both products run over twice as many rows.
 #include <new>
 #include <type_traits>
 
@@ -252,6 +253,7 @@ struct LogitArgs {
     short *G;            // [Mp][PLANES * ldg]
     long long ldg;
     int rest;            // of a row's remainder behind the row (elements); FEW rows of 16-bit elements
+    float *left;         // or [M]: the remainder of the target's entry alone; more of them; null: not wanted
     int Mp;              // rows of G that are wanted (32 at a time are written)
     float *dbias;        // [parts of the rows][ldg] or null
 };
@@ -456,6 +458,12 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
                     w[e] *= f[e];
                     if (!AGAIN) db[q] = SPLIT ? fmaf(w[e], inv[e], db[q]) : db[q] + w[e];
                 }
+                if constexpr (AGAIN && !SPLIT && !REST) {
+                    if (a.left)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (r_t[at + e] == v + q * 32 + li) a.left[i0 + at + e] = w[e] - (F16 ? (float)(_Float16)w[e] : (float)(__bf16)w[e]);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
                     auto put = [&](unsigned own, char *to) __attribute__((always_inline)) {
@@ -636,7 +644,8 @@ __global__ __launch_bounds__(256) void join_kernel(const float *part, int n, int
 }
 // dx[m][d] = sum over z, with the scales undone: 256 elements of a row a workgroup, its waves share the parts
 __global__ __launch_bounds__(256) void dx_kernel(const float *part, int n, int M, int D, const float *wscale, const float *xscale,
-                                                 const unsigned *gtop, const long long *targets, long long ignore, int elem, void *dx) {
+                                                 const unsigned *gtop, const long long *targets, long long ignore, const float *left,
+                                                 const short *Wt, long long wt_ld, int V, int elem, void *dx) {
     __shared__ float red[3][256];
     const int m = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = blockIdx.y * 256 + lane * 4;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -657,12 +666,16 @@ __global__ __launch_bounds__(256) void dx_kernel(const float *part, int n, int M
         for (int e = 0; e < 4; ++e) red[wave - 1][e * 64 + lane] = v[e];
     __syncthreads();
     if (wave) return;
-    const bool live = targets[m] != ignore;
+    const long long t = targets[m];
+    const bool live = t != ignore, add = left && live && t >= 0 && t < V;
+    const float rest = add ? left[m] : 0.f;
     const float unit = g_unit(gtop), ws = wscale ? wscale[0] : 1.f, xs = wscale ? 1.f / xscale[m] : 1.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float all = (v[e] + red[0][e * 64 + lane]) + (red[1][e * 64 + lane] + red[2][e * 64 + lane]);
-        if (d + e < D) write_elem(dx, elem, (long long)m * D + d + e, live ? all * unit * ws * xs : 0.f);
+        if (d + e >= D) continue;
+        float all = (v[e] + red[0][e * 64 + lane]) + (red[1][e * 64 + lane] + red[2][e * 64 + lane]);
+        if (add) all = fmaf(rest, read_elem(Wt, elem, t * wt_ld + d + e), all);
+        write_elem(dx, elem, (long long)m * D + d + e, live ? all * unit * ws * xs : 0.f);
     }
 }
 // db[at + j] = sum over the parts, 64 columns x 16 parts a workgroup
@@ -828,10 +841,11 @@ Split split_of(long long I, long long J, int nk, int planes, bool always_parts) 
 struct Plan {
     int Mp;
     int copies;      // backward: rows of G a row (2: its remainder too), and of x
+    bool left_wanted;
     Streams st;
     int Vc, pieces;  // backward: entries of a piece
     Split dx;        // of a whole piece
-    long long xp, xscale, part, hit, gtop, g, db, dxp, dwp, bytes;
+    long long xp, xscale, part, hit, gtop, left, g, db, dxp, dwp, bytes;
 };
 // dW of nv entries of the vocabulary: as many of them as fill whole rounds of the chip in one piece, the rest (or all of them,
 // where that is cheaper) with their k-steps split.
@@ -872,6 +886,8 @@ Plan plan(const tsc_unembed *h, long long M, bool backward, bool want_x, bool wa
         p.hit = take(4 * M);
     } else {
         p.gtop = take(4);
+        p.left_wanted = want_x && h->planes == 1 && p.copies == 1;
+        if (p.left_wanted) p.left = take(4 * M);
         p.g = take(2ll * h->planes * rows * p.Vc);
         if (want_b) p.db = take(4ll * 2 * p.st.nm * p.Vc);  // (two parts a tile of rows, or one of twice the pitch)
         if (want_x) {
@@ -1020,6 +1036,7 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
     pack_x(h, p, x, M, targets, ignore, g, ws, gtop, s);
     LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
     a.lse = lse; a.g = g; a.gtop = gtop; a.G = G; a.ldg = (long long)p.copies * p.Vc; a.rest = p.Vc;
+    a.left = p.left_wanted ? (float *)(ws + p.left) : nullptr;
     a.Mp = dW ? p.Mp : M;  // (only dW's k-steps run over the rows behind M)
     a.x.ld *= p.copies;
     a.dbias = db ? (float *)(ws + p.db) : nullptr;
@@ -1071,7 +1088,8 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
         }
         TSC_HIP_CHECK(hipGetLastError());
     }
-    if (dx) hipLaunchKernelGGL(dx_kernel, dim3(M, cdiv(h->D, 256)), dim3(256), 0, s, dxp, p.dx.z, M, h->D, a.wscale, a.xscale, gtop, targets, ignore, h->elem, dx);
+    if (dx) hipLaunchKernelGGL(dx_kernel, dim3(M, cdiv(h->D, 256)), dim3(256), 0, s, dxp, p.dx.z, M, h->D, a.wscale, a.xscale, gtop, targets, ignore, a.left, h->Wt, h->wt_ld,
+                               h->V, h->elem, dx);
     TSC_HIP_CHECK(hipGetLastError());
     return TSC_OK;
 }
