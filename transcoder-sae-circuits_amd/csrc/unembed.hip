@@ -623,59 +623,76 @@ template <class C, bool F16, int PLANES, int SCALED> __global__ __launch_bounds_
     };
     G::run(a.A, a.B, 1, [&](int) { return TileAt{bi * C::BI, bj * C::BJ}; }, 0, a.nk, lds, begin, done);
 }
-// C[i][j] = sum over z of part[z][i][j] times g_unit, 4 elements a lane: a dW whose k-steps were split
-__global__ __launch_bounds__(256) void join_kernel(const float *part, int n, int I, int J, const unsigned *gtop, void *out, long long ld, int elem) {
-    const int i = blockIdx.x, j = (blockIdx.y * 256 + threadIdx.x) * 4;
-    const float unit = g_unit(gtop);
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (j + 4 <= J) {
-        for (int z = 0; z < n; ++z) {
-            const Vec<float> u = *(const Vec<float> *)(part + ((long long)z * I + i) * J + j);
+// v = the sum of n parts, `step` apart, of 4 neighbouring elements at p (fewer where only `rest` are left).  SHARED: the four
+// waves of the workgroup take every fourth part each, and the first one, for which this is true, gets the sums.
+template <bool SHARED> __device__ __forceinline__ bool sum_parts(const float *p, int n, long long step, int rest, float (&red)[3][256], float (&v)[4]) {
+    const int lane = threadIdx.x & 63, wave = SHARED ? threadIdx.x >> 6 : 0;
+    constexpr int W = SHARED ? 4 : 1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = 0.f;
+    if (rest >= 4) {
+#pragma unroll 4
+        for (int z = wave; z < n; z += W) {
+            const Vec<float> u = *(const Vec<float> *)(p + z * step);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] += u.e[e];
         }
     } else {
-        for (int e = 0; j + e < J; ++e)
-            for (int z = 0; z < n; ++z) v[e] += part[((long long)z * I + i) * J + j + e];
+        for (int e = 0; e < rest; ++e)
+            for (int z = wave; z < n; z += W) v[e] += p[z * step + e];
     }
+    if constexpr (SHARED) {
+        if (wave)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) red[wave - 1][e * 64 + lane] = v[e];
+        __syncthreads();
+        if (wave) return false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (v[e] + red[0][e * 64 + lane]) + (red[1][e * 64 + lane] + red[2][e * 64 + lane]);
+    }
+    return true;
+}
+// C[i][j] = sum over z of part[z][i][j] times g_unit, 4 elements a lane: a dW whose k-steps were split
+template <bool SHARED> __global__ __launch_bounds__(256) void join_kernel(const float *part, int n, int I, int J, const unsigned *gtop, void *out,
+                                                                          long long ld, int elem) {
+    __shared__ float red[3][256];
+    const int i = blockIdx.x, j = SHARED ? blockIdx.y * 256 + (threadIdx.x & 63) * 4 : (blockIdx.y * 256 + threadIdx.x) * 4;
+    float v[4];
+    if (!sum_parts<SHARED>(part + (long long)i * J + j, n, (long long)I * J, J - j, red, v)) return;
+    const float unit = g_unit(gtop);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (j + e < J) write_elem(out, elem, i * ld + j + e, v[e] * unit);
 }
-// dx[m][d] = sum over z, with the scales undone: 256 elements of a row a workgroup, its waves share the parts
-__global__ __launch_bounds__(256) void dx_kernel(const float *part, int n, int M, int D, const float *wscale, const float *xscale,
+// dx[m][d] = sum over z, with the scales undone: 256 elements of a row a workgroup, whose waves share the parts, or a wave (few
+// parts, many rows: what takes the time is the way from a row's target to its row of W)
+template <bool SHARED> __global__ __launch_bounds__(256) void dx_kernel(const float *part, int n, int M, int D, const float *wscale, const float *xscale,
                                                  const unsigned *gtop, const long long *targets, long long ignore, const float *left,
                                                  const short *Wt, long long wt_ld, int V, int elem, void *dx) {
     __shared__ float red[3][256];
-    const int m = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = blockIdx.y * 256 + lane * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    const float *p = part + (long long)m * D + d;
-    if (d + 4 <= D) {
-#pragma unroll 4
-        for (int z = wave; z < n; z += 4) {
-            const Vec<float> u = *(const Vec<float> *)(p + (long long)z * M * D);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += u.e[e];
-        }
-    } else {
-        for (int e = 0; d + e < D; ++e)
-            for (int z = wave; z < n; z += 4) v[e] += p[(long long)z * M * D + e];
-    }
-    if (wave)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) red[wave - 1][e * 64 + lane] = v[e];
-    __syncthreads();
-    if (wave) return;
+    const int m = SHARED ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6), d = blockIdx.y * 256 + (threadIdx.x & 63) * 4;
+    if (!SHARED && m >= M) return;
     const long long t = targets[m];
-    const bool live = t != ignore, add = left && live && t >= 0 && t < V;
-    const float rest = add ? left[m] : 0.f;
+    const bool live = t != ignore;
+    struct __attribute__((packed, aligned(2))) Four { short e[4]; } u = {};
+    float v[4], rest = 0.f;
+    if (left && live && t >= 0 && t < V && (!SHARED || threadIdx.x < 64)) {  // (on their way while the parts are summed)
+        rest = left[m];
+        const short *p = Wt + t * wt_ld + d;
+        if (d + 4 <= D) {
+            u = *(const Four *)p;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (d + e < D) u.e[e] = p[e];
+        }
+    }
+    if (!sum_parts<SHARED>(part + (long long)m * D + d, n, (long long)M * D, D - d, red, v)) return;
     const float unit = g_unit(gtop), ws = wscale ? wscale[0] : 1.f, xs = wscale ? 1.f / xscale[m] : 1.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        if (d + e >= D) continue;
-        float all = (v[e] + red[0][e * 64 + lane]) + (red[1][e * 64 + lane] + red[2][e * 64 + lane]);
-        if (add) all = fmaf(rest, read_elem(Wt, elem, t * wt_ld + d + e), all);
-        write_elem(dx, elem, (long long)m * D + d + e, live ? all * unit * ws * xs : 0.f);
+        const float w = elem == TSC_ELEM_BF16 ? (float)__builtin_bit_cast(__bf16, u.e[e]) : (float)__builtin_bit_cast(_Float16, u.e[e]);
+        if (d + e < D) write_elem(dx, elem, (long long)m * D + d + e, live ? fmaf(rest, w, v[e]) * unit * ws * xs : 0.f);
     }
 }
 // db[at + j] = sum over the parts, 64 columns x 16 parts a workgroup
@@ -1081,15 +1098,25 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
                     q.B = by_d ? Gk : X;
                     q.nk = p.copies * p.Mp / BK; q.I = I; q.J = J; q.out = (float *)(ws + p.dwp);
                     rc = launch_dw_parts(w, h->elem, by_d, q, s);
-                    if (!rc) hipLaunchKernelGGL(join_kernel, dim3(I, cdiv(J, 1024)), dim3(256), 0, s, q.out, w.z, I, J, gtop, out, ld, h->elem);
+                    if (!rc) {  // (many parts are of few elements: 63 of 311 x 137 25 us by single waves)
+                        if (w.z >= 8) hipLaunchKernelGGL((join_kernel<true>), dim3(I, cdiv(J, 256)), dim3(256), 0, s, q.out, w.z, I, J, gtop, out, ld, h->elem);
+                        else hipLaunchKernelGGL((join_kernel<false>), dim3(I, cdiv(J, 1024)), dim3(256), 0, s, q.out, w.z, I, J, gtop, out, ld, h->elem);
+                    }
                 }
                 if (rc) return rc;
             }
         }
         TSC_HIP_CHECK(hipGetLastError());
     }
-    if (dx) hipLaunchKernelGGL(dx_kernel, dim3(M, cdiv(h->D, 256)), dim3(256), 0, s, dxp, p.dx.z, M, h->D, a.wscale, a.xscale, gtop, targets, ignore, a.left, h->Wt, h->wt_ld,
-                               h->V, h->elem, dx);
+    if (dx) {
+        const bool shared = p.dx.z >= 8;
+        const dim3 grid(shared ? M : cdiv(M, 4), cdiv(h->D, 256));
+        auto launch = [&](auto *kernel) {
+            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, dxp, p.dx.z, M, h->D, a.wscale, a.xscale, gtop, targets, ignore, a.left, h->Wt,
+                               h->wt_ld, h->V, h->elem, dx);
+        };
+        shared ? launch(dx_kernel<true>) : launch(dx_kernel<false>);
+    }
     TSC_HIP_CHECK(hipGetLastError());
     return TSC_OK;
 }
