@@ -55,8 +55,8 @@ template <int WI_, int WJ_, int VI_, int VJ_> struct Tile {  // 32 x 32 blocks o
 // (LARGE as four waves of 128 x 128, one a SIMD with its 256 sums in accumulator registers, has 2/3 of the LDS reads and a
 // loop without a spill; alone it measured 1195 TFLOP/s against 1292 of eight waves of 128 x 64 at 8192^3, and its epilogue
 // overlaps with nothing: loss of 65536 rows 6.55 ms against 4.47.  Two workgroups a CU of four waves and 128 x 192, so that one
-// multiplies while the other takes exponentials: 4.58 against 4.16 ms, 1178 against 1063 us at 16384 rows -- more bytes per
-// product, and power is what there is none of.)
+// multiplies while the other takes exponentials: 4.58 against 4.16 ms, 1178 against 1063 us at 16384 rows -- they move more bytes
+// a product, and power is the limit.)
 typedef Tile<4, 2, 2, 4> TileLarge;   // 256 x 256, one workgroup a CU
 typedef Tile<2, 2, 2, 2> TileMedium;  // 128 x 128, two
 typedef Tile<1, 2, 4, 1> TileTall;    // 128 x 64: few tokens, the vocabulary streams
