@@ -9,9 +9,10 @@
 // the workgroup.  Backward, in pieces of the vocabulary: G of a piece goes to the workspace in 16 bits (fp32: two fp16
 // planes), and the two products read it from there.  One entry carries most of a row of G, the target's, so what is lost of
 // it in 16 bits is lost of the row's gradient: as much as the result's own rounding loses on the average of many rows, up to
-// twice that in a single one.  So what the rounding took of it is kept as a number a row, and dx adds it times W's row t; and
-// up to 64 rows of 16-bit elements, whose time is W's way from memory, keep what the rounding took of all entries (rows 2 m:
-// G_m, 2 m + 1: its remainder), and both products run over twice as many rows.
+// twice that in a single one.  So what the rounding took of it is kept as a number a row; dx adds it times W's row t, and dW's
+// column t adds it times the row (target_rows_kernel).  Up to 64 rows of 16-bit elements, whose time is W's way from memory,
+// keep what the rounding took of all entries (rows 2 m: G_m, 2 m + 1: its remainder), and both products run over twice as many
+// rows.
 #include <new>
 #include <type_traits>
 
@@ -539,6 +540,196 @@ template <bool LANE> __global__ __launch_bounds__(256) void loss_kernel(const fl
     loss[m] = t == ignore ? 0.f : t < 0 || t >= V ? __builtin_nanf("") : l - h;
 }
 
+// What G's rounding took of the targets' entries, for dW: sums[m][d] = sum of left[k] x[k][d] over the rows k whose target is
+// row m's, for the first row m of every one of the tokens v0 .. v1 - 1 that has a row, and slot[v] = that row, -1 where v has
+// none.  A workgroup looks through the targets for those among its TOKENS tokens and keeps their rows in order, so that every
+// sum has a fixed order; where the list could overflow it is added up first, and the next one goes on from there.  A wave takes
+// the rows of a token one after the other, all waves together those of a token that has many, and join what they have.
+// Bound by latency (a target's way from memory, a row's, the sums' back).  Measured: 16384 rows x 768 of
+// 50257 tokens 47 us, 1999 x 1001 of 32003 11 us.
+constexpr int TOKENS = 128, LIST = 4096, MANY = 32;
+template <class T> __global__ __launch_bounds__(1024) void target_rows_kernel(const long long *targets, long long ignore, const float *left, const short *x,
+                                                                              long long ld, int M, int D, int v0, int v1, float *sums, int *slot) {
+    constexpr int WAVES = 16, PER = 4, STEP = PER * 1024;
+    static_assert(LIST >= STEP, "a step's rows fit");
+    __shared__ int row_of[LIST], first[TOKENS], many[TOKENS], before[PER * WAVES];
+    __shared__ unsigned char token_of[LIST];
+    __shared__ __attribute__((aligned(16))) float part[WAVES][512];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int e0 = v0 + blockIdx.x * TOKENS, ne = v1 - e0 < TOKENS ? v1 - e0 : TOKENS;
+    if (threadIdx.x < TOKENS) first[threadIdx.x] = -1, many[threadIdx.x] = 0;
+    // acc += left x of token e's rows, 8 elements a lane from c and C - 1 times 512 behind it, of the rows at from .. from + 63,
+    // from + step .. of the list's n; the first of these rows (the whole wave goes through them; lanes behind the row's end
+    // read its beginning, for nothing)
+    auto walk = [&](auto &acc, int e, int n, int from, int step, int c) __attribute__((always_inline)) {
+        constexpr int C = sizeof(acc) / sizeof(acc[0]), AT_ONCE = 4 / C;  // rows on their way
+        int d[C], row = -1;
+#pragma unroll
+        for (int h = 0; h < C; ++h) d[h] = c + h * 512 + lane * 8 < D ? c + h * 512 + lane * 8 : 0;
+        for (int p = from; p < n; p += step) {
+            unsigned long long mine = __builtin_amdgcn_ballot_w64(p + lane < n && token_of[p + lane < n ? p + lane : 0] == e);
+            while (mine) {
+                Vec<T> v[AT_ONCE][C];
+                float f[AT_ONCE];
+                int m = 0;
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i) {
+                    const bool there = mine != 0;
+                    if (there) m = __builtin_amdgcn_readfirstlane(row_of[p + __builtin_ctzll(mine)]);  // (else: the last one again, times 0)
+                    if (row < 0) row = m;
+                    mine &= mine - 1;
+                    f[i] = there ? left[m] : 0.f;
+#pragma unroll
+                    for (int h = 0; h < C; ++h) v[i][h] = *(const Vec<T> *)(x + (long long)m * ld + d[h]);
+                }
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+                    for (int h = 0; h < C; ++h)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) acc[h][k] = fmaf(f[i], (float)v[i][h].e[k], acc[h][k]);
+            }
+        }
+        return row;
+    };
+    auto put = [&](int m, bool more, int d, const float (&acc)[8]) __attribute__((always_inline)) {
+        float *to = sums + (long long)m * D + d;
+        if (d + 8 <= D) {
+#pragma unroll
+            for (int k = 0; k < 8; k += 4) {
+                Vec<float> v = {{acc[k], acc[k + 1], acc[k + 2], acc[k + 3]}};
+                if (more) {
+                    const Vec<float> u = *(const Vec<float> *)(to + k);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v.e[i] += u.e[i];
+                }
+                *(Vec<float> *)(to + k) = v;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (d + k < D) to[k] = more ? to[k] + acc[k] : acc[k];
+        }
+    };
+    auto add_up = [&](int n) {  // the n rows of the list
+        unsigned long long few[TOKENS / 64], lots[TOKENS / 64];  // tokens with rows in the list
+#pragma unroll
+        for (int b = 0; b < TOKENS / 64; ++b) {
+            const int count = many[b * 64 + lane];
+            few[b] = __builtin_amdgcn_ballot_w64(count > 0 && count <= MANY) & (0x0001000100010001ull << wave);  // (this wave's)
+            lots[b] = __builtin_amdgcn_ballot_w64(count > MANY);
+        }
+        static_assert(WAVES == 16 && TOKENS == 128, "every 16th token of two words");
+        auto next_of = [](unsigned long long (&set)[2]) __attribute__((always_inline)) {  // takes the first token out; -1: none
+            const int e = set[0] ? __builtin_ctzll(set[0]) : set[1] ? 64 + __builtin_ctzll(set[1]) : -1;
+            set[1] &= set[0] ? ~0ull : set[1] - 1;
+            set[0] &= set[0] - 1;
+            return e;
+        };
+        for (int e = next_of(few); e >= 0; e = next_of(few)) {
+            const int known = __builtin_amdgcn_readfirstlane(first[e]);
+            int m = known;
+            for (int c = 0; c < D; c += 1024) {
+                float acc[2][8] = {};
+                const int row = walk(acc, e, n, 0, 64, c);
+                if (m < 0) m = row;
+                put(m, known >= 0, c + lane * 8, acc[0]);
+                put(m, known >= 0, c + 512 + lane * 8, acc[1]);
+            }
+            if (lane == 0) first[e] = m;
+        }
+        for (int e = next_of(lots); e >= 0; e = next_of(lots)) {
+            const int known = __builtin_amdgcn_readfirstlane(first[e]);
+            int m = known;
+            for (int p = 0; m < 0; p += 64) {  // (there is one)
+                const unsigned long long mine = __builtin_amdgcn_ballot_w64(p + lane < n && token_of[p + lane < n ? p + lane : 0] == e);
+                if (mine) m = __builtin_amdgcn_readfirstlane(row_of[p + __builtin_ctzll(mine)]);
+            }
+            for (int c = 0; c < D; c += 512) {
+                float acc[1][8] = {};
+                walk(acc, e, n, wave * 64, 1024, c);
+                *(f32x4 *)&part[wave][lane * 8] = (f32x4){acc[0][0], acc[0][1], acc[0][2], acc[0][3]};
+                *(f32x4 *)&part[wave][lane * 8 + 4] = (f32x4){acc[0][4], acc[0][5], acc[0][6], acc[0][7]};
+                __syncthreads();
+                if (threadIdx.x < 512 && c + (int)threadIdx.x < D) {
+                    float v = 0.f;
+#pragma unroll
+                    for (int w = 0; w < WAVES; ++w) v += part[w][threadIdx.x];
+                    float *to = sums + (long long)m * D + c + threadIdx.x;
+                    *to = known >= 0 ? *to + v : v;
+                }
+                __syncthreads();
+            }
+            if (threadIdx.x == 0) first[e] = m;
+        }
+        __syncthreads();  // the list and the counts are no longer read
+        if (threadIdx.x < TOKENS) many[threadIdx.x] = 0;
+    };
+    int n = 0;
+    long long next[PER];
+    auto load = [&](int r) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const long long m = (long long)r + i * 1024 + threadIdx.x;
+            next[i] = m < M ? targets[m] : ignore;
+        }
+    };
+    load(0);
+    for (int r = 0; r < M; r += STEP) {
+        int token[PER], at[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const long long t = next[i];
+            token[i] = t != ignore && t >= e0 && t < e0 + ne ? (int)(t - e0) : -1;
+        }
+        if (r + STEP < M) load(r + STEP);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const unsigned long long found = __builtin_amdgcn_ballot_w64(token[i] >= 0);
+            at[i] = __popcll(found & ((1ull << lane) - 1));
+            if (lane == 0) before[i * WAVES + wave] = __popcll(found);
+        }
+        __syncthreads();
+        // how many were found before each of this wave's 64 (a lane a count: PER * WAVES of them)
+        static_assert(PER * WAVES == 64, "a lane a count");
+        const int count = before[lane];
+        int upto = count;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int u = __shfl_up(upto, o);
+            if (lane >= o) upto += u;
+        }
+        const int total = __shfl(upto, 63);
+        if (total) {  // (of the whole workgroup)
+            if (n + total > LIST) {
+                add_up(n);
+                n = 0;
+                __syncthreads();
+            }
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int from = __shfl(upto - count, i * WAVES + wave);
+                if (token[i] >= 0) {
+                    row_of[n + from + at[i]] = r + i * 1024 + threadIdx.x;
+                    token_of[n + from + at[i]] = token[i];
+                    atomicAdd(&many[token[i]], 1);  // (a count has no order)
+                }
+            }
+            n += total;
+        }
+        __syncthreads();  // the list is there, and the counts are no longer read
+    }
+    if (n) add_up(n);
+    __syncthreads();
+    if (threadIdx.x < ne) slot[e0 + threadIdx.x] = first[threadIdx.x];
+}
+// The targets' part of a product of dW (target_rows_kernel), slot: of its first token; null: none
+struct Targets {
+    const float *sums;
+    const int *slot;
+    int by_col;  // the vocabulary is the product's columns
+};
+
 struct SumArgs {  // C[z][i][j] = (or +=) the z-th part of the k-steps; pair: of rows 2 i and 2 i + 1 of A
     Operand A, B;
     int nk, per, ti, tj, I, J, add, pair;
@@ -550,7 +741,7 @@ struct OutArgs {  // C[i][j] * g_unit, in the elements' type
     const unsigned *gtop;
     void *out;
     long long ld;
-    int elem;
+    Targets more;
 };
 template <class C, bool KMAJOR, bool F16, int PLANES, int SCALED> __global__ __launch_bounds__(C::NT, C::OCC) void sum_kernel(const SumArgs a) {
     typedef Gemm<C, KMAJOR, F16, PLANES, SCALED> G;
@@ -603,7 +794,14 @@ template <class C, bool F16, int PLANES, int SCALED> __global__ __launch_bounds_
     tile_of(blockIdx.x, a.ti, a.tj, bi, bj);
     const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5, wave = threadIdx.x >> 6;
     const int wi0 = bi * C::BI + (wave / C::VJ) * (C::WI * 32), wj0 = bj * C::BJ + (wave % C::VJ) * (C::WJ * 32);
+    constexpr int ELEM = PLANES == 2 ? TSC_ELEM_F32 : F16 ? TSC_ELEM_F16 : TSC_ELEM_BF16;  // (a type that is asked for at every store costs more than the store)
     const float post = g_unit(a.gtop);
+    __shared__ int slots[PLANES == 1 ? (C::BI > C::BJ ? C::BI : C::BJ) : 1];  // of the tile's part of the vocabulary
+    if (PLANES == 1 && a.more.slot) {
+        const int at = a.more.by_col ? bj * C::BJ : bi * C::BI, n = a.more.by_col ? a.J : a.I;
+        for (int i = threadIdx.x; i < (a.more.by_col ? C::BJ : C::BI); i += C::NT) slots[i] = at + i < n ? a.more.slot[at + i] : -1;
+        __syncthreads();
+    }
     auto begin = [&](int, f32x16 (&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
 #pragma unroll
         for (int p = 0; p < C::WI; ++p)
@@ -612,14 +810,71 @@ template <class C, bool F16, int PLANES, int SCALED> __global__ __launch_bounds_
     };
     auto done = [&](int, f32x16 (&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
         const long long at = (long long)(wi0 + 4 * lh) * a.ld + wj0 + li;
+        auto put = [&](int p, int q, int r, float v) __attribute__((always_inline)) {
+            if (wi0 + p * 32 + block_row(r, lh) < a.I && wj0 + q * 32 + li < a.J)
+                write_elem(a.out, ELEM, at + (long long)(p * 32 + block_row(r, 0)) * a.ld + q * 32, v * post);
+        };
+        // The targets' part is added on the way out (sums that change in a branch are copied, and spilled): block by block, the
+        // next one's loads in front of a block's stores, behind which they would have to wait, and a row's blocks one after the other,
+        // so that the halves of a line leave together: 1999 x 1001 x 32003 136 us.
+        constexpr int N = C::WI * C::WJ, AHEAD = 2;
+        float v[AHEAD][16];
+        if (PLANES == 1 && a.more.slot && a.more.by_col) {
+            auto load = [&](int b) __attribute__((always_inline)) {
+                const int p = b / C::WJ, q = b % C::WJ, from = slots[wj0 - bj * C::BJ + q * 32 + li];
+                const float *s = a.more.sums + (long long)(from < 0 ? 0 : from) * a.I + wi0 + p * 32 + 4 * lh;
 #pragma unroll
-        for (int p = 0; p < C::WI; ++p)
+                for (int r = 0; r < 16; r += 4) {
+                    const int i = wi0 + p * 32 + block_row(r, lh);
+                    Vec<float> u = {};
+                    if (from >= 0 && i + 4 <= a.I) {
+                        u = *(const Vec<float> *)(s + block_row(r, 0));
+                    } else if (from >= 0) {
 #pragma unroll
-            for (int q = 0; q < C::WJ; ++q)
+                        for (int e = 0; e < 4; ++e)
+                            if (i + e < a.I) u.e[e] = s[block_row(r, 0) + e];
+                    }
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (wi0 + p * 32 + block_row(r, lh) < a.I && wj0 + q * 32 + li < a.J)
-                        write_elem(a.out, a.elem, at + (long long)(p * 32 + block_row(r, 0)) * a.ld + q * 32, acc[p][q][r] * post);
+                    for (int e = 0; e < 4; ++e) v[b % AHEAD][r + e] = u.e[e];
+                }
+            };
+#pragma unroll
+            for (int b = 0; b < AHEAD - 1; ++b) load(b);
+#pragma unroll
+            for (int b = 0; b < N; ++b) {
+                if (b + AHEAD - 1 < N) load(b + AHEAD - 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) put(b / C::WJ, b % C::WJ, r, acc[b / C::WJ][b % C::WJ][r] + v[b % AHEAD][r]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else if (PLANES == 1 && a.more.slot) {
+            auto load = [&](int b) __attribute__((always_inline)) {
+                const int p = b / C::WJ, j = wj0 + b % C::WJ * 32 + li;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int from = slots[wi0 - bi * C::BI + p * 32 + block_row(r, lh)];
+                    v[b % AHEAD][r] = from >= 0 && j < a.J ? a.more.sums[(long long)from * a.J + j] : 0.f;
+                }
+            };
+#pragma unroll
+            for (int b = 0; b < AHEAD - 1; ++b) load(b);
+#pragma unroll
+            for (int b = 0; b < N; ++b) {
+                if (b + AHEAD - 1 < N) load(b + AHEAD - 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) put(b / C::WJ, b % C::WJ, r, acc[b / C::WJ][b % C::WJ][r] + v[b % AHEAD][r]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+#pragma unroll
+            for (int p = 0; p < C::WI; ++p)
+#pragma unroll
+                for (int q = 0; q < C::WJ; ++q)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) put(p, q, r, acc[p][q][r]);
+        }
     };
     G::run(a.A, a.B, 1, [&](int) { return TileAt{bi * C::BI, bj * C::BJ}; }, 0, a.nk, lds, begin, done);
 }
@@ -653,12 +908,20 @@ template <bool SHARED> __device__ __forceinline__ bool sum_parts(const float *p,
     return true;
 }
 // C[i][j] = sum over z of part[z][i][j] times g_unit, 4 elements a lane: a dW whose k-steps were split
-template <bool SHARED> __global__ __launch_bounds__(256) void join_kernel(const float *part, int n, int I, int J, const unsigned *gtop, void *out,
-                                                                          long long ld, int elem) {
+template <bool SHARED> __global__ __launch_bounds__(256) void join_kernel(const float *part, int n, int I, int J, const Targets more, const unsigned *gtop,
+                                                                          void *out, long long ld, int elem) {
     __shared__ float red[3][256];
     const int i = blockIdx.x, j = SHARED ? blockIdx.y * 256 + (threadIdx.x & 63) * 4 : (blockIdx.y * 256 + threadIdx.x) * 4;
     float v[4];
     if (!sum_parts<SHARED>(part + (long long)i * J + j, n, (long long)I * J, J - j, red, v)) return;
+    if (more.slot) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (j + e < J) {
+                const int from = more.slot[more.by_col ? j + e : i];
+                if (from >= 0) v[e] += more.by_col ? more.sums[(long long)from * I + i] : more.sums[(long long)from * J + j + e];
+            }
+    }
     const float unit = g_unit(gtop);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -858,11 +1121,11 @@ Split split_of(long long I, long long J, int nk, int planes, bool always_parts) 
 struct Plan {
     int Mp;
     int copies;      // backward: rows of G a row (2: its remainder too), and of x
-    bool left_wanted;
+    bool left_wanted, targets_wanted;  // what 16 bits take of the targets' entries: kept; summed by token for dW
     Streams st;
     int Vc, pieces;  // backward: entries of a piece
     Split dx;        // of a whole piece
-    long long xp, xscale, part, hit, gtop, left, g, db, dxp, dwp, bytes;
+    long long xp, xscale, part, hit, gtop, left, sums, slot, g, db, dxp, dwp, bytes;
 };
 // dW of nv entries of the vocabulary: as many of them as fill whole rounds of the chip in one piece, the rest (or all of them,
 // where that is cheaper) with their k-steps split.
@@ -903,8 +1166,13 @@ Plan plan(const tsc_unembed *h, long long M, bool backward, bool want_x, bool wa
         p.hit = take(4 * M);
     } else {
         p.gtop = take(4);
-        p.left_wanted = want_x && h->planes == 1 && p.copies == 1;
+        p.left_wanted = (want_x || want_w) && h->planes == 1 && p.copies == 1;
+        p.targets_wanted = p.left_wanted && want_w;
         if (p.left_wanted) p.left = take(4 * M);
+        if (p.targets_wanted) {
+            p.sums = take(4ll * M * h->D);
+            p.slot = take(4ll * h->V);
+        }
         p.g = take(2ll * h->planes * rows * p.Vc);
         if (want_b) p.db = take(4ll * 2 * p.st.nm * p.Vc);  // (two parts a tile of rows, or one of twice the pitch)
         if (want_x) {
@@ -1079,6 +1347,14 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
         }
         if (dW) {
             const bool by_d = h->sv == 1;  // dW is dense in W's order: [D][V] or [V][D]
+            float *sums = (float *)(ws + p.sums);
+            int *slot = (int *)(ws + p.slot);
+            if (p.targets_wanted) {
+                auto launch = [&](auto *kernel) {
+                    hipLaunchKernelGGL(kernel, dim3(cdiv(nv, TOKENS)), dim3(1024), 0, s, targets, ignore, a.left, xp, xld, M, h->D, v0, v0 + nv, sums, slot);
+                };
+                f16 ? launch(target_rows_kernel<_Float16>) : launch(target_rows_kernel<__bf16>);
+            }
             const DwPlan parts = dw_plan(h, (long long)p.copies * p.Mp, nv);
             for (int i = 0, at = 0; i < 2 && parts.n[i]; at += parts.n[i++]) {
                 const Split &w = parts.w[i];
@@ -1086,11 +1362,12 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
                 const int I = by_d ? h->D : parts.n[i], J = by_d ? parts.n[i] : h->D;
                 const long long first = by_d ? v0 + at : (long long)(v0 + at) * h->D, ld = by_d ? h->V : h->D;
                 void *out = (char *)dW + first * (h->elem == TSC_ELEM_F32 ? 4 : 2);
+                const Targets more = {sums, p.targets_wanted ? slot + v0 + at : nullptr, by_d};
                 if (w.z == 1) {
                     OutArgs q{};
                     q.A = by_d ? X : Gk;
                     q.B = by_d ? Gk : X;
-                    q.nk = p.copies * p.Mp / BK; q.I = I; q.J = J; q.gtop = gtop; q.elem = h->elem; q.ld = ld; q.out = out;
+                    q.nk = p.copies * p.Mp / BK; q.I = I; q.J = J; q.gtop = gtop; q.ld = ld; q.out = out; q.more = more;
                     rc = launch_dw(w, h->elem, by_d, q, s);
                 } else {
                     SumArgs q{};
@@ -1099,8 +1376,8 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
                     q.nk = p.copies * p.Mp / BK; q.I = I; q.J = J; q.out = (float *)(ws + p.dwp);
                     rc = launch_dw_parts(w, h->elem, by_d, q, s);
                     if (!rc) {  // (many parts are of few elements: 63 of 311 x 137 25 us by single waves)
-                        if (w.z >= 8) hipLaunchKernelGGL((join_kernel<true>), dim3(I, cdiv(J, 256)), dim3(256), 0, s, q.out, w.z, I, J, gtop, out, ld, h->elem);
-                        else hipLaunchKernelGGL((join_kernel<false>), dim3(I, cdiv(J, 1024)), dim3(256), 0, s, q.out, w.z, I, J, gtop, out, ld, h->elem);
+                        if (w.z >= 8) hipLaunchKernelGGL((join_kernel<true>), dim3(I, cdiv(J, 256)), dim3(256), 0, s, q.out, w.z, I, J, more, gtop, out, ld, h->elem);
+                        else hipLaunchKernelGGL((join_kernel<false>), dim3(I, cdiv(J, 1024)), dim3(256), 0, s, q.out, w.z, I, J, more, gtop, out, ld, h->elem);
                     }
                 }
                 if (rc) return rc;
