@@ -441,8 +441,13 @@ int tsc_layer_norm_backward(int elem, const tsc_rows_t *dy, const tsc_rows_t *x,
  * The handle owns what the matrix pipe reads: W in both orders, padded, in 16 bits (an order that a 16-bit W has already, at
  * 16-byte alignment and with an inner axis that is a multiple of 64, is read in place) -- for TSC_ELEM_F32 as two fp16 planes
  * that hold 22 bits of every weight down to 2^-17 of the largest and a fixed 2^-39 of it below -- 2 x 77 MB (fp32: 2 x 154)
- * at 768 x 50257.  After an in-place change of W or bias call tsc_unembed_refresh, in order with the calls that use the
- * handle.  d_model <= 32768, d_vocab <= 2^20.  One handle may be used from several streams.
+ * at 768 x 50257.  After an in-place change of W or bias call tsc_unembed_refresh.  d_model <= 32768, d_vocab <= 2^20.
+ *
+ * Stream order: one handle may be used from several streams.  tsc_unembed_create and tsc_unembed_refresh ENQUEUE the layout
+ * on `stream` and return; a later call on another stream waits for it by itself (a captured one is refused with TSC_ERR_ARG
+ * while it still runs: synchronize before the capture).  What the caller orders is the change of W or bias, behind the calls
+ * that still read them and before the refresh; and a refresh behind the calls on other streams that still use the handle.  A
+ * refresh that was captured is ordered like the rest of its graph.
  */
 typedef struct tsc_unembed tsc_unembed_t;
 int tsc_unembed_create(tsc_unembed_t **out, int d_model, int d_vocab, int elem, const void *W, int64_t stride_d,

@@ -13,6 +13,7 @@
 // column t adds it times the row (target_rows_kernel).  Up to 64 rows of 16-bit elements, whose time is W's way from memory,
 // keep what the rounding took of all entries (rows 2 m: G_m, 2 m + 1: its remainder), and both products run over twice as many
 // rows.
+#include <mutex>
 #include <new>
 #include <type_traits>
 
@@ -994,7 +995,41 @@ struct tsc_unembed {
     long long wt_ld, wd_ld;
     bool own_t, own_d;
     float *bias32, *wscale;
+    mutable std::mutex lock;             // of what follows
+    hipEvent_t laid;                     // behind the last layout that was not captured
+    mutable bool pending;                // ... which may still run
 };
+
+namespace {
+
+bool capturing(hipStream_t s) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &st) == hipSuccess) return st != hipStreamCaptureStatusNone;
+    (void)hipGetLastError();
+    return false;
+}
+
+// Work on s comes after the layout, whichever stream that runs on.  A captured stream cannot wait for one outside the
+// capture: the layout has to be over by then.
+int after_layout(const tsc_unembed *h, hipStream_t s) {
+    std::lock_guard<std::mutex> own(h->lock);
+    if (!h->pending) return TSC_OK;
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;  // (asking for an event's state would end somebody's capture otherwise)
+    TSC_HIP_CHECK(hipThreadExchangeStreamCaptureMode(&mode));
+    const hipError_t e = hipEventQuery(h->laid);
+    TSC_HIP_CHECK(hipThreadExchangeStreamCaptureMode(&mode));
+    if (e == hipSuccess) {
+        h->pending = false;
+        return TSC_OK;
+    }
+    (void)hipGetLastError();
+    if (e != hipErrorNotReady) return tsc_fail(TSC_ERR_HIP, "hipEventQuery failed: %s", hipGetErrorString(e));
+    if (capturing(s)) return tsc_fail(TSC_ERR_ARG, "the unembedding is still being laid out: synchronize before the capture");
+    TSC_HIP_CHECK(hipStreamWaitEvent(s, h->laid, 0));
+    return TSC_OK;
+}
+
+}  // namespace
 
 // ------------------------------------------------------------------------------------------------ handle
 int tsc_unembed_destroy_(tsc_unembed *h) {
@@ -1003,6 +1038,7 @@ int tsc_unembed_destroy_(tsc_unembed *h) {
     if (h->own_d && h->Wd) (void)hipFree((void *)h->Wd);
     if (h->bias32) (void)hipFree(h->bias32);
     if (h->wscale) (void)hipFree(h->wscale);
+    if (h->laid) (void)hipEventDestroy(h->laid);
     delete h;
     return TSC_OK;
 }
@@ -1010,6 +1046,8 @@ int tsc_unembed_destroy_(tsc_unembed *h) {
 void tsc_unembed_shape_(const tsc_unembed *h, int *elem, int *D, int *V) { *elem = h->elem; *D = h->D; *V = h->V; }
 
 int tsc_unembed_refresh_(tsc_unembed *h, hipStream_t s) {
+    const int rc = after_layout(h, s);  // (two at once would meet in the scale)
+    if (rc) return rc;
     hipLaunchKernelGGL(bias_kernel, dim3(cdiv(h->Vb, 256)), dim3(256), 0, s, h->bias, h->belem, h->V, h->Vb, h->bias32);
     if (h->elem == TSC_ELEM_F32) {
         hipLaunchKernelGGL(fill_kernel, dim3(1), dim3(256), 0, s, h->wscale, 0.f, 1ll);
@@ -1025,6 +1063,10 @@ int tsc_unembed_refresh_(tsc_unembed *h, hipStream_t s) {
     if (h->own_t) pack(h->sv, h->sd, h->V, h->D, h->Dp, (short *)h->Wt);
     if (h->own_d) pack(h->sd, h->sv, h->D, h->V, h->Vp, (short *)h->Wd);
     TSC_HIP_CHECK(hipGetLastError());
+    if (capturing(s)) return TSC_OK;  // (nothing has been laid out yet)
+    std::lock_guard<std::mutex> own(h->lock);
+    TSC_HIP_CHECK(hipEventRecord(h->laid, s));
+    h->pending = true;
     return TSC_OK;
 }
 
@@ -1047,7 +1089,8 @@ int tsc_unembed_create_(tsc_unembed **out, int D, int V, int elem, const void *W
     else if (e == hipSuccess) e = hipMalloc((void **)&h->Wd, (size_t)D * h->planes * h->Vp * 2);
     if (e == hipSuccess) e = hipMalloc((void **)&h->bias32, (size_t)h->Vb * 4);
     if (e == hipSuccess) e = hipMalloc((void **)&h->wscale, 256);
-    int rc = e == hipSuccess ? tsc_unembed_refresh_(h, s) : tsc_fail(TSC_ERR_HIP, "hipMalloc of the unembedding's operands failed: %s", hipGetErrorString(e));
+    if (e == hipSuccess) e = hipEventCreateWithFlags(&h->laid, hipEventDisableTiming);
+    int rc = e == hipSuccess ? tsc_unembed_refresh_(h, s) : tsc_fail(TSC_ERR_HIP, "making the unembedding's operands failed: %s", hipGetErrorString(e));
     if (rc != TSC_OK) {
         tsc_unembed_destroy_(h);
         return rc;
@@ -1287,6 +1330,8 @@ size_t tsc_unembed_workspace_(const tsc_unembed *h, long long M, int backward, i
 
 int tsc_launch_unembed_loss(const tsc_unembed *h, const TscRows &x, int M, const long long *targets, long long ignore, float *loss,
                             float *lse, char *ws, hipStream_t s) {
+    const int ordered = after_layout(h, s);
+    if (ordered) return ordered;
     const Plan p = plan(h, M, false, false, false, false);
     LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
     const bool one_stride = x.inner_stride * x.inner == x.outer_stride;
@@ -1313,6 +1358,8 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
         TSC_HIP_CHECK(hipGetLastError());
         return TSC_OK;
     }
+    const int ordered = after_layout(h, s);
+    if (ordered) return ordered;
     const Plan p = plan(h, M, true, dx != nullptr, dW != nullptr, db != nullptr);
     short *xp = (short *)(ws + p.xp), *G = (short *)(ws + p.g);
     float *dxp = (float *)(ws + p.dxp);

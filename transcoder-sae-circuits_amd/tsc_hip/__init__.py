@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 from typing import Optional, Tuple
 
 import torch
@@ -1021,8 +1022,11 @@ class UnembedHead:
     Borrows both tensors and owns 16-bit copies of ``W_U`` in both orders, laid out at construction and again by
     :meth:`refresh`.  :meth:`loss` and :meth:`loss_backward` do that by themselves when torch's version counters say that a
     tensor was changed in place (inference tensors have none, and the replay of a graph that changes them does not count, nor does a
-    replayed call look: call :meth:`refresh` after the change).  Calls on several streams may run at once; one that lays out again is ordered with the others by
-    the caller, like the change itself."""
+    replayed call look: call :meth:`refresh` after the change).
+
+    Calls on several streams, also of several threads, may run at once.  A call waits for a layout that another stream is still
+    making, and a layout for the calls on other streams that came before it; what the caller orders is the change of the
+    tensors, as for any other reader of them.  A call that is captured while the layout still runs is refused."""
 
     def __init__(self, W_U: torch.Tensor, b_U: Optional[torch.Tensor] = None):
         self._handle = ctypes.c_void_p()
@@ -1043,6 +1047,7 @@ class UnembedHead:
                 raise TscError(f"b_U must be a contiguous [{self.d_vocab}] tensor of {W_U.dtype} or float32")
             _same_device(W_U.get_device(), b_U=b_U)
         self._by_d = sv == 1
+        self._lock, self._users = threading.RLock(), {}  # streams that used the last layout
         self._keep = [W_U] if b_U is None else [W_U, b_U]
         self.W_U, self.b_U, self.device, self.dtype = W_U, b_U, W_U.device, W_U.dtype
         with torch.cuda.device(self.device):
@@ -1057,13 +1062,34 @@ class UnembedHead:
         """Lay the weights out again (``tsc_unembed_refresh``).  Captured into a graph it is part of every replay."""
         if not self._handle:
             raise TscError("this UnembedHead is closed")
-        _launch(self.device.index, lib().tsc_unembed_refresh, self._handle)
-        if not torch.cuda.is_current_stream_capturing():  # (a captured one has laid out nothing yet)
-            self._versions = self._param_versions()
+        with self._lock, torch.cuda.device(self.device):
+            captured = torch.cuda.is_current_stream_capturing()
+            if not captured:
+                here = torch.cuda.current_stream()
+                for raw, stream in self._users.items():
+                    if raw != here.cuda_stream:
+                        here.wait_stream(stream)
+                self._users.clear()
+            versions = self._param_versions()
+            _launch(self.device.index, lib().tsc_unembed_refresh, self._handle)
+            if not captured:  # (a captured one has laid out nothing yet)
+                self._versions = versions
 
     def refresh_if_modified(self) -> None:
-        if self._param_versions() != self._versions:
-            self.refresh()
+        with self._lock:
+            if self._param_versions() != self._versions:
+                self.refresh()
+
+    def _use(self) -> None:
+        """Before a call that reads the layout: it is the tensors', and the next one waits for this stream."""
+        with self._lock:
+            self.refresh_if_modified()
+            i = self.device.index
+            raw = torch._C._cuda_getCurrentRawStream(i)
+            if raw not in self._users:
+                with torch.cuda.device(i):
+                    if not torch.cuda.is_current_stream_capturing():  # (replays are ordered by the caller)
+                        self._users[raw] = torch.cuda.current_stream()
 
     def close(self) -> None:
         if self._handle:
@@ -1097,7 +1123,7 @@ class UnembedHead:
         target is ``ignore_index``, NaN where it is outside the vocabulary otherwise) and the logarithm of its sum of
         exponentials, which :meth:`loss_backward` takes."""
         rows, m = self._operands(x, targets)
-        self.refresh_if_modified()
+        self._use()
         loss = torch.empty(targets.shape, dtype=torch.float32, device=self.device)
         lse = torch.empty_like(loss)
         ws, n = self._workspace(m, 0, 0, 0, 0)
@@ -1115,7 +1141,7 @@ class UnembedHead:
             if _dev(t, torch.float32, name).shape != targets.shape:
                 raise TscError(f"{name} must be {tuple(targets.shape)} (got {tuple(t.shape)})")
             _same_device(self.device.index, **{name: t})
-        self.refresh_if_modified()
+        self._use()
         dx = _dense_like(x) if want_x else None
         dW = None
         if want_weight:
