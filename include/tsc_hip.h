@@ -478,7 +478,8 @@ int tsc_unembed_loss(const tsc_unembed_t *head, const tsc_rows_t *x, int64_t row
  * target outside the vocabulary makes its row's dx and all of dW NaN.  G is made in pieces of the vocabulary (2 GiB of
  * workspace) and rounded to 16 bits as the operand of the two products (fp32: two planes, 22 bits down to 2^-28 of the
  * largest and a fixed 2^-50 of it below; fp16: 11 bits down to 2^-28, a fixed 2^-39 below; the largest: of |dloss|, for fp32
- * of |dloss| times the row's largest |x|); what that takes of the targets' entries is added to dx and dW all the same,
+ * of |dloss| times the row's largest |x|, so that the dx of a row 2^-28 below that loses bits; rows without elements are held
+ * like the largest); what that takes of the targets' entries is added to dx and dW all the same,
  * and of all entries for up to 64 rows of 16-bit elements.  dbias sums unrounded values.
  * Sums are fp32 in a fixed order: the same call gives the same bits.
  * workspace: tsc_unembed_workspace_bytes(head, rows, 1, dx != NULL, dW != NULL, dbias != NULL) bytes, 256-byte aligned.

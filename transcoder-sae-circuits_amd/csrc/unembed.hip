@@ -136,19 +136,22 @@ __device__ __forceinline__ long long row_at(const TscRows &r, long long row) {
 }
 
 // One wave a row, n rows one after the other: x[m] / s_m, pitch Dp, rows behind M (up to Mp) and rows without a loss zero; s_m
-// to xscale (fp32); `copies` of each row one after the other.  With gtop: it takes the largest |g_m| s_m, from which G is scaled (a maximum does not depend on the order
-// of the atomics; one a workgroup, only where it raises the value).
+// to xscale (fp32); `copies` of each row one after the other.  With gtop: it takes the largest |g_m| s_m, from which G is scaled (a
+// maximum does not depend on the order of the atomics; one a workgroup, only where it raises the value).  A row of fp32 without
+// elements has no scale (0 in xscale, see row_scale) and must not count as one of scale 1, 2^13 times that of common rows: its
+// |g_m| goes to gtop[1], which counts where there are no others.
 template <class T> __global__ __launch_bounds__(256) void pack_x_kernel(const TscRows x, int M, int Mp, int D, int Dp, int n, int copies, const long long *targets,
                                                                         long long ignore, const float *g, short *out, float *xscale, unsigned *gtop) {
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int VE = 16 / sizeof(T);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float most = 0.f;
+    float most[2] = {0.f, 0.f};
     for (int m = (blockIdx.x * 4 + wave) * n, end = m + n < Mp ? m + n : Mp; m < end; ++m) {
         short *o = out + (long long)m * (SPLIT ? 2 : copies) * Dp;
         const bool live = m < M && (!targets || targets[m] != ignore);
         const T *p = (const T *)x.data + (live ? row_at(x, m) : 0);
         float s = 1.f;
+        bool empty = false;
         auto load = [&](int d) __attribute__((always_inline)) {
             Vec<T> v;
             if (live && d + VE <= D) {
@@ -174,11 +177,15 @@ template <class T> __global__ __launch_bounds__(256) void pack_x_kernel(const Ts
             for (int d = (HELD * 64 + lane) * VE; d < D; d += 64 * VE) take(load(d));
             for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
             s = pow2_scale(top);
-            if (lane == 0 && m < M) xscale[m] = s;
+            empty = gtop && live && top == 0.f;
+            if (lane == 0 && m < M) xscale[m] = empty ? 0.f : s;
         }
         if (gtop && live) {
             const float v = fabsf(g[m] * s);
-            most = v < __builtin_inff() ? fmaxf(most, v) : most;
+            if (v < __builtin_inff()) {
+                if (empty) most[1] = fmaxf(most[1], v);
+                else most[0] = fmaxf(most[0], v);
+            }
         }
         const float inv = 1.f / s;
         auto store = [&](int d, const Vec<T> &v) __attribute__((always_inline)) {
@@ -204,17 +211,26 @@ template <class T> __global__ __launch_bounds__(256) void pack_x_kernel(const Ts
         for (int d = (HELD * 64 + lane) * VE; d < Dp; d += 64 * VE) store(d, load(d));
     }
     if (!gtop) return;
-    __shared__ float all[4];
-    if (lane == 0) all[wave] = most;
+    __shared__ float all[2][4];
+    if (lane == 0)
+        for (int i = 0; i < 2; ++i) all[i][wave] = most[i];
     __syncthreads();
-    if (threadIdx.x) return;
-    most = fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3]));
-    if (__float_as_uint(most) > __atomic_load_n(gtop, __ATOMIC_RELAXED)) atomicMax(gtop, __float_as_uint(most));
+    if (threadIdx.x >= (SPLIT ? 2 : 1)) return;
+    const float *a = all[threadIdx.x];
+    const unsigned top = __float_as_uint(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
+    if (top > __atomic_load_n(gtop + threadIdx.x, __ATOMIC_RELAXED)) atomicMax(gtop + threadIdx.x, top);
 }
 
 // G' = G s_m S in 16 bits: S is 1 for bf16, whose range is fp32's, and for the fp16 planes the power of two that keeps |G'| =
 // |g_m| s_m S |p - [v = t]| below 2^15.  This is 1 / S.
-__device__ __forceinline__ float g_unit(const unsigned *gtop) { return gtop ? pow2_scale(__uint_as_float(*gtop)) : 1.f; }
+__device__ __forceinline__ float g_unit(const unsigned *gtop) { return gtop ? pow2_scale(__uint_as_float(gtop[0] ? gtop[0] : gtop[1])) : 1.f; }
+// s_m of a row of x in the backward pass.  One without elements is 0 at any scale; it takes the power of two that brings |g_m| s_m
+// next to the largest of the others, so that its entries of G are held like theirs.
+__device__ __forceinline__ float row_scale(float s, const unsigned *gtop, float g) {
+    if (s > 0.f || !gtop[0] || !(fabsf(g) > 0.f) || !(fabsf(g) < __builtin_inff())) return s > 0.f ? s : 1.f;
+    const int e = (int)(__float_as_uint(__uint_as_float(gtop[0]) / fabsf(g)) >> 23);
+    return __uint_as_float((unsigned)(e < 1 ? 1 : e > 254 ? 254 : e) << 23);
+}
 
 // ------------------------------------------------------------------------------------------------ products
 // Tiles of a launch: workgroups b and b + 8 share an XCD, so each XCD gets a run of neighbouring tiles, and within a run
@@ -251,7 +267,7 @@ struct LogitArgs {
     float *hit;          // [M]
     // backward
     const float *lse, *g;    // of the rows: kept, and d(loss)
-    const unsigned *gtop;    // g_unit
+    const unsigned *gtop;    // g_unit, row_scale
     short *G;            // [Mp][PLANES * ldg]
     long long ldg;
     int rest;            // of a row's remainder behind the row (elements); FEW rows of 16-bit elements
@@ -392,11 +408,12 @@ template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::
         // rows without a loss: every exponential is 2^-inf = 0
         r_lse[i] = live ? a.lse[mc] * LOG2E : __builtin_inff();
         const bool known = t >= 0 && t < a.V;
-        r_f[i] = !live ? 0.f : known ? a.g[mc] * (SPLIT ? a.xscale[mc] : 1.f) * unit : __builtin_nanf("");
+        const float s = SPLIT ? row_scale(a.xscale[mc], a.gtop, a.g[mc]) : 1.f;
+        r_f[i] = !live ? 0.f : known ? a.g[mc] * s * unit : __builtin_nanf("");
         r_t[i] = live && known ? (int)t - a.v0 : -1;
         if (SPLIT) {
-            r_sc[i] = a.xscale[mc] * a.wscale[0] * LOG2E;
-            r_inv[i] = 1.f / a.xscale[mc];
+            r_sc[i] = a.xscale[mc] * a.wscale[0] * LOG2E;  // (0 for a row without elements, whose products are 0)
+            r_inv[i] = 1.f / s;
         }
     }
     __syncthreads();
@@ -931,8 +948,8 @@ template <bool SHARED> __global__ __launch_bounds__(256) void join_kernel(const 
 // dx[m][d] = sum over z, with the scales undone: 256 elements of a row a workgroup, whose waves share the parts, or a wave (few
 // parts, many rows: what takes the time is the way from a row's target to its row of W)
 template <bool SHARED> __global__ __launch_bounds__(256) void dx_kernel(const float *part, int n, int M, int D, const float *wscale, const float *xscale,
-                                                 const unsigned *gtop, const long long *targets, long long ignore, const float *left,
-                                                 const short *Wt, long long wt_ld, int V, int elem, void *dx) {
+                                                 const unsigned *gtop, const float *g, const long long *targets, long long ignore,
+                                                 const float *left, const short *Wt, long long wt_ld, int V, int elem, void *dx) {
     __shared__ float red[3][256];
     const int m = SHARED ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6), d = blockIdx.y * 256 + (threadIdx.x & 63) * 4;
     if (!SHARED && m >= M) return;
@@ -952,7 +969,7 @@ template <bool SHARED> __global__ __launch_bounds__(256) void dx_kernel(const fl
         }
     }
     if (!sum_parts<SHARED>(part + (long long)m * D + d, n, (long long)M * D, D - d, red, v)) return;
-    const float unit = g_unit(gtop), ws = wscale ? wscale[0] : 1.f, xs = wscale ? 1.f / xscale[m] : 1.f;
+    const float unit = g_unit(gtop), ws = wscale ? wscale[0] : 1.f, xs = wscale ? 1.f / row_scale(xscale[m], gtop, g[m]) : 1.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const float w = elem == TSC_ELEM_BF16 ? (float)__builtin_bit_cast(__bf16, u.e[e]) : (float)__builtin_bit_cast(_Float16, u.e[e]);
@@ -1208,7 +1225,7 @@ Plan plan(const tsc_unembed *h, long long M, bool backward, bool want_x, bool wa
         p.part = take(8ll * p.st.ns * M);
         p.hit = take(4 * M);
     } else {
-        p.gtop = take(4);
+        p.gtop = take(8);
         p.left_wanted = (want_x || want_w) && h->planes == 1 && p.copies == 1;
         p.targets_wanted = p.left_wanted && want_w;
         if (p.left_wanted) p.left = take(4 * M);
@@ -1364,7 +1381,7 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
     short *xp = (short *)(ws + p.xp), *G = (short *)(ws + p.g);
     float *dxp = (float *)(ws + p.dxp);
     unsigned *gtop = f16 ? (unsigned *)(ws + p.gtop) : nullptr;
-    if (gtop) hipLaunchKernelGGL(fill_kernel, dim3(1), dim3(256), 0, s, (float *)gtop, 0.f, 1ll);
+    if (gtop) hipLaunchKernelGGL(fill_kernel, dim3(1), dim3(256), 0, s, (float *)gtop, 0.f, 2ll);
     pack_x(h, p, x, M, targets, ignore, g, ws, gtop, s);
     LogitArgs a = logit_args(h, p, ws, M, targets, ignore);
     a.lse = lse; a.g = g; a.gtop = gtop; a.G = G; a.ldg = (long long)p.copies * p.Vc; a.rest = p.Vc;
@@ -1436,7 +1453,7 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
         const bool shared = p.dx.z >= 8;
         const dim3 grid(shared ? M : cdiv(M, 4), cdiv(h->D, 256));
         auto launch = [&](auto *kernel) {
-            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, dxp, p.dx.z, M, h->D, a.wscale, a.xscale, gtop, targets, ignore, a.left, h->Wt,
+            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, dxp, p.dx.z, M, h->D, a.wscale, a.xscale, gtop, g, targets, ignore, a.left, h->Wt,
                                h->wt_ld, h->V, h->elem, dx);
         };
         shared ? launch(dx_kernel<true>) : launch(dx_kernel<false>);
