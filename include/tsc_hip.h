@@ -445,7 +445,8 @@ int tsc_layer_norm_backward(int elem, const tsc_rows_t *dy, const tsc_rows_t *x,
  *
  * Stream order: one handle may be used from several streams.  tsc_unembed_create and tsc_unembed_refresh ENQUEUE the layout
  * on `stream` and return; a later call on another stream waits for it by itself (a captured one is refused with TSC_ERR_ARG
- * while it still runs: synchronize before the capture).  What the caller orders is the change of W or bias, behind the calls
+ * while it still runs: synchronize before the capture).  tsc_unembed_create inside a capture is refused (TSC_ERR_ARG); a
+ * graph that calls were captured into needs the handle for as long as it is replayed.  What the caller orders is the change of W or bias, behind the calls
  * that still read them and before the refresh; and a refresh behind the calls on other streams that still use the handle.  A
  * refresh that was captured is ordered like the rest of its graph.
  */

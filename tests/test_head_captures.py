@@ -1,0 +1,54 @@
+"""``UnembedHead`` and ``model_head`` around a capture: what cannot be captured is refused and leaves the capture whole."""
+import pytest
+import torch
+
+from test_lm_head import model_of, tokens_of
+from test_unembed import DEV, make
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_making_a_head_inside_a_capture_is_refused(dtype):
+    import tsc_hip
+
+    x, W, b, t, _ = make(20, 64, 300, dtype, seed=71)
+    some = torch.zeros(4, device=DEV)
+    for mode in ("global", "relaxed"):
+        some.zero_()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, capture_error_mode=mode):
+            some.add_(1)
+            with pytest.raises(tsc_hip.TscError, match="capture"):
+                tsc_hip.UnembedHead(W, b)
+            some.add_(1)
+        for k in range(3):
+            g.replay()
+            torch.cuda.synchronize()
+            assert some.eq(2 * (k + 1)).all()
+    head = tsc_hip.UnembedHead(W, b)
+    assert torch.equal(head.loss(x, t)[0], tsc_hip.UnembedHead(W, b).loss(x, t)[0])
+
+
+@pytest.mark.gpu
+def test_a_model_without_a_head_is_not_captured():
+    import tsc_hip
+
+    m = model_of(DEV)
+    tok = tokens_of(m)
+    final = m.run_with_cache(tok)[1]["ln_final.hook_normalized"].clone()
+    import lm_head
+
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        final.add_(0.0)
+        with pytest.raises(tsc_hip.TscError, match="capture"):
+            lm_head.next_token_loss(final, tok, lm_head.model_head(m))
+    want = lm_head.next_token_loss(final, tok, lm_head.model_head(m))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = lm_head.next_token_loss(final, tok, lm_head.model_head(m))
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)

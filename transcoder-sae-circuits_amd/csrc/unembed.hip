@@ -1088,6 +1088,7 @@ int tsc_unembed_refresh_(tsc_unembed *h, hipStream_t s) {
 }
 
 int tsc_unembed_create_(tsc_unembed **out, int D, int V, int elem, const void *W, long long sd, long long sv, const void *bias, int belem, hipStream_t s) {
+    if (capturing(s)) return tsc_fail(TSC_ERR_ARG, "an unembedding cannot be made inside a capture: make it before");
     tsc_unembed *h = new (std::nothrow) tsc_unembed();
     if (!h) return tsc_fail(TSC_ERR_HIP, "out of host memory");
     h->D = D; h->V = V; h->elem = elem; h->belem = belem; h->planes = elem == TSC_ELEM_F32 ? 2 : 1;

@@ -1026,7 +1026,8 @@ class UnembedHead:
 
     Calls on several streams, also of several threads, may run at once.  A call waits for a layout that another stream is still
     making, and a layout for the calls on other streams that came before it; what the caller orders is the change of the
-    tensors, as for any other reader of them.  A call that is captured while the layout still runs is refused."""
+    tensors, as for any other reader of them.  A call that is captured while the layout still runs is refused, and so is making a head
+    inside a capture; a graph needs the heads that were captured into it for as long as it is replayed."""
 
     def __init__(self, W_U: torch.Tensor, b_U: Optional[torch.Tensor] = None):
         self._handle = ctypes.c_void_p()
