@@ -32,6 +32,25 @@ def test_making_a_head_inside_a_capture_is_refused(dtype):
 
 
 @pytest.mark.gpu
+def test_a_head_dropped_inside_a_capture_leaves_it_whole():
+    import tsc_hip
+
+    x, W, b, t, _ = make(20, 64, 300, torch.float32, seed=72)
+    keep, drop = tsc_hip.UnembedHead(W, b), tsc_hip.UnembedHead(W, b)
+    want = keep.loss(x, t)[0]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        first = keep.loss(x, t)[0]
+        drop.close()
+        second = keep.loss(x, t)[0]
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and torch.equal(second, want)
+
+
+@pytest.mark.gpu
 def test_a_model_without_a_head_is_not_captured():
     import tsc_hip
 

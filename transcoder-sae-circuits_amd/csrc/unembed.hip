@@ -1051,11 +1051,14 @@ int after_layout(const tsc_unembed *h, hipStream_t s) {
 // ------------------------------------------------------------------------------------------------ handle
 int tsc_unembed_destroy_(tsc_unembed *h) {
     if (!h) return TSC_OK;
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;  // (a handle may be dropped while somebody captures)
+    const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
     if (h->own_t && h->Wt) (void)hipFree((void *)h->Wt);
     if (h->own_d && h->Wd) (void)hipFree((void *)h->Wd);
     if (h->bias32) (void)hipFree(h->bias32);
     if (h->wscale) (void)hipFree(h->wscale);
     if (h->laid) (void)hipEventDestroy(h->laid);
+    if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
     delete h;
     return TSC_OK;
 }
