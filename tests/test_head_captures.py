@@ -1,4 +1,5 @@
-"""``UnembedHead`` and ``model_head`` around a capture: what cannot be captured is refused and leaves the capture whole."""
+"""``UnembedHead`` and ``model_head`` around a capture: what cannot be captured is refused and leaves the capture whole; what is
+captured stays valid for as long as the model lives."""
 import pytest
 import torch
 
@@ -71,3 +72,31 @@ def test_a_model_without_a_head_is_not_captured():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_a_captured_loss_outlives_the_models_tensors():
+    """A graph of a model's loss is replayed after the model got other weights (and a head of them): the captured weights, which
+    the caller still has, are what it reads, through the layout that was made of them."""
+    import lm_head
+
+    m = model_of(DEV)
+    tok = tokens_of(m)
+    final = m.run_with_cache(tok)[1]["ln_final.hook_normalized"].clone()
+    want = lm_head.next_token_loss(final, tok, lm_head.model_head(m)).clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = lm_head.next_token_loss(final, tok, lm_head.model_head(m))
+    first = m.W_U
+    for k in range(3):
+        m.W_U = first * (k + 2.0)
+        other = lm_head.next_token_loss(final, tok, lm_head.model_head(m))
+        assert len(lm_head._captured[m]) == 1 and lm_head._heads[m][1] not in lm_head._captured[m]
+        assert all(h._handle for h in lm_head._captured[m])
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and not torch.equal(got, other)
+    models = len(lm_head._captured)
+    del g
+    del m, first
+    assert len(lm_head._captured) == models - 1
