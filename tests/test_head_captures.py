@@ -1,9 +1,9 @@
 """``UnembedHead`` and ``model_head`` around a capture: what cannot be captured is refused and leaves the capture whole; what is
-captured stays valid for as long as the model lives."""
+captured stays valid for as long as the model lives, and a pass captures one layout at most."""
 import pytest
 import torch
 
-from test_lm_head import model_of, tokens_of
+from test_lm_head import leaves, model_of, tokens_of
 from test_unembed import DEV, make
 
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -100,3 +100,51 @@ def test_a_captured_loss_outlives_the_models_tensors():
     del g
     del m, first
     assert len(lm_head._captured) == models - 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("learning", [True, False])
+def test_a_captured_pass_lays_out_once(learning, dtype, monkeypatch):
+    """After a change of the weights: of weights that learn the capture takes one layout, of frozen ones the one that their change
+    asks for; replays with changes between them give what eager passes give."""
+    import lm_head
+    import tsc_hip
+
+    x, w, b, W, bu, t = leaves(34, 64, 700, dtype, seed=73)
+    if not learning:
+        W, bu = W.detach(), bu.detach()
+    ps = [w, b] + ([W, bu] if learning else [])
+    head = tsc_hip.UnembedHead(W, bu)
+
+    def grads():
+        loss = lm_head.unembed_loss(lm_head.layer_norm(x, w, b), t, head)
+        return (loss.detach(),) + torch.autograd.grad(loss, [x] + ps)
+
+    def change(k):
+        with torch.no_grad():
+            W.mul_(k)
+            bu.add_(k - 1)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grads()
+        change(1.25)
+    torch.cuda.current_stream().wait_stream(side)
+    layouts = []
+    refresh = tsc_hip.UnembedHead.refresh
+    monkeypatch.setattr(tsc_hip.UnembedHead, "refresh", lambda self: (layouts.append(self), refresh(self))[1])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = grads()
+    assert layouts == [head]
+    monkeypatch.undo()
+    for k in (1.0, 0.75, 1.5):
+        change(k)
+        g.replay()
+        torch.cuda.synchronize()
+        kept = [q.clone() for q in got]
+        want = grads()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(kept, want)) and all(torch.equal(p, q) for p, q in zip(got, want))

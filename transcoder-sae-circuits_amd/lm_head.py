@@ -81,9 +81,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
 class _UnembedLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, W_U, b_U, targets, head, ignore_index):
-        loss, lse = head.loss(x, targets, ignore_index)
-        # (the weights are saved for their version: a change in place between the two passes is an error, not a wrong gradient)
+    def forward(ctx, x, W_U, b_U, targets, head, ignore_index, laid_out):
+        loss, lse = head._loss(x, targets, ignore_index, laid_out)
+        # (the weights are saved for their version: a change in place between the two passes is an error, not a wrong gradient;
+        # so the backward pass finds the forward pass' layout, which in a capture only the forward pass has captured)
         ctx.save_for_backward(x, W_U, b_U, targets, lse)
         ctx.head, ctx.ignore_index = head, ignore_index
         return loss
@@ -93,9 +94,9 @@ class _UnembedLoss(torch.autograd.Function):
     def backward(ctx, dloss):
         x, _, _, targets, lse = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx, dw, db = ctx.head.loss_backward(dloss.contiguous(), x, targets, lse, ctx.ignore_index, want_x=need_x,
-                                            want_weight=need_w, want_bias=need_b)
-        return dx, dw, db, None, None, None
+        dx, dw, db = ctx.head._loss_backward(dloss.contiguous(), x, targets, lse, ctx.ignore_index, need_x, need_w, need_b,
+                                             laid_out=True)
+        return dx, dw, db, None, None, None, None
 
 
 def _total(v: torch.Tensor) -> torch.Tensor:
@@ -115,6 +116,7 @@ def unembed_loss(x: torch.Tensor, targets: torch.Tensor, head: "tsc_hip.UnembedH
     ``"mean"`` -- over the rows whose target is not ``ignore_index`` (NaN where there are none)."""
     if reduction not in ("none", "sum", "mean"):
         raise tsc_hip.TscError(f"reduction must be 'none', 'sum' or 'mean' (got {reduction!r})")
+    laid_out = False
     if torch.is_grad_enabled():
         held = _mark_leaves(x, head.W_U, head.b_U)  # noqa: F841
         learning = [p for p in (head.W_U, head.b_U) if p is not None and p.requires_grad]
@@ -123,7 +125,8 @@ def unembed_loss(x: torch.Tensor, targets: torch.Tensor, head: "tsc_hip.UnembedH
                 raise tsc_hip.TscError("the head's W_U or b_U is a view of the leaf that learns, made before the capture: its "
                                        "accumulator may belong to another stream; make the head of leaves, or step eagerly")
             head.refresh()  # part of the graph: a replay finds the weights that the step before it left
-    rows = _UnembedLoss.apply(x, head.W_U, head.b_U, targets, head, ignore_index)
+            laid_out = True
+    rows = _UnembedLoss.apply(x, head.W_U, head.b_U, targets, head, ignore_index, laid_out)
     if reduction == "none":
         return rows
     total = _total(rows)

@@ -1081,10 +1081,12 @@ class UnembedHead:
             if self._param_versions() != self._versions:
                 self.refresh()
 
-    def _use(self) -> None:
-        """Before a call that reads the layout: it is the tensors', and the next one waits for this stream."""
+    def _use(self, laid_out: bool = False) -> None:
+        """Before a call that reads the layout: it is the tensors' (the caller says so, or it is made again), and the next one
+        waits for this stream."""
         with self._lock:
-            self.refresh_if_modified()
+            if not laid_out:
+                self.refresh_if_modified()
             i = self.device.index
             raw = torch._C._cuda_getCurrentRawStream(i)
             if raw not in self._users:
@@ -1123,8 +1125,11 @@ class UnembedHead:
         contiguous): every row's cross entropy (0 where the
         target is ``ignore_index``, NaN where it is outside the vocabulary otherwise) and the logarithm of its sum of
         exponentials, which :meth:`loss_backward` takes."""
+        return self._loss(x, targets, ignore_index)
+
+    def _loss(self, x, targets, ignore_index, laid_out=False):
         rows, m = self._operands(x, targets)
-        self._use()
+        self._use(laid_out)
         loss = torch.empty(targets.shape, dtype=torch.float32, device=self.device)
         lse = torch.empty_like(loss)
         ws, n = self._workspace(m, 0, 0, 0, 0)
@@ -1137,12 +1142,15 @@ class UnembedHead:
         """``tsc_unembed_loss_backward``: ``(dx, dW, db)`` for the gradient ``dloss`` (float32, ``x.shape[:-1]``, contiguous) of the rows'
         losses, None where not wanted (``db`` also without ``b_U``).  ``dx`` and ``dW`` have x's type, ``dW`` the shape and
         the order of ``W_U``, ``db`` the type of ``b_U``."""
+        return self._loss_backward(dloss, x, targets, lse, ignore_index, want_x, want_weight, want_bias)
+
+    def _loss_backward(self, dloss, x, targets, lse, ignore_index, want_x, want_weight, want_bias, laid_out=False):
         rows, m = self._operands(x, targets)
         for name, t in (("dloss", dloss), ("lse", lse)):
             if _dev(t, torch.float32, name).shape != targets.shape:
                 raise TscError(f"{name} must be {tuple(targets.shape)} (got {tuple(t.shape)})")
             _same_device(self.device.index, **{name: t})
-        self._use()
+        self._use(laid_out)
         dx = _dense_like(x) if want_x else None
         dW = None
         if want_weight:
