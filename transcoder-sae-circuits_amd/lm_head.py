@@ -139,12 +139,15 @@ _captured: "weakref.WeakKeyDictionary" = weakref.WeakKeyDictionary()  # model ->
 
 def model_head(model) -> "tsc_hip.UnembedHead":
     """The :class:`tsc_hip.UnembedHead` of ``model.W_U`` and ``model.b_U``, laid out once for as long as the model keeps these
-    tensors (a change in place lays it out again).  A capture needs one that is there already; a head that was asked for inside
+    tensors (a change in place lays it out again; inference tensors do not tell of one, so a model of them lays out for every
+    call).  A capture needs one that is there already; a head that was asked for inside
     a capture lives as long as the model, whatever tensors the model gets, because a graph may hold it."""
     key = tuple((t.data_ptr(), t.dtype, t.shape, t.stride()) for t in (model.W_U, model.b_U))
     entry = _heads.get(model)
     if entry is None or entry[0] != key:
         entry = _heads[model] = (key, tsc_hip.UnembedHead(model.W_U.detach(), model.b_U.detach()))
+    elif model.W_U.is_inference() or model.b_U.is_inference():
+        entry[1].refresh()
     if torch.cuda.is_current_stream_capturing():
         _captured.setdefault(model, set()).add(entry[1])
     return entry[1]
