@@ -991,9 +991,8 @@ __global__ __launch_bounds__(1024) void dbias_kernel(const float *part, int n, l
     for (int i = 1; i < 16; ++i) v += red[i][c];
     write_elem(out, elem, at + j, v * g_unit(gtop));
 }
-__global__ void zero_elem_kernel(void *p, int elem, long long n) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) write_elem(p, elem, i, 0.f);
+__global__ void zero_elem_kernel(void *p, int elem, long long n) {  // (a launch holds fewer than 2^32 threads, dW up to 2^35 elements)
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) write_elem(p, elem, i, 0.f);
 }
 
 inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -1374,8 +1373,11 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
                                 const float *lse, void *dx, void *dW, void *db, char *ws, hipStream_t s) {
     const bool f16 = h->elem != TSC_ELEM_BF16;
     if (M == 0) {
-        if (dW) hipLaunchKernelGGL(zero_elem_kernel, dim3(cdiv((long long)h->D * h->V, 256)), dim3(256), 0, s, dW, h->elem, (long long)h->D * h->V);
-        if (db) hipLaunchKernelGGL(zero_elem_kernel, dim3(cdiv(h->V, 256)), dim3(256), 0, s, db, h->belem, (long long)h->V);
+        auto zero = [&](void *p, int elem, long long n) {
+            hipLaunchKernelGGL(zero_elem_kernel, dim3((int)(n < 1 << 24 ? cdiv(n, 256) : 1 << 16)), dim3(256), 0, s, p, elem, n);
+        };
+        if (dW) zero(dW, h->elem, (long long)h->D * h->V);
+        if (db) zero(db, h->belem, h->V);
         TSC_HIP_CHECK(hipGetLastError());
         return TSC_OK;
     }
