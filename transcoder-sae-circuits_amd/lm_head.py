@@ -23,6 +23,7 @@ from torch.autograd.graph import get_gradient_edge
 import tsc_hip
 
 _MARK = "tsc_eager_stream"
+_FINAL = "ln_final.hook_normalized"
 
 
 def _mark_leaves(*tensors) -> list:
@@ -158,3 +159,28 @@ def next_token_loss(normalized: torch.Tensor, tokens: torch.Tensor, head: "tsc_h
     """A model's training loss from its final normalised residual ``[batch, n, d_model]``: the cross entropy of token
     ``t + 1`` at position ``t``, as mean or ``[batch, n - 1]`` (padding counts like any token)."""
     return unembed_loss(normalized[:, :-1], tokens[:, 1:].contiguous(), head, reduction="none" if per_token else "mean")
+
+
+def hooked_loss(model, tokens: torch.Tensor, fwd_hooks) -> torch.Tensor:
+    """Mean next-token loss of a hooked model under ``fwd_hooks``: ``model.run_with_hooks(tokens, return_type="loss", ...)``, on a
+    GPU from the final normalised residual (``ln_final.hook_normalized``) and :func:`model_head`, so that the model makes no
+    ``[batch, n, d_vocab]`` logits.  A model whose head is more than that -- a final norm with a weight of its own (not folded),
+    capped logits, a loss that leaves out left padding, a type that the operator does not take -- computes its own loss."""
+
+    def own():
+        return model.run_with_hooks(tokens, return_type="loss", fwd_hooks=fwd_hooks)
+
+    W, b, cfg = getattr(model, "W_U", None), getattr(model, "b_U", None), getattr(model, "cfg", None)
+    if not all(isinstance(t, torch.Tensor) for t in (W, b, tokens)) or not W.is_cuda or W.device != b.device or tokens.dim() > 2:
+        return own()
+    if W.dtype not in (torch.float32, torch.bfloat16, torch.float16) or b.dtype not in (W.dtype, torch.float32):
+        return own()
+    if (getattr(getattr(model, "ln_final", None), "w", None) is not None or (getattr(cfg, "output_logits_soft_cap", None) or 0) > 0
+            or getattr(getattr(model, "tokenizer", None), "padding_side", None) == "left"
+            or _FINAL not in getattr(model, "hook_dict", (_FINAL,))):
+        return own()
+    seen = []
+    model.run_with_hooks(tokens, return_type=None, fwd_hooks=list(fwd_hooks) + [(_FINAL, lambda act, hook: seen.append(act))])
+    if len(seen) != 1 or seen[0].dtype != W.dtype or seen[0].device != W.device:
+        return own()
+    return next_token_loss(seen[0], torch.atleast_2d(tokens).to(W.device, torch.int64), model_head(model))

@@ -17,6 +17,7 @@ from torch import nn
 
 import tsc_hip
 from _dictionary import HipDictionaryMixin, HookPoint
+from lm_head import hooked_loss
 
 
 class SparseTranscoder(HipDictionaryMixin, nn.Module):
@@ -116,7 +117,7 @@ class SparseTranscoder(HipDictionaryMixin, nn.Module):
 
             hooks = [(self.cfg.hook_point, read),
                      (f"blocks.{self.cfg.hook_point_layer}.hook_mlp_out", lambda act, hook: reconstruct(seen["in"]))]
-        return model.run_with_hooks(batch_tokens, return_type="loss", fwd_hooks=hooks)
+        return hooked_loss(model, batch_tokens, hooks)
 
     # ------------------------------------------------------------------ loaders (local files only)
     @classmethod

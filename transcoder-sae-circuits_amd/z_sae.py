@@ -12,6 +12,7 @@ from torch import nn
 
 from _dictionary import HipDictionaryMixin
 from dtypes import DTYPES
+from lm_head import hooked_loss
 
 # layer -> run name on the HF hub (reference :10-23).  Entry 10 names an L0 run there too; kept
 # as found because it decides which weights a user of the reference actually gets.
@@ -88,7 +89,7 @@ class ZSAE(HipDictionaryMixin, nn.Module):
         def replace(z, hook):
             return self.forward(z.reshape(-1, self.W_enc.shape[0]))[1].to(z.dtype).reshape(z.shape)
 
-        return model.run_with_hooks(batch_tokens, return_type="loss", fwd_hooks=[(f"blocks.{layer}.attn.hook_z", replace)])
+        return hooked_loss(model, batch_tokens, [(f"blocks.{layer}.attn.hook_z", replace)])
 
     @classmethod
     def load_from_files(cls, cfg_json: str, weights_pt: str, device=None):
