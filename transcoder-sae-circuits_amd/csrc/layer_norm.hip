@@ -251,9 +251,11 @@ template <class T, int NV, int TPR, int NT> __global__ __launch_bounds__(NT) voi
 }
 
 // The row's elements stay as they were read and are widened in each of the two passes, and the weight lies in LDS (its place
-// is needed for the sums only at the end), so that 16 waves a CU keep their rows and sums in registers.
+// is needed for the sums only at the end), so that 16 waves a CU keep their rows and sums in registers.  At 16 elements a thread
+// one or two of them do not fit: they are stored once and read back behind the rows, in the loop over them only for fp16 rows of
+// more than 8192 elements (15 registers) and fp32 rows of more than 12288 (one).
 // Measured: 65536 x 768 fp32 125 us = 4.8 TB/s, bf16 80 us = 3.8 TB/s; 16384 x 768 fp32 27 us and 4 for the sums' last step;
-// 1021 x 4099 bf16 16 us.  Reading the next row ahead, as the forward pass does, changed nothing (and spills with two vectors).
+// 1021 x 4099 bf16 16 us.  Reading the next row ahead, as the forward pass does, changed nothing (and spills more with two vectors).
 template <class T, int NV, int TPR, int NT> __global__ __launch_bounds__(NT) void ln_backward_kernel(const LnArgs a) {
     typedef RowEnd<T, NV, TPR> R;
     constexpr int N = NV * R::VE, GROUPS = NT / TPR;

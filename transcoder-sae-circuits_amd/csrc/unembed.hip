@@ -280,7 +280,8 @@ struct LogitArgs {
 // tile of the vocabulary for one block of rows.  The first tile's maximum becomes the row's reference; from then on a tile
 // costs an fma, an exponential and an add an element: sums of 2^(l - reference) are exact enough whatever the later maxima
 // are, as long as nothing overflows (the tile is then repeated with its own maximum) -- what underflows is below 2^-126 of a
-// term that is already in the sum.
+// term that is already in the sum.  (fp32 at LARGE: 13 registers do not fit; the loop over k touches none of them, a tile's end
+// reads eight back.)
 template <class C, bool F16, bool SPLIT> __global__ __launch_bounds__(C::NT, C::OCC) void loss_logits_kernel(const LogitArgs a) {
     typedef Gemm<C, false, F16, SPLIT ? 2 : 1> G;
     __shared__ __attribute__((aligned(16))) char lds[G::LDS_BYTES];
