@@ -85,3 +85,15 @@ def test_error_of_the_whole_is_the_results_rounding(dtype):
     got = float((dW - want).norm() / want.norm())
     # (the two are independent; 1.05: the second one's terms are taken as uncorrelated, 128 x 8001 of them)
     assert got <= 1.05 * math.hypot(own, others) + 2.0 ** -20, (got, own, others)
+
+
+@pytest.mark.gpu
+def test_workspace_of_more_rows_than_tokens():
+    """The sums are kept by token then: a further row costs its 16-bit copy, its row of G and some numbers, not 4 D bytes more."""
+    import tsc_hip
+
+    D, V = 512, 300
+    head = tsc_hip.UnembedHead(torch.zeros(D, V, dtype=torch.bfloat16, device=DEV))
+    size = [tsc_hip.lib().tsc_unembed_workspace_bytes(head._handle, m, 1, 0, 1, 0) for m in (100_000, 200_000)]
+    parts = 128 * 4 * D * V  # of a split dW, at most
+    assert size[1] - size[0] <= 100_000 * (2 * D + 2 * 512 + 16) + parts < 100_000 * (2 * D + 2 * 512 + 4 * D)

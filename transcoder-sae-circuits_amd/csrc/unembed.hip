@@ -559,15 +559,15 @@ template <bool LANE> __global__ __launch_bounds__(256) void loss_kernel(const fl
     loss[m] = t == ignore ? 0.f : t < 0 || t >= V ? __builtin_nanf("") : l - h;
 }
 
-// What G's rounding took of the targets' entries, for dW: sums[m][d] = sum of left[k] x[k][d] over the rows k whose target is
-// row m's, for the first row m of every one of the tokens v0 .. v1 - 1 that has a row, and slot[v] = that row, -1 where v has
-// none.  A workgroup looks through the targets for those among its TOKENS tokens and keeps their rows in order, so that every
+// What G's rounding took of the targets' entries, for dW: sums[slot[v]][d] = sum of left[m] x[m][d] over the rows m whose target
+// is v, for every one of the tokens v0 .. v1 - 1 that has a row; slot[v] is the first of them, or v itself (BY_TOKEN: of more
+// rows than tokens), and -1 where v has none.  A workgroup looks through the targets for those among its TOKENS tokens and keeps their rows in order, so that every
 // sum has a fixed order; where the list could overflow it is added up first, and the next one goes on from there.  A wave takes
 // the rows of a token one after the other, all waves together those of a token that has many, and join what they have.
 // Bound by latency (a target's way from memory, a row's, the sums' back).  Measured: 16384 rows x 768 of
 // 50257 tokens 47 us, 1999 x 1001 of 32003 11 us.
 constexpr int TOKENS = 128, LIST = 4096, MANY = 32;
-template <class T> __global__ __launch_bounds__(1024) void target_rows_kernel(const long long *targets, long long ignore, const float *left, const short *x,
+template <class T, bool BY_TOKEN> __global__ __launch_bounds__(1024) void target_rows_kernel(const long long *targets, long long ignore, const float *left, const short *x,
                                                                               long long ld, int M, int D, int v0, int v1, float *sums, int *slot) {
     constexpr int WAVES = 16, PER = 4, STEP = PER * 1024;
     static_assert(LIST >= STEP, "a step's rows fit");
@@ -651,7 +651,7 @@ template <class T> __global__ __launch_bounds__(1024) void target_rows_kernel(co
             for (int c = 0; c < D; c += 1024) {
                 float acc[2][8] = {};
                 const int row = walk(acc, e, n, 0, 64, c);
-                if (m < 0) m = row;
+                if (m < 0) m = BY_TOKEN ? e0 + e : row;
                 put(m, known >= 0, c + lane * 8, acc[0]);
                 put(m, known >= 0, c + 512 + lane * 8, acc[1]);
             }
@@ -659,7 +659,7 @@ template <class T> __global__ __launch_bounds__(1024) void target_rows_kernel(co
         }
         for (int e = next_of(lots); e >= 0; e = next_of(lots)) {
             const int known = __builtin_amdgcn_readfirstlane(first[e]);
-            int m = known;
+            int m = BY_TOKEN ? e0 + e : known;
             for (int p = 0; m < 0; p += 64) {  // (there is one)
                 const unsigned long long mine = __builtin_amdgcn_ballot_w64(p + lane < n && token_of[p + lane < n ? p + lane : 0] == e);
                 if (mine) m = __builtin_amdgcn_readfirstlane(row_of[p + __builtin_ctzll(mine)]);
@@ -1234,7 +1234,7 @@ Plan plan(const tsc_unembed *h, long long M, bool backward, bool want_x, bool wa
         p.targets_wanted = p.left_wanted && want_w;
         if (p.left_wanted) p.left = take(4 * M);
         if (p.targets_wanted) {
-            p.sums = take(4ll * M * h->D);
+            p.sums = take(4ll * (M < h->V ? M : h->V) * h->D);
             p.slot = take(4ll * h->V);
         }
         p.g = take(2ll * h->planes * rows * p.Vc);
@@ -1424,7 +1424,8 @@ int tsc_launch_unembed_backward(const tsc_unembed *h, const float *g, const TscR
                 auto launch = [&](auto *kernel) {
                     hipLaunchKernelGGL(kernel, dim3(cdiv(nv, TOKENS)), dim3(1024), 0, s, targets, ignore, a.left, xp, xld, M, h->D, v0, v0 + nv, sums, slot);
                 };
-                f16 ? launch(target_rows_kernel<_Float16>) : launch(target_rows_kernel<__bf16>);
+                if (M <= h->V) f16 ? launch(target_rows_kernel<_Float16, false>) : launch(target_rows_kernel<__bf16, false>);
+                else f16 ? launch(target_rows_kernel<_Float16, true>) : launch(target_rows_kernel<__bf16, true>);
             }
             const DwPlan parts = dw_plan(h, (long long)p.copies * p.Mp, nv);
             for (int i = 0, at = 0; i < 2 && parts.n[i]; at += parts.n[i++]) {
