@@ -200,3 +200,23 @@ def test_a_capture_while_the_layout_runs_is_refused():
         g.replay()
         torch.cuda.synchronize()
         same(out, want)
+
+
+@pytest.mark.gpu
+def test_streams_that_are_not_torchs_are_not_kept():
+    """Their owner may destroy them; a torch stream is there for good."""
+    import tsc_hip
+
+    x, W, b, t, dloss = make(100, 72, 1999, torch.float32, seed=66)
+    head = tsc_hip.UnembedHead(W, b)
+    want = run(x, W, b, t, dloss)
+    pooled = torch.cuda.Stream()
+    outside = torch.cuda.ExternalStream(torch.cuda.Stream().cuda_stream)
+    torch.cuda.synchronize()
+    for s, kept in ((torch.cuda.current_stream(), True), (pooled, True), (outside, False)):
+        with torch.cuda.stream(s):
+            same(run(x, W, b, t, dloss, head=head), want)
+        assert (s.cuda_stream in head._users) == kept
+    head.refresh()
+    assert not head._users
+    same(run(x, W, b, t, dloss, head=head), want)

@@ -909,6 +909,14 @@ def _launch(i: int, fn, *args) -> None:
         _check(rc)
 
 
+def _capturing(i: int) -> bool:
+    """Is the current stream of device ``i`` being captured."""
+    if torch._C._cuda_getDevice() == i:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(i):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _rows(t: torch.Tensor, name: str) -> _RowsStruct:
     """``tsc_rows_t`` of a ``[..., D]`` tensor: its last axis is dense, the leading ones step with at most two strides
     (``x[:, :-1]`` of a dense ``[B, T, D]``, a slice of one position, an expanded gradient)."""
@@ -1025,8 +1033,8 @@ class UnembedHead:
     replayed call look: call :meth:`refresh` after the change).
 
     Calls on several streams, also of several threads, may run at once.  A call waits for a layout that another stream is still
-    making, and a layout for the calls on other streams that came before it; what the caller orders is the change of the
-    tensors, as for any other reader of them.  A call that is captured while the layout still runs is refused, and so is making a head
+    making, and a layout for the calls on torch's other streams that came before it; what the caller orders is the change of the
+    tensors, as for any other reader of them, and a layout behind calls on a ``torch.cuda.ExternalStream``.  A call that is captured while the layout still runs is refused, and so is making a head
     inside a capture; a graph needs the heads that were captured into it for as long as it is replayed."""
 
     def __init__(self, W_U: torch.Tensor, b_U: Optional[torch.Tensor] = None):
@@ -1063,16 +1071,17 @@ class UnembedHead:
         """Lay the weights out again (``tsc_unembed_refresh``).  Captured into a graph it is part of every replay."""
         if not self._handle:
             raise TscError("this UnembedHead is closed")
-        with self._lock, torch.cuda.device(self.device):
-            captured = torch.cuda.is_current_stream_capturing()
+        i = self.device.index
+        with self._lock:
+            captured = _capturing(i)
             if not captured:
-                here = torch.cuda.current_stream()
-                for raw, stream in self._users.items():
-                    if raw != here.cuda_stream:
-                        here.wait_stream(stream)
+                here = torch._C._cuda_getCurrentRawStream(i)
+                others = [stream for raw, stream in self._users.items() if raw != here]
+                for stream in others:
+                    torch.cuda.current_stream(i).wait_stream(stream)
                 self._users.clear()
             versions = self._param_versions()
-            _launch(self.device.index, lib().tsc_unembed_refresh, self._handle)
+            _launch(i, lib().tsc_unembed_refresh, self._handle)
             if not captured:  # (a captured one has laid out nothing yet)
                 self._versions = versions
 
@@ -1089,10 +1098,10 @@ class UnembedHead:
                 self.refresh_if_modified()
             i = self.device.index
             raw = torch._C._cuda_getCurrentRawStream(i)
-            if raw not in self._users:
-                with torch.cuda.device(i):
-                    if not torch.cuda.is_current_stream_capturing():  # (replays are ordered by the caller)
-                        self._users[raw] = torch.cuda.current_stream()
+            if raw not in self._users and not _capturing(i):  # (replays are ordered by the caller)
+                stream = torch.cuda.current_stream(i)
+                if raw == 0 or stream.stream_id != raw:  # (one that is not torch's may be gone when it is to be waited for)
+                    self._users[raw] = stream
 
     def close(self) -> None:
         if self._handle:
