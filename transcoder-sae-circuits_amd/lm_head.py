@@ -161,6 +161,12 @@ def next_token_loss(normalized: torch.Tensor, tokens: torch.Tensor, head: "tsc_h
     return unembed_loss(normalized[:, :-1], tokens[:, 1:].contiguous(), head, reduction="none" if per_token else "mean")
 
 
+def _plain_head(model) -> bool:
+    """Are the model's logits ``hook_normalized @ W_U + b_U`` -- no weight of the final norm (not folded), no cap."""
+    return (getattr(getattr(model, "ln_final", None), "w", None) is None
+            and not (getattr(getattr(model, "cfg", None), "output_logits_soft_cap", None) or 0) > 0)
+
+
 def hooked_loss(model, tokens: torch.Tensor, fwd_hooks) -> torch.Tensor:
     """Mean next-token loss of a hooked model under ``fwd_hooks``: ``model.run_with_hooks(tokens, return_type="loss", ...)``, on a
     GPU from the final normalised residual (``ln_final.hook_normalized``) and :func:`model_head`, so that the model makes no
@@ -170,13 +176,12 @@ def hooked_loss(model, tokens: torch.Tensor, fwd_hooks) -> torch.Tensor:
     def own():
         return model.run_with_hooks(tokens, return_type="loss", fwd_hooks=fwd_hooks)
 
-    W, b, cfg = getattr(model, "W_U", None), getattr(model, "b_U", None), getattr(model, "cfg", None)
+    W, b = getattr(model, "W_U", None), getattr(model, "b_U", None)
     if not all(isinstance(t, torch.Tensor) for t in (W, b, tokens)) or not W.is_cuda or W.device != b.device or tokens.dim() > 2:
         return own()
     if W.dtype not in (torch.float32, torch.bfloat16, torch.float16) or b.dtype not in (W.dtype, torch.float32):
         return own()
-    if (getattr(getattr(model, "ln_final", None), "w", None) is not None or (getattr(cfg, "output_logits_soft_cap", None) or 0) > 0
-            or getattr(getattr(model, "tokenizer", None), "padding_side", None) == "left"
+    if (not _plain_head(model) or getattr(getattr(model, "tokenizer", None), "padding_side", None) == "left"
             or _FINAL not in getattr(model, "hook_dict", (_FINAL,))):
         return own()
     seen = []

@@ -90,6 +90,8 @@ class TaskEvaluation:
         """Every prompt's final residual at ``eval_index`` of its own length (as ``BatchedCircuitLens``: padding sits behind
         it), normalised, and its answer's last token."""
         model = self.model
+        if getattr(model.cfg, "normalization_type", "LNPre") != "LNPre" or not lm_head._plain_head(model):
+            raise NotImplementedError("the answer's loss is that of a model with a folded final layer norm and uncapped logits")
         if any(p["correct"] is None for p in self.prompts):
             raise ValueError("Prompt does not have correct token")
         name = f"blocks.{model.cfg.n_layers - 1}.hook_resid_post"
