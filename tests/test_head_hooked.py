@@ -106,3 +106,14 @@ def test_types_that_the_operator_does_not_take(monkeypatch):
     d = dictionaries(m.inner, monkeypatch)[0]
     d.get_test_loss(tok, m)
     assert m.asked == [None, "loss"]  # (its residual is of another type than its unembedding)
+
+
+@pytest.mark.gpu
+def test_the_loss_of_a_model_in_64_bits():
+    m = model_of(DEV, dtype=torch.float64)
+    tok = tokens_of(m)
+    logits, loss = m(tok, return_type="both")
+    want = torch.nn.functional.cross_entropy(logits[:, :-1].flatten(0, 1), tok[:, 1:].flatten())
+    assert loss.dtype == torch.float64 and abs(float(loss) - float(want)) < 1e-12
+    each = m(tok, return_type="loss", loss_per_token=True)
+    assert each.shape == (3, 8) and abs(float(each.mean()) - float(want)) < 1e-12

@@ -241,12 +241,14 @@ class SyntheticHookedTransformer(nn.Module):
         return self._forward(tokens, put, return_type, stop_at_layer, loss_per_token)
 
     def _loss(self, final: torch.Tensor, tokens: torch.Tensor, per_token: bool) -> torch.Tensor:
-        """Next-token cross entropy: without the ``[batch, n, d_vocab]`` logits on a GPU, plainly on the CPU."""
-        if final.is_cuda:
+        """Next-token cross entropy: without the ``[batch, n, d_vocab]`` logits on a GPU, plainly on the CPU and in a type that
+        the operator does not take."""
+        if final.is_cuda and final.dtype in (torch.float32, torch.bfloat16, torch.float16):
             from lm_head import model_head, next_token_loss
 
             return next_token_loss(final, tokens, model_head(self), per_token)
-        logits = (final[:, :-1] @ self.W_U + self.b_U).float()
+        logits = final[:, :-1] @ self.W_U + self.b_U
+        logits = logits if logits.dtype == torch.float64 else logits.float()
         loss = logits.logsumexp(-1) - logits.gather(-1, tokens[:, 1:, None])[..., 0]
         return loss if per_token else loss.mean()
 
