@@ -446,9 +446,9 @@ int tsc_layer_norm_backward(int elem, const tsc_rows_t *dy, const tsc_rows_t *x,
  * Stream order: one handle may be used from several streams.  tsc_unembed_create and tsc_unembed_refresh ENQUEUE the layout
  * on `stream` and return; a later call on another stream waits for it by itself (a captured one is refused with TSC_ERR_ARG
  * while it still runs: synchronize before the capture).  tsc_unembed_create inside a capture is refused (TSC_ERR_ARG); a
- * graph that calls were captured into needs the handle for as long as it is replayed.  What the caller orders is the change of W or bias, behind the calls
- * that still read them and before the refresh; and a refresh behind the calls on other streams that still use the handle.  A
- * refresh that was captured is ordered like the rest of its graph.
+ * graph that calls were captured into needs the handle for as long as it is replayed.  What the caller orders is the change of
+ * W or bias, behind the calls that still read them and before the refresh; and a refresh behind the calls on other streams
+ * that still use the handle.  A refresh that was captured is ordered like the rest of its graph.
  */
 typedef struct tsc_unembed tsc_unembed_t;
 int tsc_unembed_create(tsc_unembed_t **out, int d_model, int d_vocab, int elem, const void *W, int64_t stride_d,

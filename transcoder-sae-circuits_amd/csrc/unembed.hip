@@ -561,14 +561,16 @@ template <bool LANE> __global__ __launch_bounds__(256) void loss_kernel(const fl
 
 // What G's rounding took of the targets' entries, for dW: sums[slot[v]][d] = sum of left[m] x[m][d] over the rows m whose target
 // is v, for every one of the tokens v0 .. v1 - 1 that has a row; slot[v] is the first of them, or v itself (BY_TOKEN: of more
-// rows than tokens), and -1 where v has none.  A workgroup looks through the targets for those among its TOKENS tokens and keeps their rows in order, so that every
-// sum has a fixed order; where the list could overflow it is added up first, and the next one goes on from there.  A wave takes
-// the rows of a token one after the other, all waves together those of a token that has many, and join what they have.
-// Bound by latency (a target's way from memory, a row's, the sums' back).  Measured: 16384 rows x 768 of
-// 50257 tokens 47 us, 1999 x 1001 of 32003 11 us.
+// rows than tokens), and -1 where v has none.  A workgroup looks through the targets for those among its TOKENS tokens and keeps
+// their rows in order, so that every sum has a fixed order; where the list could overflow it is added up first, and the next one
+// goes on from there.  A wave takes the rows of a token one after the other, all waves together those of a token that has many,
+// and join what they have.
+// Bound by latency (a target's way from memory, a row's, the sums' back).  Measured: 16384 rows x 768 of 50257 tokens 47 us,
+// 1999 x 1001 of 32003 11 us.
 constexpr int TOKENS = 128, LIST = 4096, MANY = 32;
-template <class T, bool BY_TOKEN> __global__ __launch_bounds__(1024) void target_rows_kernel(const long long *targets, long long ignore, const float *left, const short *x,
-                                                                              long long ld, int M, int D, int v0, int v1, float *sums, int *slot) {
+template <class T, bool BY_TOKEN> __global__ __launch_bounds__(1024) void target_rows_kernel(const long long *targets, long long ignore, const float *left,
+                                                                                             const short *x, long long ld, int M, int D, int v0, int v1,
+                                                                                             float *sums, int *slot) {
     constexpr int WAVES = 16, PER = 4, STEP = PER * 1024;
     static_assert(LIST >= STEP, "a step's rows fit");
     __shared__ int row_of[LIST], first[TOKENS], many[TOKENS], before[PER * WAVES];

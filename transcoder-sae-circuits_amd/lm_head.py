@@ -142,7 +142,8 @@ def model_head(model) -> "tsc_hip.UnembedHead":
     """The :class:`tsc_hip.UnembedHead` of ``model.W_U`` and ``model.b_U``, laid out once for as long as the model keeps these
     tensors (a change in place lays it out again; inference tensors do not tell of one, so a model of them lays out for every
     call).  A capture needs one that is there already; a head that was asked for inside
-    a capture lives as long as the model, whatever tensors the model gets, because a graph may hold it."""
+    a capture lives as long as the model, whatever tensors the model gets, because a graph may hold it.  A change that no loss
+    has seen before the capture is laid out by every replay, which the caller then orders with losses on other streams."""
     key = tuple((t.data_ptr(), t.dtype, t.shape, t.stride()) for t in (model.W_U, model.b_U))
     entry = _heads.get(model)
     if entry is None or entry[0] != key:
